@@ -78,7 +78,7 @@ const char *smeg_version(void);
 int smeg_device_info(int *sm_count, size_t *hbm_bytes);
 /* Reads and clears the device status word (bit 0: a shared-memory barrier wait
  * gave up, bit 1: a tensor-memory pipeline wait gave up, bit 2: a peer wait gave
- * up).  Synchronises the device.  0 = no kernel ever abandoned a wait. */
+ * up, bit 3: a paged cache's table named no page of its pool).  Synchronises the device.  0 = none of these. */
 unsigned smeg_last_status(void);
 /* SME_GEMM_TRACE twin (src/warm.rs:115-179): when on (or env SMEG_TRACE=1) every
  * host-pointer entry prints "smeg: <kernel> MxNxK <us>" to stderr. */
@@ -276,6 +276,82 @@ int smeg_attn_kv_causal_dev(float *out, const void *q, int q_f32, size_t q_strid
 int smeg_attn_kv_causal_f16_dev(uint16_t *out, const void *q, int q_f32, size_t q_stride, const uint16_t *k,
                                 const uint16_t *v, size_t start, size_t rows, size_t heads, size_t kv_heads,
                                 size_t head_dim, float scale, void *stream);
+
+/* ---- packed batches of sequences: rotation, the 8-bit paged cache, attention --------------------------------------- */
+/* No counterpart in the reference (its SelfAttention applies no rotation, src/self_attention.rs:66-231, and its KvCache is one f16 buffer a
+ * sequence, src/kernels/kv_attention.rs:354-581): what a model with rotated, normalised heads and a server with many sequences need around the
+ * same two projections.
+ *
+ * A batch packs the rows of its sequences one behind the other: rows cu_rows[s] .. cu_rows[s + 1] (int32, device, seqs + 1 of them) are
+ * sequence s's; rows behind the last one are left as they are.  Rows are heads * head_dim 16-bit values (f16, or bf16 with bf16 = 1), stride
+ * elements apart.  starts[s] is the position of the sequence's first row, below zero for a sequence that is idle in this call; table[s *
+ * table_cols + i] is the pool's page that holds its positions i * page ... (int32, device).  Row offsets outside the batch are clamped;
+ * a position whose table entry names no page of the pool is skipped and raises bit 3 of smeg_last_status.
+ *
+ * The cache: codes uint8 [pages][kv_heads][keys, values][page][head_dim], scales f32 [pages][kv_heads][keys, values]; a value is (code - 128) *
+ * scale.  page: a power of two in 16..=256; head_dim a multiple of 16 in 16..=256.  Scale = largest magnitude / 127 over the positions that were
+ * appended since the page's first one; it starts over with that one and otherwise only grows, and codes that are there are then rounded
+ * again.  A block that received a NaN or an infinity has a NaN scale until its page starts over.  A page that is appended to belongs to
+ * one sequence; pages may be shared by the tables of any number of sequences that only read them. */
+typedef struct smeg_rotate_args {
+    const uint16_t *q, *k, *v;          /* q may be NULL; v NULL in smeg_rotate_heads_dev */
+    uint16_t *q_out, *k_out;            /* may be q and k themselves; k_out may be NULL in smeg_paged_append_dev */
+    size_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    const float *q_norm, *k_norm;       /* head_dim weights of the heads' RMS norms, or NULL */
+    const double *turns;                /* turns per position (frequency / 2 pi) of the rot / 2 rotated pairs, or NULL: no rotation */
+    float q_eps, k_eps, factor;         /* factor: on the cosines and sines */
+    int interleaved, bf16, reserved;    /* pairs (2 i, 2 i + 1) instead of (i, i + rot / 2) */
+    size_t rot, rows, heads, kv_heads, head_dim;
+    const int32_t *positions;           /* of each row, or NULL: start + row (smeg_rotate_heads_dev) */
+    int64_t start;
+    const int32_t *cu_rows, *starts, *table;
+    size_t seqs, table_cols;
+    uint8_t *codes;
+    float *scales;
+    size_t pages, page;
+} smeg_rotate_args;
+/* q_out = turn(norm(q)) and k_out = turn(norm(k)), one pass, one rounding: per head y = x / sqrt(mean(x^2) + q_eps) * q_norm, then the pair (a, b)
+ * becomes (a c - b s, b c + a s) with the cosine and sine of position * frequency, formed and reduced to a turn in 64 bits.  The batch and cache fields
+ * are not read.  head_dim a multiple of 8 in 8..=256, rot even and at most that. */
+int smeg_rotate_heads_dev(const smeg_rotate_args *a, void *stream);
+/* The same at the sequences' positions, with the keys (un-rounded) and values quantised into the cache on the way.  Rows of idle sequences are left
+ * as they are in q_out and k_out too. */
+int smeg_paged_append_dev(const smeg_rotate_args *a, void *stream);
+/* The values of n whole pages as 16-bit rows, out [n][kv_heads][keys, values][page][head_dim]; a page id outside the pool reads as zeros. */
+int smeg_paged_read_dev(uint16_t *out, const uint8_t *codes, const float *scales, const int32_t *ids, size_t n, size_t pages, size_t page,
+                        size_t kv_heads, size_t head_dim, int bf16, void *stream);
+
+/* Attention of a batch's rows against the cache, which already holds them: row i of sequence s attends to positions 0..=starts[s] + i; per
+ * head softmax(scale * q . k) @ v in 32 bits, one rounding.  Rows of idle sequences become zeros.  Query head h uses KV head h / (heads / kv_heads).
+ * workspace: smeg_paged_attend_workspace(...) bytes of device memory, 16-byte aligned, that nothing else uses until the call has run. */
+typedef struct smeg_paged_attend_args {
+    const uint16_t *q;
+    uint16_t *out;
+    size_t q_stride, out_stride;
+    const uint8_t *codes;
+    const float *scales;
+    const int32_t *cu_rows, *starts, *table;
+    size_t seqs, table_cols, pages, page, rows, heads, kv_heads, head_dim;
+    float scale;
+    int bf16;
+    void *workspace;
+    size_t workspace_bytes;
+} smeg_paged_attend_args;
+size_t smeg_paged_attend_workspace(size_t rows, size_t seqs, size_t table_cols, size_t page, size_t heads, size_t kv_heads, size_t head_dim);
+int smeg_paged_attend_dev(const smeg_paged_attend_args *a, void *stream);
+
+/* Causal attention over whole packed prompts, 16-bit keys and values: row i of a sequence attends to the sequence's rows 0..=i.  head_dim a
+ * multiple of 8 in 8..=256; any strides and starts, the tensor-core form for rows that start on 16-byte boundaries. */
+typedef struct smeg_attn_packed_args {
+    const uint16_t *q, *k, *v;
+    uint16_t *out;
+    size_t q_stride, k_stride, v_stride, out_stride;
+    const int32_t *cu_rows;
+    size_t seqs, rows, heads, kv_heads, head_dim;
+    float scale;
+    int bf16;
+} smeg_attn_packed_args;
+int smeg_attn_packed_dev(const smeg_attn_packed_args *a, void *stream);
 
 /* Mlp::gated (src/mlp.rs:80-92): gate_up is the 2*hidden-column interleaved
  * matrix GatedLinear::quantize builds (32 gate columns then 32 up columns,

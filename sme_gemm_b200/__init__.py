@@ -11,3 +11,4 @@ from .host import (  # noqa: F401
     matmul_q1, matmul_q1_ep, matmul_q1_mopa, matmul_q1_mopa_ep, matmul_q2, matmul_q2_ep, matmul_q2_mopa,
     matmul_q2_mopa_ep, matmul_q4, matmul_q4_bf16, matmul_q4_bf16_ep, matmul_q4_ep, prepack_bf16, prepack_f16,
 )
+from .paged import PagedBatch, PagedKvCache, Rotary, attend_packed, rotate_heads  # noqa: F401

@@ -50,6 +50,11 @@ class BlockArgs(C.Structure):
 # The same fields, packed by one call (0.3 us where filling a structure takes 1.6, of some 25 us of host work a layer at one row).
 BLOCK_ARGS = struct.Struct("@PNNPPPPffiiPPNNNPPNPPPfI")
 
+# smeg_rotate_args, smeg_paged_attend_args and smeg_attn_packed_args, packed the same way.
+ROTATE_ARGS = struct.Struct("@PPPPPNNNNNPPPfffiiiNNNNNPqPPPNNPPNN")
+PAGED_ATTEND_ARGS = struct.Struct("@PPNNPPPPPNNNNNNNNfiPN")
+ATTN_PACKED_ARGS = struct.Struct("@PPPPNNNNPNNNNNfi")
+
 assert BLOCK_ARGS.size == C.sizeof(BlockArgs) and BlockArgs.act.offset == BLOCK_ARGS.size - 4
 assert C.sizeof(EpNode) == 32 and EpNode.ptr.offset == 16 and EpNode.ld.offset == 24
 
@@ -127,6 +132,12 @@ SIGNATURES = {
     "smeg_kv_append_dev": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _vp]),
     "smeg_attn_kv_causal_dev": (_i, [_vp, _vp, _i, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, C.c_float, _vp]),
     "smeg_attn_kv_causal_f16_dev": (_i, [_vp, _vp, _i, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, C.c_float, _vp]),
+    "smeg_rotate_heads_dev": (_i, [_vp, _vp]),
+    "smeg_paged_append_dev": (_i, [_vp, _vp]),
+    "smeg_paged_read_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _i, _vp]),
+    "smeg_paged_attend_workspace": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz, _sz]),
+    "smeg_paged_attend_dev": (_i, [_vp, _vp]),
+    "smeg_attn_packed_dev": (_i, [_vp, _vp]),
     "smeg_mlp_finish_dev": (_i, [_vp, _vp, _sz, _vp]),
     "smeg_mlp_reduce_finish_dev": (_i, [_vp, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), _i, _i, _sz, _u32, _i, _vp]),
     "smeg_mlp_partial_push_dev": (_i, [_vp, _vp, C.POINTER(C.c_uint64), _i, _i, _sz, _vp]),

@@ -1313,6 +1313,123 @@ int smeg_attn_kv_causal_f16_dev(uint16_t* out, const void* q, int q_f32, size_t 
     return attn_dev(out, 1, q, q_f32, q_stride, k, v, start, rows, heads, kv_heads, head_dim, scale, stream);
 }
 
+// ---- packed batches: rotation, the 8-bit paged cache, attention ----
+static bool page_ok(size_t page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0; }
+static int log2_of(size_t page) {
+    int l = 0;
+    while ((size_t)1 << l < page) ++l;
+    return l;
+}
+// Sizes that the index arithmetic of paged.h is 32 bits wide for.
+static bool too_long(size_t rows, size_t heads, size_t kv_heads, size_t seqs, size_t cols, size_t page, size_t pages) {
+    if (kv_heads == 0 || page == 0) return true;
+    return rows > 0x7fffffffu / (heads / kv_heads) || heads > 65535 || seqs > 0xffffffu || cols > 0x7fffffffu / page || pages > 0x7fffffffu;
+}
+static int rotate_dev(const smeg_rotate_args* b, bool paged, cudaStream_t stream) {
+    if (!b) return -4;
+    if (b->rows == 0) return 0;
+    const size_t hd = b->head_dim, step = paged ? 16 : 8;
+    if (hd % step != 0 || hd < step || hd > 256 || b->rot % 2 != 0 || b->rot > hd || (b->turns && b->rot == 0)) return -4;
+    if (!b->q && !b->k) return -4;
+    if (b->q && (!b->q_out || b->heads == 0 || b->q_stride < b->heads * hd || b->q_out_stride < b->heads * hd)) return -4;
+    if (b->k && (b->kv_heads == 0 || b->k_stride < b->kv_heads * hd || (b->k_out && b->k_out_stride < b->kv_heads * hd))) return -4;
+    if (!paged && b->k && !b->k_out) return -4;
+    if (b->rows > 0x7fffffffu || b->heads > 65535 || b->kv_heads > 65535) return -3;
+    if (paged) {
+        if (!b->k || !b->v || !b->codes || !b->scales || !b->cu_rows || !b->starts || !b->table || !page_ok(b->page) || b->v_stride < b->kv_heads * hd) return -4;
+        if (((uintptr_t)b->codes & 15) != 0) return -4;
+        if (b->seqs == 0) return 0;
+        if (too_long(b->rows, b->kv_heads, b->kv_heads, b->seqs, b->table_cols, b->page, b->pages)) return -3;
+    }
+    DeviceState* ds = dev_state();
+    if (!ds) return -5;
+    RotateArgs a;
+    memset(&a, 0, sizeof(a));
+    a.q = b->q; a.k = b->k; a.q_out = b->q_out; a.k_out = b->k_out;
+    a.q_stride = b->q ? b->q_stride : 0; a.k_stride = b->k ? b->k_stride : 0; a.qo_stride = b->q ? b->q_out_stride : 0; a.ko_stride = b->k_out ? b->k_out_stride : 0;
+    a.q_w = b->q ? b->q_norm : nullptr; a.k_w = b->k ? b->k_norm : nullptr; a.q_eps = b->q_eps; a.k_eps = b->k_eps;
+    a.turns = b->turns; a.rot = b->turns ? (int)b->rot : 0; a.interleaved = b->interleaved != 0; a.factor = b->factor;
+    a.rows = (int)b->rows; a.heads = (int)b->heads; a.kv_heads = (int)b->kv_heads; a.head_dim = (int)hd; a.status = ds->status;
+    if (paged) {
+        a.v = b->v; a.v_stride = b->v_stride; a.codes = b->codes; a.scales = b->scales;
+        a.seqs = {b->cu_rows, b->starts, b->table, (int)b->seqs, (int)b->table_cols, (int)b->rows, (int)b->pages, log2_of(b->page)};
+    } else {
+        a.positions = b->positions; a.start = b->start;
+        if (!a.k) a.k_out = nullptr;
+    }
+    const cudaError_t e = rotate_append_launch(a, b->bf16 != 0, ds->sm_count, stream);
+    return e == cudaSuccess ? 0 : (e == cudaErrorInvalidValue ? -3 : -6);
+}
+int smeg_rotate_heads_dev(const smeg_rotate_args* a, void* stream) { return rotate_dev(a, false, (cudaStream_t)stream); }
+int smeg_paged_append_dev(const smeg_rotate_args* a, void* stream) { return rotate_dev(a, true, (cudaStream_t)stream); }
+int smeg_paged_read_dev(uint16_t* out, const uint8_t* codes, const float* scales, const int32_t* ids, size_t n, size_t pages, size_t page, size_t kv_heads,
+                        size_t head_dim, int bf16, void* stream) {
+    if (n == 0) return 0;
+    if (!out || !codes || !scales || !ids || !page_ok(page) || kv_heads == 0 || head_dim % 16 != 0 || head_dim < 16 || head_dim > 256 || ((uintptr_t)codes & 15) != 0) return -4;
+    if (kv_heads > 65535 || pages > 0x7fffffffu || n > 0x7fffffffu) return -3;
+    DeviceState* ds = dev_state();
+    if (!ds) return -5;
+    const cudaError_t e = paged_read_launch(out, codes, scales, ids, n, (int)pages, (int)page, (int)kv_heads, (int)head_dim, bf16 != 0, ds->status, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : (e == cudaErrorInvalidValue ? -3 : -6);
+}
+
+static bool heads_ok(size_t heads, size_t kv_heads, size_t hd, size_t step) {
+    return kv_heads != 0 && heads != 0 && heads % kv_heads == 0 && hd % step == 0 && hd >= step && hd <= 256;
+}
+static void attend_sizes(PagedAttendArgs& a, size_t rows, size_t seqs, size_t cols, size_t page, size_t pages, size_t heads, size_t kv_heads, size_t hd) {
+    memset(&a, 0, sizeof(a));
+    a.seqs.seqs = (int)seqs; a.seqs.cols = (int)cols; a.seqs.rows = (int)rows; a.seqs.pages = (int)pages; a.seqs.page_log2 = log2_of(page);
+    a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.head_dim = (int)hd;
+    a.max_rows = (int)((rows + seqs - 1) / seqs);
+}
+size_t smeg_paged_attend_workspace(size_t rows, size_t seqs, size_t table_cols, size_t page, size_t heads, size_t kv_heads, size_t head_dim) {
+    if (rows == 0 || seqs == 0 || !page_ok(page) || !heads_ok(heads, kv_heads, head_dim, 16) || too_long(rows, heads, kv_heads, seqs, table_cols, page, 0)) return 0;
+    DeviceState* ds = dev_state();
+    if (!ds) return 0;
+    PagedAttendArgs a;
+    attend_sizes(a, rows, seqs, table_cols, page, 0, heads, kv_heads, head_dim);
+    return paged_attend_ws_floats(a, ds->sm_count) * sizeof(float);
+}
+int smeg_paged_attend_dev(const smeg_paged_attend_args* b, void* stream) {
+    if (!b) return -4;
+    if (b->rows == 0 || b->seqs == 0) return 0;
+    if (!heads_ok(b->heads, b->kv_heads, b->head_dim, 16) || !page_ok(b->page)) return -4;
+    if (!b->q || !b->out || !b->codes || !b->scales || !b->cu_rows || !b->starts || !b->table || ((uintptr_t)b->codes & 15) != 0) return -4;
+    if (b->q_stride < b->heads * b->head_dim || b->out_stride < b->heads * b->head_dim) return -4;
+    if (too_long(b->rows, b->heads, b->kv_heads, b->seqs, b->table_cols, b->page, b->pages)) return -3;
+    DeviceState* ds = dev_state();
+    if (!ds) return -5;
+    PagedAttendArgs a;
+    attend_sizes(a, b->rows, b->seqs, b->table_cols, b->page, b->pages, b->heads, b->kv_heads, b->head_dim);
+    const size_t need = paged_attend_ws_floats(a, ds->sm_count) * sizeof(float);
+    if (need && (!b->workspace || b->workspace_bytes < need || ((uintptr_t)b->workspace & 15) != 0)) return -4;
+    a.q = b->q; a.out = b->out; a.q_stride = b->q_stride; a.out_stride = b->out_stride; a.codes = b->codes; a.scales = b->scales;
+    a.seqs.cu = b->cu_rows; a.seqs.starts = b->starts; a.seqs.table = b->table;
+    a.scale_log2e = b->scale * 1.4426950408889634f; a.ws = (float*)b->workspace; a.status = ds->status;
+    const cudaError_t e = paged_attend_launch(a, b->bf16 != 0, ds->sm_count, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : (e == cudaErrorInvalidValue ? -3 : -6);
+}
+
+int smeg_attn_packed_dev(const smeg_attn_packed_args* b, void* stream) {
+    if (!b) return -4;
+    if (b->rows == 0 || b->seqs == 0) return 0;
+    const size_t q_len = b->heads * b->head_dim, kv_len = b->kv_heads * b->head_dim;
+    if (!heads_ok(b->heads, b->kv_heads, b->head_dim, 8) || !b->q || !b->k || !b->v || !b->out || !b->cu_rows) return -4;
+    if (b->q_stride < q_len || b->out_stride < q_len || b->k_stride < kv_len || b->v_stride < kv_len) return -4;
+    if (too_long(b->rows, b->heads, b->kv_heads, b->seqs, 0, 16, 0)) return -3;
+    DeviceState* ds = dev_state();
+    if (!ds) return -5;
+    PromptArgs a;
+    memset(&a, 0, sizeof(a));
+    a.q = b->q; a.k = b->k; a.v = b->v; a.out = b->out;
+    a.q_stride = b->q_stride; a.k_stride = b->k_stride; a.v_stride = b->v_stride; a.out_stride = b->out_stride;
+    a.seqs.cu = b->cu_rows; a.seqs.seqs = (int)b->seqs; a.seqs.rows = (int)b->rows;
+    a.rows = (int)b->rows; a.heads = (int)b->heads; a.kv_heads = (int)b->kv_heads; a.head_dim = (int)b->head_dim; a.bf16 = b->bf16 != 0;
+    a.scale_log2e = b->scale * 1.4426950408889634f; a.status = ds->status;
+    const cudaError_t e = prompt_launch(a, ds->sm_count, (cudaStream_t)stream);
+    return e == cudaSuccess ? 0 : (e == cudaErrorInvalidValue ? -3 : -6);
+}
+
 int smeg_mlp_create(const smeg_q4* gate_up, const smeg_q4* down, uint32_t gate_act, smeg_mlp** out) {
     if (!out || !gate_up || !down) return -4;
     *out = nullptr;

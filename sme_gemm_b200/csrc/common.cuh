@@ -14,6 +14,7 @@ enum : unsigned {
     STATUS_MBAR_TIMEOUT = 1u,   // a shared-memory barrier never completed
     STATUS_TMEM_TIMEOUT = 2u,   // a tensor-memory pipeline barrier never completed
     STATUS_PEER_TIMEOUT = 4u,   // a peer flag never arrived (multi-GPU reduce)
+    STATUS_PAGE = 8u,           // a position of a paged cache whose table entry names no page of the pool (skipped)
 };
 
 // Wall-clock bound of one wait (nanoseconds of the global timer).  Never reached

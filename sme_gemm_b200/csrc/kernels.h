@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "epilogue.cuh"
+#include "paged.h"
 
 namespace smeg {
 
@@ -256,6 +257,59 @@ struct AttnArgs {
 cudaError_t attn_kv_causal_launch(AttnArgs a, int q_f32, int sm_count, cudaStream_t stream);
 cudaError_t kv_append_launch(uint16_t* kc, uint16_t* vc, const uint16_t* src, size_t stride, size_t k_off, size_t v_off, size_t row_len,
                              size_t pos, size_t rows, cudaStream_t stream);
+
+// ---- norms of heads, rotation by position, the append to an 8-bit paged cache (rotary.cu) ----
+struct RotateArgs {
+    const uint16_t *q, *k, *v;             // rows of heads, strides in elements; q null: no queries, v null: no cache
+    uint16_t *q_out, *k_out;
+    size_t q_stride, k_stride, v_stride, qo_stride, ko_stride;
+    const float *q_w, *k_w;                // weights of the heads' norms; null: none
+    float q_eps, k_eps;
+    const double* turns;                   // turns per position of each rotated pair; null: no rotation
+    int rot, interleaved;
+    float factor;                          // on the cosines and sines
+    const int* positions;                  // of the rows; null: start + row, or (with a batch) the sequences'
+    long long start;
+    int rows, heads, kv_heads, head_dim;
+    PackedSeqs seqs;                       // the batch and its pages; seqs.cu null: none
+    uint8_t* codes;                        // [page][KV head][keys | values][position][depth]
+    float* scales;                         // [page][KV head][keys | values]
+    unsigned* status;
+    int lanes, q_heads_here, k_heads_here, row_tile, head_tile, head_tiles, page_heads, page_units;      // launcher-filled
+};
+cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStream_t stream);
+cudaError_t paged_read_launch(uint16_t* out, const uint8_t* codes, const float* scales, const int* ids, size_t n, int pages, int page, int kv_heads, int head_dim,
+                              int bf16, unsigned* status, cudaStream_t stream);
+
+// ---- attention against the 8-bit paged cache (paged.cu) ----
+struct PagedAttendArgs {
+    const uint16_t* q;                     // rows of heads * head_dim
+    uint16_t* out;
+    size_t q_stride, out_stride;
+    const uint8_t* codes;
+    const float* scales;
+    PackedSeqs seqs;
+    int heads, kv_heads, head_dim;
+    int max_rows;                          // rows of a sequence to lay tiles out for (any number is right)
+    float scale_log2e;
+    float* ws;                             // paged_attend_ws_floats()
+    unsigned* status;
+    int q_vec, out_vec;                    // launcher-filled
+};
+size_t paged_attend_ws_floats(const PagedAttendArgs& a, int sm_count);
+cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaStream_t stream);
+
+// ---- causal attention over packed prompts (prompt.cu) ----
+struct PromptArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    size_t q_stride, k_stride, v_stride, out_stride;
+    PackedSeqs seqs;                       // cu, seqs, rows
+    int rows, heads, kv_heads, head_dim, bf16;
+    float scale_log2e;
+    unsigned* status;
+};
+cudaError_t prompt_launch(PromptArgs a, int sm_count, cudaStream_t stream);
 
 struct TpReduceArgs {
     float* bufs[8];        // every rank's buffer, peer-mapped into this process: len f32 partial sums, then len f16 results
