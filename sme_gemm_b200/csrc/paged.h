@@ -44,6 +44,10 @@ SMEG_HD long long pieces(long long n, long long d, int log2_len) {
 // sequences share a slot, and there are (total >> log2_len) + extra * seqs of them: the grid needs neither the lengths nor a prefix sum.
 SMEG_HD long long first_slot(long long first, int s, int log2_len, int extra) { return (first >> log2_len) + (long long)extra * s; }
 
+// The same for pieces of any length that start where their sequence does.
+SMEG_HD long long first_slot_of(long long first, int s, int len) { return first / len + s; }
+SMEG_HD long long pieces_of(long long n, int len) { return (n + len - 1) / len; }
+
 // The pool's page that holds position pos of sequence s; -1: none.
 SMEG_HD int page_of(const PackedSeqs& p, int s, long long pos) {
     const long long col = pos >> p.page_log2;

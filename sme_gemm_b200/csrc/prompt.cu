@@ -7,6 +7,9 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
+#include "tc_common.cuh"
+
+#include <string.h>
 
 namespace smeg {
 namespace {
@@ -246,6 +249,352 @@ __global__ void __launch_bounds__(kPwThreads) prompt_mma_kernel(const __grid_con
     }
 }
 
+// ---- heads of up to 128 depths, rows on 16-byte boundaries: tcgen05 ----
+constexpr int kPtThreads = 320;                    // warps 0-3 and 4-7: softmax of the two query tiles, 8: TMA, 9: MMA
+constexpr int kPtKeys = 128;
+constexpr int kPtChunk = 128 * 128;                // bytes of 128 rows x 64 depths
+constexpr int kPtMaxSlots = 10;
+constexpr uint32_t kPtO = 256;                     // tensor memory: scores / probabilities at columns 0 and 128, results behind them
+constexpr float kLazy = 8.0f;                      // a row's reference follows its maximum when that is 2^8 above it
+
+__device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr) {              // [key][64 depths]: 64 MN elements a row, as the values lie
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr >> 4) & 0x3fffu);
+    d |= (uint64_t)(kPtChunk >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pack64(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack64(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+struct PromptTc {
+    CUtensorMap q, k, v;
+    PromptArgs p;
+    int tokens;                                    // of a query tile: 128 / heads of a group
+    int slots;                                     // K / V ring
+    long long pieces;                              // work slots of a KV head
+};
+
+template <int BF16, int NCH>
+__global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptTc a) {
+    constexpr int kTile = NCH * kPtChunk;
+    const PromptArgs& p = a.p;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t bars[2 * kPtMaxSlots + 7];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int* abort_flag = &abort_word;
+    uint64_t *full = bars, *empty = full + kPtMaxSlots, *q_full = empty + kPtMaxSlots, *s_full = q_full + 1, *p_full = s_full + 2, *o_done = p_full + 2;
+    const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+    const int hd = p.head_dim, hd16 = (hd + 15) & ~15, group = p.heads / p.kv_heads, tt = a.tokens;
+    const int kvh = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    const long long slot_id = a.pieces - 1 - blockIdx.x / (unsigned)p.kv_heads;        // the pieces with the most keys first
+    pdl_wait();
+    int first = 0, rows = 0;
+    long long piece = 0;
+    {
+        int n = 0;
+        for (int s0 = 0; s0 < p.seqs.seqs; s0 += kPtThreads) {
+            const int s = s0 + tid;
+            int f = 0;
+            const bool at = s < p.seqs.seqs && (seq_rows(p.seqs, s, &f), first_slot_of(f, s, 2 * tt) <= slot_id);
+            n += __syncthreads_count(at);
+        }
+        if (n > 0) {
+            rows = seq_rows(p.seqs, n - 1, &first);
+            piece = slot_id - first_slot_of(first, n - 1, 2 * tt);
+        }
+        if (n == 0 || piece < 0 || piece >= pieces_of(rows, 2 * tt)) return;
+    }
+    const int tok0 = (int)(piece * 2 * tt);                        // tile x: the sequence's rows tok0 + x * tt ...
+    const int ntok[2] = {min(tt, rows - tok0), max(0, min(tt, rows - tok0 - tt))};
+    const int nblk[2] = {(tok0 + ntok[0] - 1) / kPtKeys + 1, ntok[1] ? (tok0 + tt + ntok[1] - 1) / kPtKeys + 1 : 0};
+    const int nmax = max(nblk[0], nblk[1]);
+    unsigned char *q_s = smem, *ring = smem + 2 * kTile;
+
+    if (tid == 0) {
+        abort_word = 0;
+        for (int i = 0; i < a.slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(q_full, 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+        fence_barrier_init();
+    }
+    if (warp == 9) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_launch_dependents();
+    const uint32_t tmem = tmem_slot;
+
+    if (warp == 8) {                                               // ---- loads ----
+        if (elect_one()) {
+            const int tiles = ntok[1] ? 2 : 1;
+            mbar_expect_tx(q_full, tiles * NCH * tt * group * 128);
+            for (int x = 0; x < tiles; ++x)
+                for (int c = 0; c < NCH; ++c) tma_4d(q_s + x * kTile + c * kPtChunk, &a.q, c * 64, 0, kvh, first + tok0 + x * tt, q_full);
+            int slot = 0, round = 0;
+            auto load = [&](const CUtensorMap* map, int j) {
+                if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, p.status)) return false;
+                mbar_expect_tx(&full[slot], kTile);
+                for (int c = 0; c < NCH; ++c) tma_3d(ring + (size_t)slot * kTile + c * kPtChunk, map, c * 64, kvh, first + j * kPtKeys, &full[slot]);
+                if (++slot == a.slots) { slot = 0; ++round; }
+                return true;
+            };
+            for (int j = 0; j < nmax; ++j)
+                if (!load(&a.k, j) || !load(&a.v, j)) break;
+        }
+        __syncwarp();
+    } else if (warp == 9) {                                        // ---- products ----
+        const uint32_t idesc_s = umma_idesc(BF16, 128, kPtKeys), idesc_o = umma_idesc(BF16, 128, hd16) | (1u << 16);
+        const int ksteps = hd16 >> 4;
+        const uint32_t q_a = smem_u32(q_s), ring_a = smem_u32(ring);
+        int slot = 0, par = 0;
+        bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag, p.status));
+        auto take = [&](uint32_t& addr, int& at) {
+            at = slot;
+            addr = ring_a + (uint32_t)slot * kTile;
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[slot], par, abort_flag, p.status));
+            if (++slot == a.slots) { slot = 0; par ^= 1; }
+            tc_fence_after();
+        };
+        auto scores = [&](int x, uint32_t k_addr) {
+            if (elect_one()) {
+                for (int s = 0; s < ksteps; ++s) {
+                    const uint32_t off = (uint32_t)((s >> 2) * kPtChunk + (s & 3) * 32);
+                    umma_f16(tmem + 128 * x, umma_desc_sw128(q_a + x * kTile + off), umma_desc_sw128(k_addr + off), idesc_s, s > 0);
+                }
+                umma_commit(&s_full[x]);
+            }
+            __syncwarp();
+        };
+        uint32_t k_addr = 0, v_addr = 0;
+        int k_slot = 0, v_slot = 0;
+        if (ok) take(k_addr, k_slot);
+        if (ok) {
+            scores(0, k_addr);
+            if (nblk[1]) scores(1, k_addr);
+            if (elect_one()) umma_commit(&empty[k_slot]);
+            __syncwarp();
+        }
+        for (int j = 0; ok && j < nmax; ++j) {
+            take(v_addr, v_slot);
+            const bool more = j + 1 < nmax;
+            if (ok && more) take(k_addr, k_slot);
+            for (int x = 0; ok && x < 2; ++x) {
+                if (j >= nblk[x]) continue;
+                ok = __all_sync(0xffffffffu, mbar_wait_poll(&p_full[x], j & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    for (int s = 0; s < kPtKeys / 16; ++s)
+                        umma_f16_ts(tmem + kPtO + 128 * x, tmem + 128 * x + 8 * s, desc_mn(v_addr + s * 2048), idesc_o, j > 0 || s > 0);
+                    if (j + 1 == nblk[x]) umma_commit(&o_done[x]);
+                }
+                __syncwarp();
+                if (j + 1 < nblk[x]) scores(x, k_addr);
+            }
+            if (ok && elect_one()) {
+                umma_commit(&empty[v_slot]);
+                if (more) umma_commit(&empty[k_slot]);
+            }
+            __syncwarp();
+        }
+    } else {                                                       // ---- softmax ----
+        const int x = warp >> 2, row = (warp & 3) * 32 + lane;
+        const int t = row / group, tok = tok0 + x * tt + min(t, ntok[x] - 1), n = nblk[x], head = kvh * group + row - t * group;
+        const bool in = t < ntok[x];
+        const int low = tok0 + x * tt;                             // the tile's first row
+        const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * x, to = ts - 128 * x + kPtO + 128 * x;
+        const float sc = p.scale_log2e;
+        float m = -kInf, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait_poll(&s_full[x], j & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+            tmem_ld_wait();
+            const int key0 = j * kPtKeys;
+            if (key0 + kPtKeys - 1 > low) {                        // keys behind some row's own
+                const int lim = tok - key0;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[c][i] = 32 * c + i <= lim ? s[c][i] : 0xff800000u;
+            }
+            float mx[4] = {m, m, m, m};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+            const float now = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+            const bool far = j == 0 ? true : (now - m) * sc > kLazy;              // (from -inf: inf; -inf to -inf: NaN, no)
+            if (j == 0) {
+                m = now;
+            } else if (__any_sync(0xffffffffu, far)) {
+                const float f = far ? ex2((m - now) * sc) : 1.0f;
+                if (far) m = now;
+                l *= f;
+                const uint64_t f2 = pack64(f, f);
+                for (int c = 0; c < hd16; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(to + c, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float u, v;
+                        unpack64(mul2(pack64(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), f2), u, v);
+                        o[i] = __float_as_uint(u);
+                        o[i + 1] = __float_as_uint(v);
+                    }
+                    tmem_st16(to + c, o);
+                }
+            }
+            const float ref = m == -kInf ? 0.0f : m * sc;
+            const uint64_t sc2 = pack64(sc, sc), ref2 = pack64(-ref, -ref);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    float u, v;
+                    unpack64(fma2(pack64(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, ref2), u, v);
+                    u = ex2(u);
+                    v = ex2(v);
+                    sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack64(u, v));
+                    w[i / 2] = pack2_t<BF16>(u, v);
+                }
+                tmem_st16(ts + 16 * c, w);
+            }
+            tmem_st_wait();
+            float u, v;
+            unpack64(add2(sum[0], sum[1]), u, v);
+            l += u + v;
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[x]);
+        }
+        if (n > 0) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&o_done[x], 0, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+            tc_fence_after();
+            const float inv = __fdiv_rn(1.0f, l);
+            uint16_t* dst = p.out + (size_t)(first + tok) * p.out_stride + (size_t)head * hd;
+            bool bad = false;
+            const bool vec = (((uintptr_t)p.out | (p.out_stride * 2)) & 15) == 0;
+            for (int c = 0; ok && c < hd16; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(to + c, o);
+                tmem_ld_wait();
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float u = __uint_as_float(o[i]) * inv, v = __uint_as_float(o[i + 1]) * inv;
+                    bad = bad || !(fabsf(u) <= 3.402823466e38f) || !(fabsf(v) <= 3.402823466e38f);
+                    w[i / 2] = pack2_t<BF16>(u, v);
+                }
+                if (!in) continue;
+                if (vec) {
+                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (c + 8 < hd) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (c + i < hd) dst[c + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+                }
+            }
+            unsigned mask = __ballot_sync(0xffffffffu, ok && in && bad && l > 0.0f);
+            if (mask && any_bad_value(p, kvh, first + low + 1, min(first + n * kPtKeys, p.rows)))
+                for (; mask; mask &= mask - 1) {
+                    const int r = __ffs(mask) - 1, tk = __shfl_sync(0xffffffffu, tok, r), h = __shfl_sync(0xffffffffu, head, r);
+                    __syncwarp();
+                    exact_row<BF16>(p, first, first + tk, h);
+                }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int BF16, int NCH>
+cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
+    *taken = false;
+    TensorMapEncodeFn enc = tensor_map_encoder();
+    const int group = p.heads / p.kv_heads;
+    if (!enc || group > 128) return cudaSuccess;
+    PromptTc a;
+    memset(&a, 0, sizeof(a));
+    a.p = p;
+    a.tokens = 128 / group;
+    a.slots = (int)((227 * 1024 - 2048 - 2 * NCH * kPtChunk) / (NCH * kPtChunk));
+    if (a.slots > kPtMaxSlots) a.slots = kPtMaxSlots;
+    a.pieces = p.rows / (2 * a.tokens) + (long long)p.seqs.seqs;
+    if (a.pieces * p.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;
+    const CUtensorMapDataType type = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t hd = (cuuint64_t)p.head_dim;
+    const cuuint64_t qd[4] = {hd, (cuuint64_t)group, (cuuint64_t)p.kv_heads, (cuuint64_t)p.rows}, qs[3] = {hd * 2, hd * 2 * group, (cuuint64_t)p.q_stride * 2};
+    const cuuint32_t qb[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)a.tokens}, ones[4] = {1, 1, 1, 1};
+    if (enc(&a.q, type, 4, (void*)p.q, qd, qs, qb, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return cudaSuccess;
+    const cuuint64_t kd[3] = {hd, (cuuint64_t)p.kv_heads, (cuuint64_t)p.rows}, ks[2] = {hd * 2, (cuuint64_t)p.k_stride * 2}, vs[2] = {hd * 2, (cuuint64_t)p.v_stride * 2};
+    const cuuint32_t kb[3] = {64, 1, (cuuint32_t)kPtKeys};
+    if (enc(&a.k, type, 3, (void*)p.k, kd, ks, kb, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS ||
+        enc(&a.v, type, 3, (void*)p.v, kd, vs, kb, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaSuccess;
+    auto kern = prompt_tc_kernel<BF16, NCH>;
+    const size_t smem = 1024 + (size_t)(2 + a.slots) * NCH * kPtChunk;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    *taken = true;
+    return launch_pdl(kern, dim3((unsigned)(a.pieces * p.kv_heads)), dim3(kPtThreads), smem, stream, a);
+}
+
 template <int BF16, int HD>
 cudaError_t mma_launch(const PromptArgs& a, cudaStream_t stream) {
     auto kern = prompt_mma_kernel<BF16, HD>;
@@ -263,6 +612,16 @@ cudaError_t mma_launch(const PromptArgs& a, cudaStream_t stream) {
 
 cudaError_t prompt_launch(PromptArgs a, int sm_count, cudaStream_t stream) {
     if (a.rows == 0 || a.seqs.seqs == 0) return cudaSuccess;
+    // rows and heads on 16-byte boundaries (what a tensor map needs), strides that it can hold, a positive scale (the maximum is taken before it)
+    const bool aligned = ((a.q_stride | a.k_stride | a.v_stride) & 7) == 0 && (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0 &&
+                         ((a.q_stride | a.k_stride | a.v_stride) >> 38) == 0;
+    if (aligned && a.head_dim <= 128 && a.scale_log2e > 0.0f && a.scale_log2e < 1e30f) {
+        bool taken = false;
+        cudaError_t e;
+        if (a.bf16) e = a.head_dim <= 64 ? tc_launch<1, 1>(a, stream, &taken) : tc_launch<1, 2>(a, stream, &taken);
+        else e = a.head_dim <= 64 ? tc_launch<0, 1>(a, stream, &taken) : tc_launch<0, 2>(a, stream, &taken);
+        if (taken || e != cudaSuccess) return e;
+    }
     if (a.bf16) return a.head_dim <= 64 ? mma_launch<1, 64>(a, stream) : (a.head_dim <= 128 ? mma_launch<1, 128>(a, stream) : mma_launch<1, 256>(a, stream));
     return a.head_dim <= 64 ? mma_launch<0, 64>(a, stream) : (a.head_dim <= 128 ? mma_launch<0, 128>(a, stream) : mma_launch<0, 256>(a, stream));
 }

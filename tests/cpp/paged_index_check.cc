@@ -118,6 +118,24 @@ int main(int argc, char** argv) {
                 for (int s = 0; s < seqs; ++s)
                     for (int r = b.cu[s] * g; r < b.cu[s + 1] * g; ++r) REQUIRE(seen[r] == (extra == 2 && b.starts[s] < 0 ? 0 : 1));
         }
+        {                                                          // pieces of any length
+            const int len = (int)pick(1, 300);
+            std::vector<int> seen((size_t)rows + 1, 0);
+            for (long long j = 0; j < rows / len + b.p.seqs; ++j) {
+                int n = 0, first = 0;
+                for (int s = 0; s < b.p.seqs; ++s) n += (seq_rows(b.p, s, &first), first_slot_of(first, s, len) <= j);
+                if (!n) continue;
+                const int mine = seq_rows(b.p, n - 1, &first);
+                const long long piece = j - first_slot_of(first, n - 1, len);
+                if (piece < 0 || piece >= pieces_of(mine, len)) continue;
+                for (long long r = piece * len; r < std::min<long long>(mine, (piece + 1) * len); ++r) {
+                    REQUIRE(first + r >= 0 && first + r < rows);
+                    seen[first + r]++;
+                }
+            }
+            if (sound)
+                for (int r = 0; r < b.cu[seqs]; ++r) REQUIRE(seen[r] == 1);
+        }
         for (int tile : {8, 16})
             if (shares(b, group, (int)pick(1, 5), tile, (int)pick(1, 500))) return 1;
     }
