@@ -21,7 +21,7 @@ _DTYPES = (torch.float16, torch.bfloat16)
 class _On:
     """The tensors' device as the current one, for a call from elsewhere."""
 
-    def __init__(self, device):
+    def __init__(self, device: int):
         self._device = device
 
     def __enter__(self):
@@ -46,36 +46,48 @@ def _enqueue(name: str, device: int, args: bytes) -> None:
         check(name, rc)
 
 
-def _rows(x, what: str, width: int, like=None):
-    """Checks a tensor of rows; its row stride in elements."""
+def _first_rows(x, what: str):
+    """(type, device index, number) of the rows that the other tensors of a call have to be like."""
+    assert isinstance(x, torch.Tensor) and x.is_cuda, f"{what} is a CUDA tensor"
+    assert x.dtype in _DTYPES, f"{what} is f16 or bf16"
+    assert x.dim() == 2, f"{what} has rows"
+    return x.dtype, x.get_device(), x.shape[0]
+
+
+def _rows(x, what: str, width: int, like) -> int:
+    """Checks a tensor of rows; their stride in elements.  (A call is some eight of these checks, and a small one is over in the time they take: the
+    sound case is one condition, what is wrong is found afterwards.)"""
+    dtype, device, rows = like
+    if type(x) is torch.Tensor and x.dtype is dtype and x.get_device() == device and x.shape == (rows, width):
+        stride, one = x.stride()
+        if one == 1 and stride >= width:
+            return stride
+        if rows <= 1 and (one == 1 or width == 1):
+            return width
     assert isinstance(x, torch.Tensor) and x.is_cuda, f"{what} is a CUDA tensor"
     assert x.dtype in _DTYPES, f"{what} is f16 or bf16"
     assert x.dim() == 2 and x.shape[1] == width, f"{what} has rows of {width} values"
-    rows = x.shape[0]
-    stride = x.stride(0)
-    if rows > 1:
-        assert x.stride(1) == 1 and stride >= width, f"{what} has its rows' values side by side"
-    else:
-        assert width == 1 or x.stride(1) == 1, f"{what} has its rows' values side by side"
-        stride = width
-    if like is not None:
-        assert x.dtype == like.dtype and x.device == like.device, f"{what} has the same type and device as the other rows"
-        assert rows == like.shape[0], f"{what} has as many rows as the others"
-    return stride
+    assert x.dtype is dtype and x.get_device() == device, f"{what} has the same type and device as the other rows"
+    assert x.shape[0] == rows, f"{what} has as many rows as the others"
+    stride, one = x.stride()
+    assert rows <= 1 or stride >= width and one == 1 or width == 1, f"{what} has its rows' values side by side"
+    assert one == 1 or width == 1 or rows == 0, f"{what} has its rows' values side by side"
+    return max(stride, width)
 
 
-def _ints(x, what: str, device) -> None:
-    assert isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.int32 and x.is_contiguous(), f"{what} is a contiguous int32 CUDA tensor"
-    assert device is None or x.device == device, f"{what} is on the rows' device"
+def _ints(x, what: str, device: int) -> None:
+    assert isinstance(x, torch.Tensor) and x.is_cuda and x.dtype is torch.int32 and x.is_contiguous(), f"{what} is a contiguous int32 CUDA tensor"
+    assert device is None or x.get_device() == device, f"{what} is on the rows' device"
 
 
-def _head_norm(norm, what: str, head_dim: int, device):
+def _head_norm(norm, what: str, head_dim: int, device: int):
     if norm is None:
         return 0, 0.0
     assert isinstance(norm, Norm) and norm.is_rms, f"{what} is an RMS norm"
-    assert norm.width() == head_dim, f"{what} has head_dim weights"
-    assert norm.weight.device == device, f"{what} is on the rows' device"
-    return norm.weight.data_ptr(), norm.eps
+    w = norm.weight
+    assert w.numel() == head_dim, f"{what} has head_dim weights"
+    assert w.get_device() == device, f"{what} is on the rows' device"
+    return w.data_ptr(), norm.eps
 
 
 class Rotary:
@@ -93,7 +105,7 @@ class Rotary:
 
     def _set(self, frequencies, factor: float) -> None:
         self._frequencies, self._factor = frequencies, float(factor)
-        self._turns = {}                                       # device -> turns per position
+        self._turns = {}                                       # device -> turns per position, and where they are
 
     def _scaled(self, frequencies, factor: float = 1.0) -> "Rotary":
         r = Rotary(self._head_dim, self._base, self._rot, self._interleaved)
@@ -143,19 +155,20 @@ class Rotary:
         """On the cosines and sines."""
         return self._factor
 
-    def turns(self, device):
-        """The frequencies as turns per position, on `device` (kept from the first call on: before a capture, then)."""
+    def turns(self, device: int):
+        """(turns per position of each pair, f64 on the device; their address).  Made by the first call on a device: before a capture, then."""
         t = self._turns.get(device)
         if t is None:
-            t = self._turns[device] = torch.tensor(self._frequencies / (2.0 * math.pi), dtype=torch.float64, device=device)
+            x = torch.tensor(self._frequencies / (2.0 * math.pi), dtype=torch.float64, device=torch.device("cuda", device))
+            t = self._turns[device] = x, x.data_ptr()
         return t
 
 
-def _rotation(rotary, head_dim: int, device):
+def _rotation(rotary, head_dim: int, device: int):
     if rotary is None:
         return 0, 0, 0, 1.0
     assert isinstance(rotary, Rotary) and rotary._head_dim == head_dim, "the rotation is one of heads of head_dim"
-    return rotary.turns(device).data_ptr(), rotary._rot, int(rotary._interleaved), rotary._factor
+    return rotary.turns(device)[1], rotary._rot, rotary._interleaved, rotary._factor
 
 
 def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=None, head_dim: int | None = None) -> None:
@@ -166,17 +179,24 @@ def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=N
     hd = rotary._head_dim if rotary is not None else head_dim
     assert head_dim is None or head_dim == hd, "the rotation is one of heads of head_dim"
     assert hd % 8 == 0 and 8 <= hd <= 256, "head_dim must be a multiple of 8 in 8..=256"
-    one = q if q is not None else k
-    assert one is not None, "there are queries or keys"
-    ptr, stride, heads = [0, 0, 0, 0], [0, 0, 0, 0], [0, 0]
-    for i, (x, out, what) in enumerate(((q, q_out, "q"), (k, k_out, "k"))):
-        assert (x is None) == (out is None), f"{what} and {what}_out come together"
-        if x is None:
-            continue
-        assert x.dim() == 2 and x.shape[1] % hd == 0 and x.shape[1] > 0, f"{what} has rows of whole heads"
-        stride[i], stride[2 + i] = _rows(x, what, x.shape[1], one), _rows(out, what + "_out", x.shape[1], one)
-        ptr[i], ptr[2 + i], heads[i] = x.data_ptr(), out.data_ptr(), x.shape[1] // hd
-    rows, device = one.shape[0], one.device
+    assert q is not None or k is not None, "there are queries or keys"
+    assert (q is None) == (q_out is None), "q and q_out come together"
+    assert (k is None) == (k_out is None), "k and k_out come together"
+    like = dtype, device, rows = _first_rows(q, "q") if q is not None else _first_rows(k, "k")
+    q_ptr = k_ptr = qo_ptr = ko_ptr = qs = ks = qos = kos = heads = kv_heads = 0
+    if q is not None:
+        width = q.shape[1]
+        heads = width // hd
+        assert heads * hd == width and heads > 0, "q has rows of whole heads"
+        qs, qos = _rows(q, "q", width, like), _rows(q_out, "q_out", width, like)
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        _first_rows(k, "k")
+        width = k.shape[1]
+        kv_heads = width // hd
+        assert kv_heads * hd == width and kv_heads > 0, "k has rows of whole heads"
+        ks, kos = _rows(k, "k", width, like), _rows(k_out, "k_out", width, like)
+        k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
     pos_ptr, start = 0, 0
     if isinstance(positions, torch.Tensor):
         _ints(positions, "positions", device)
@@ -189,9 +209,9 @@ def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=N
     kn, ke = _head_norm(k_norm, "k_norm", hd, device)
     if rows == 0:
         return
-    _enqueue("smeg_rotate_heads_dev", device.index, ROTATE_ARGS.pack(
-        ptr[0], ptr[1], 0, ptr[2], ptr[3], stride[0], stride[1], 0, stride[2], stride[3], qn, kn, turns, qe, ke, factor, inter,
-        one.dtype == torch.bfloat16, 0, rot, rows, heads[0], heads[1], hd, pos_ptr, start, 0, 0, 0, 0, 0, 0, 0, 0, 0))
+    _enqueue("smeg_rotate_heads_dev", device, ROTATE_ARGS.pack(
+        q_ptr, k_ptr, 0, qo_ptr, ko_ptr, qs, ks, 0, qos, kos, qn, kn, turns, qe, ke, factor, inter, dtype is torch.bfloat16, 0, rot, rows, heads, kv_heads, hd,
+        pos_ptr, start, 0, 0, 0, 0, 0, 0, 0, 0, 0))
 
 
 class PagedBatch:
@@ -201,18 +221,29 @@ class PagedBatch:
 
     def __init__(self, cu_rows, starts, table):
         _ints(starts, "starts", None)
-        _ints(cu_rows, "cu_rows", starts.device)
-        _ints(table, "table", starts.device)
+        _ints(cu_rows, "cu_rows", starts.get_device())
+        _ints(table, "table", starts.get_device())
         n = starts.numel()
         assert cu_rows.numel() == n + 1, "cu_rows has one value more than there are sequences"
         assert table.dim() == 2 and table.shape[0] == n, "table has a row of pages for each sequence"
-        self.cu_rows, self.starts, self.table = cu_rows, starts, table
+        self._tensors = cu_rows, starts, table
+        self._device = starts.get_device()
+        self._fields = cu_rows.data_ptr(), starts.data_ptr(), table.data_ptr(), n, table.shape[1]
+
+    @property
+    def cu_rows(self):
+        return self._tensors[0]
+
+    @property
+    def starts(self):
+        return self._tensors[1]
+
+    @property
+    def table(self):
+        return self._tensors[2]
 
     def seqs(self) -> int:
-        return self.starts.numel()
-
-    def _fields(self):
-        return self.cu_rows.data_ptr(), self.starts.data_ptr(), self.table.data_ptr(), self.starts.numel(), self.table.shape[1]
+        return self._fields[3]
 
 
 class PagedKvCache:
@@ -229,11 +260,20 @@ class PagedKvCache:
         assert pages >= 0, "pages is a number of pages"
         self._heads, self._kv_heads, self._head_dim, self._pages, self._page = heads, kv_heads, head_dim, pages, page
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        self.codes = torch.full((max(pages, 1), kv_heads, 2, page, head_dim), 128, dtype=torch.uint8, device=device)
-        self.scales = torch.zeros((max(pages, 1), kv_heads, 2), dtype=torch.float32, device=device)
-        self._device = self.codes.device
+        self._codes = torch.full((max(pages, 1), kv_heads, 2, page, head_dim), 128, dtype=torch.uint8, device=device)
+        self._scales = torch.zeros((max(pages, 1), kv_heads, 2), dtype=torch.float32, device=device)
+        self._device = self._codes.get_device()
+        self._at = self._codes.data_ptr(), self._scales.data_ptr()
         self._scale = float(np.float32(1.0) / np.sqrt(np.float32(head_dim)))
         self._ws_bytes = {}
+
+    @property
+    def codes(self):
+        return self._codes
+
+    @property
+    def scales(self):
+        return self._scales
 
     def with_scale(self, scale: float) -> "PagedKvCache":
         self._scale = float(np.float32(scale))
@@ -263,68 +303,76 @@ class PagedKvCache:
     def query_len(self) -> int:
         return self._heads * self._head_dim
 
-    def _mine(self, x, batch) -> None:
-        assert x.device == self._device, "the rows are on the cache's device"
-        assert isinstance(batch, PagedBatch) and batch.starts.device == self._device, "the batch is on the cache's device"
+    def _like(self, x, what: str, batch):
+        like = _first_rows(x, what)
+        assert like[1] == self._device, "the rows are on the cache's device"
+        assert isinstance(batch, PagedBatch) and batch._device == self._device, "the batch is on the cache's device"
+        return like
 
     def append(self, k, v, batch: PagedBatch, rotary: Rotary | None = None, *, k_norm=None, k_out=None, q=None, q_out=None, q_norm=None) -> None:
         """The rows k and v (kv_heads * head_dim values) to the pages of their sequences' positions; keys are normalised (k_norm) and rotated on the way.
         k_out: the keys so treated as 16-bit rows as well.  q, q_out: the queries, normalised (q_norm) and rotated, in the same pass.  The outputs
         may be the inputs.  Rows of idle sequences and rows behind the last sequence are left as they are."""
-        row, hd = self.row_len(), self._head_dim
-        ks, vs = _rows(k, "k", row), _rows(v, "v", row, k)
-        self._mine(k, batch)
-        kos = _rows(k_out, "k_out", row, k) if k_out is not None else 0
+        hd = self._head_dim
+        row, device = self._kv_heads * hd, self._device
+        like = self._like(k, "k", batch)
+        ks, vs = _rows(k, "k", row, like), _rows(v, "v", row, like)
+        q_ptr = qo_ptr = ko_ptr = qs = qos = kos = 0
+        if k_out is not None:
+            kos, ko_ptr = _rows(k_out, "k_out", row, like), k_out.data_ptr()
         assert (q is None) == (q_out is None), "q and q_out come together"
-        qs = qos = 0
         if q is not None:
-            qs, qos = _rows(q, "q", self.query_len(), k), _rows(q_out, "q_out", self.query_len(), k)
-        turns, rot, inter, factor = _rotation(rotary, hd, self._device)
-        qn, qe = _head_norm(q_norm, "q_norm", hd, self._device)
-        kn, ke = _head_norm(k_norm, "k_norm", hd, self._device)
-        cu, starts, table, seqs, cols = batch._fields()
-        if k.shape[0] == 0 or seqs == 0:
+            q_len = self._heads * hd
+            qs, qos = _rows(q, "q", q_len, like), _rows(q_out, "q_out", q_len, like)
+            q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+        turns, rot, inter, factor = _rotation(rotary, hd, device)
+        qn, qe = _head_norm(q_norm, "q_norm", hd, device)
+        kn, ke = _head_norm(k_norm, "k_norm", hd, device)
+        if like[2] == 0 or batch._fields[3] == 0:
             return
-        _enqueue("smeg_paged_append_dev", self._device.index, ROTATE_ARGS.pack(
-            q.data_ptr() if q is not None else 0, k.data_ptr(), v.data_ptr(), q_out.data_ptr() if q is not None else 0,
-            k_out.data_ptr() if k_out is not None else 0, qs, ks, vs, qos, kos, qn, kn, turns, qe, ke, factor, inter, k.dtype == torch.bfloat16, 0,
-            rot, k.shape[0], self._heads, self._kv_heads, hd, 0, 0, cu, starts, table, seqs, cols, self.codes.data_ptr(), self.scales.data_ptr(),
-            self._pages, self._page))
+        _enqueue("smeg_paged_append_dev", device, ROTATE_ARGS.pack(
+            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, qs, ks, vs, qos, kos, qn, kn, turns, qe, ke, factor, inter, like[0] is torch.bfloat16, 0, rot,
+            like[2], self._heads, self._kv_heads, hd, 0, 0, *batch._fields, *self._at, self._pages, self._page))
 
     def attend(self, q, batch: PagedBatch, out) -> None:
         """out = the attention of the query rows (heads * head_dim values) against their sequences' cached positions, which already hold the rows' own
         (append, then attend, with the same batch): row i of a sequence attends to positions 0..=start + i.  Rows of idle sequences become
         zeros, rows behind the last sequence stay as they are."""
-        qs, os_ = _rows(q, "q", self.query_len()), _rows(out, "out", self.query_len(), q)
-        self._mine(q, batch)
-        cu, starts, table, seqs, cols = batch._fields()
-        rows = q.shape[0]
+        like = dtype, device, rows = self._like(q, "q", batch)
+        width = self._heads * self._head_dim
+        qs, os_ = _rows(q, "q", width, like), _rows(out, "out", width, like)
+        cu, starts, table, seqs, cols = batch._fields
         if rows == 0 or seqs == 0:
             return
-        size = (rows, seqs, cols)
+        size = rows, seqs, cols
         need = self._ws_bytes.get(size)
         if need is None:
-            with _On(self._device.index):
+            with _On(device):
                 need = lib().smeg_paged_attend_workspace(rows, seqs, cols, self._page, self._heads, self._kv_heads, self._head_dim)
             self._ws_bytes[size] = need
         # the call's own memory, from the stream's pool: two streams, or two captured graphs, never share it
-        ws = torch.empty(need, dtype=torch.uint8, device=self._device) if need else None
-        _enqueue("smeg_paged_attend_dev", self._device.index, PAGED_ATTEND_ARGS.pack(
-            q.data_ptr(), out.data_ptr(), qs, os_, self.codes.data_ptr(), self.scales.data_ptr(), cu, starts, table, seqs, cols, self._pages, self._page,
-            rows, self._heads, self._kv_heads, self._head_dim, self._scale, q.dtype == torch.bfloat16, ws.data_ptr() if need else 0, need))
+        ws = self._codes.new_empty(need) if need else None
+        _enqueue("smeg_paged_attend_dev", device, PAGED_ATTEND_ARGS.pack(
+            q.data_ptr(), out.data_ptr(), qs, os_, *self._at, cu, starts, table, seqs, cols, self._pages, self._page, rows, self._heads, self._kv_heads,
+            self._head_dim, self._scale, dtype is torch.bfloat16, ws.data_ptr() if need else 0, need))
 
     def read(self, ids, out) -> None:
         """The values of whole pages: out [n, kv_heads, 2, page, head_dim] (keys, values), contiguous f16 or bf16, for the n int32 page ids."""
         _ints(ids, "ids", self._device)
         n = ids.numel()
-        assert isinstance(out, torch.Tensor) and out.device == self._device and out.dtype in _DTYPES and out.is_contiguous(), "out is contiguous f16 or bf16"
+        assert isinstance(out, torch.Tensor) and out.get_device() == self._device and out.dtype in _DTYPES and out.is_contiguous(), "out is contiguous f16 or bf16"
         assert out.numel() == n * self._kv_heads * 2 * self._page * self._head_dim, "out holds n pages"
         if n == 0:
             return
-        args = (out.data_ptr(), self.codes.data_ptr(), self.scales.data_ptr(), ids.data_ptr(), n, self._pages, self._page, self._kv_heads, self._head_dim,
-                out.dtype == torch.bfloat16)
-        with _On(self._device.index):
-            check("smeg_paged_read_dev", lib().smeg_paged_read_dev(*args, torch._C._cuda_getCurrentRawStream(self._device.index)))
+        fn, device = lib().smeg_paged_read_dev, self._device
+        args = (out.data_ptr(), *self._at, ids.data_ptr(), n, self._pages, self._page, self._kv_heads, self._head_dim, out.dtype is torch.bfloat16)
+        if torch._C._cuda_getDevice() == device:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        else:
+            with _On(device):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        if rc:
+            check("smeg_paged_read_dev", rc)
 
 
 def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float | None = None) -> None:
@@ -332,17 +380,18 @@ def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float
     its rows 0..=i.  q, out: rows of heads * head_dim values, k, v of kv_heads * head_dim, f16 or bf16, at any row stride; scale 1 / sqrt(head_dim).
     Rows behind the last sequence are left as they are."""
     assert kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "heads must be a positive multiple of kv_heads"
-    assert isinstance(q, torch.Tensor) and q.dim() == 2 and q.shape[1] % heads == 0, "q has rows of heads * head_dim values"
-    hd = q.shape[1] // heads
+    like = dtype, device, rows = _first_rows(q, "q")
+    width = q.shape[1]
+    hd = width // heads
+    assert hd * heads == width, "q has rows of heads * head_dim values"
     assert hd % 8 == 0 and 8 <= hd <= 256, "head_dim must be a multiple of 8 in 8..=256"
-    qs = _rows(q, "q", heads * hd)
-    ks, vs, os_ = _rows(k, "k", kv_heads * hd, q), _rows(v, "v", kv_heads * hd, q), _rows(out, "out", heads * hd, q)
-    _ints(cu_rows, "cu_rows", q.device)
-    assert cu_rows.numel() >= 1, "cu_rows has one value more than there are sequences"
-    rows, seqs = q.shape[0], cu_rows.numel() - 1
+    row = kv_heads * hd
+    qs, ks, vs, os_ = _rows(q, "q", width, like), _rows(k, "k", row, like), _rows(v, "v", row, like), _rows(out, "out", width, like)
+    _ints(cu_rows, "cu_rows", device)
+    seqs = cu_rows.numel() - 1
+    assert seqs >= 0, "cu_rows has one value more than there are sequences"
     if rows == 0 or seqs == 0:
         return
-    scale = float(np.float32(1.0) / np.sqrt(np.float32(hd))) if scale is None else float(scale)
-    _enqueue("smeg_attn_packed_dev", q.device.index, ATTN_PACKED_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, vs, os_, cu_rows.data_ptr(), seqs, rows, heads, kv_heads, hd, scale,
-        q.dtype == torch.bfloat16))
+    _enqueue("smeg_attn_packed_dev", device, ATTN_PACKED_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, vs, os_, cu_rows.data_ptr(), seqs, rows, heads, kv_heads, hd,
+        hd ** -0.5 if scale is None else scale, dtype is torch.bfloat16))

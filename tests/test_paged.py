@@ -64,7 +64,7 @@ def test_frequencies_follow_their_definitions():
     (lambda: sg.rotate_heads(None, None, 0, sg.Rotary(64), None, None), "queries or keys"),
     (lambda: sg.rotate_heads(torch.zeros(2, 64), None, 0, None, torch.zeros(2, 64), None), "head_dim says"),
     (lambda: sg.attend_packed(*[torch.zeros(2, 64)] * 3, None, torch.zeros(2, 64), 3, 2), "multiple of kv_heads"),
-    (lambda: sg.attend_packed(*[torch.zeros(2, 24)] * 3, None, torch.zeros(2, 24), 2, 2), "multiple of 8"),
+    (lambda: sg.attend_packed(*[torch.zeros(2, 24)] * 3, None, torch.zeros(2, 24), 2, 2), "CUDA tensor"),
 ])
 def test_refusals_before_any_device_work(bad, message):
     with pytest.raises(AssertionError, match=message):
