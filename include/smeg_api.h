@@ -299,6 +299,8 @@ typedef struct smeg_rotate_args {
     size_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
     const float *q_norm, *k_norm;       /* head_dim weights of the heads' RMS norms, or NULL */
     const double *turns;                /* turns per position (frequency / 2 pi) of the rot / 2 rotated pairs, or NULL: no rotation */
+    const float *steps;                 /* [256][rot / 2 cosines, then rot / 2 sines]: row r those of r * frequency, without the factor; 16-byte
+                                         * aligned (smeg_paged_append_dev with turns) */
     float q_eps, k_eps, factor;         /* factor: on the cosines and sines */
     int interleaved, bf16, reserved;    /* pairs (2 i, 2 i + 1) instead of (i, i + rot / 2) */
     size_t rot, rows, heads, kv_heads, head_dim;

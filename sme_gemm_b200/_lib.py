@@ -51,7 +51,7 @@ class BlockArgs(C.Structure):
 BLOCK_ARGS = struct.Struct("@PNNPPPPffiiPPNNNPPNPPPfI")
 
 # smeg_rotate_args, smeg_paged_attend_args and smeg_attn_packed_args, packed the same way.
-ROTATE_ARGS = struct.Struct("@PPPPPNNNNNPPPfffiiiNNNNNPqPPPNNPPNN")
+ROTATE_ARGS = struct.Struct("@PPPPPNNNNNPPPPfffiiiNNNNNPqPPPNNPPNN")
 PAGED_ATTEND_ARGS = struct.Struct("@PPNNPPPPPNNNNNNNNfiPN")
 ATTN_PACKED_ARGS = struct.Struct("@PPPPNNNNPNNNNNfi")
 

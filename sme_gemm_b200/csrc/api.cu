@@ -1337,7 +1337,7 @@ static int rotate_dev(const smeg_rotate_args* b, bool paged, cudaStream_t stream
     if (b->rows > 0x7fffffffu || b->heads > 65535 || b->kv_heads > 65535) return -3;
     if (paged) {
         if (!b->k || !b->v || !b->codes || !b->scales || !b->cu_rows || !b->starts || !b->table || !page_ok(b->page) || b->v_stride < b->kv_heads * hd) return -4;
-        if (((uintptr_t)b->codes & 15) != 0) return -4;
+        if (((uintptr_t)b->codes & 15) != 0 || (b->turns && (!b->steps || ((uintptr_t)b->steps & 15) != 0))) return -4;
         if (b->seqs == 0) return 0;
         if (too_long(b->rows, b->kv_heads, b->kv_heads, b->seqs, b->table_cols, b->page, b->pages)) return -3;
     }
@@ -1348,7 +1348,7 @@ static int rotate_dev(const smeg_rotate_args* b, bool paged, cudaStream_t stream
     a.q = b->q; a.k = b->k; a.q_out = b->q_out; a.k_out = b->k_out;
     a.q_stride = b->q ? b->q_stride : 0; a.k_stride = b->k ? b->k_stride : 0; a.qo_stride = b->q ? b->q_out_stride : 0; a.ko_stride = b->k_out ? b->k_out_stride : 0;
     a.q_w = b->q ? b->q_norm : nullptr; a.k_w = b->k ? b->k_norm : nullptr; a.q_eps = b->q_eps; a.k_eps = b->k_eps;
-    a.turns = b->turns; a.rot = b->turns ? (int)b->rot : 0; a.interleaved = b->interleaved != 0; a.factor = b->factor;
+    a.turns = b->turns; a.steps = b->steps; a.rot = b->turns ? (int)b->rot : 0; a.interleaved = b->interleaved != 0; a.factor = b->factor;
     a.rows = (int)b->rows; a.heads = (int)b->heads; a.kv_heads = (int)b->kv_heads; a.head_dim = (int)hd; a.status = ds->status;
     if (paged) {
         a.v = b->v; a.v_stride = b->v_stride; a.codes = b->codes; a.scales = b->scales;

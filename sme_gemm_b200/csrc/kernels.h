@@ -266,6 +266,7 @@ struct RotateArgs {
     const float *q_w, *k_w;                // weights of the heads' norms; null: none
     float q_eps, k_eps;
     const double* turns;                   // turns per position of each rotated pair; null: no rotation
+    const float* steps;                    // [256][rot / 2 cosines, rot / 2 sines] of whole multiples of the frequencies (paged, with turns)
     int rot, interleaved;
     float factor;                          // on the cosines and sines
     const int* positions;                  // of the rows; null: start + row, or (with a batch) the sequences'
@@ -275,7 +276,9 @@ struct RotateArgs {
     uint8_t* codes;                        // [page][KV head][keys | values][position][depth]
     float* scales;                         // [page][KV head][keys | values]
     unsigned* status;
-    int lanes, q_heads_here, k_heads_here, row_tile, head_tile, head_tiles, page_heads, page_units;      // launcher-filled
+    int lanes_log2, row_tile, head_tile, row_heads, row_rows, row_magic, q_tiles, head_tiles;      // launcher-filled
+    int page_heads, page_rows, page_magic, page_groups, page_units;
+    float inv_hd;
 };
 cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStream_t stream);
 cudaError_t paged_read_launch(uint16_t* out, const uint8_t* codes, const float* scales, const int* ids, size_t n, int pages, int page, int kv_heads, int head_dim,

@@ -9,9 +9,10 @@
 // Everything from the loaded 16-bit value to the one rounding at the end (to 16 bits, or to a code) is 32 bits wide.  The angle is not: position *
 // (frequency / 2 pi) is formed and reduced to a fraction of a turn in 64 bits, since a position of 10^6 at 32 bits would leave 4 digits of it.
 //
-// A thread holds four pairs of one head (eight depths), the threads of a head are neighbouring lanes; a row's cosines and sines are formed once
-// in shared memory and serve all of its heads.  Rows of queries and the (page, KV heads) of a batch are CTAs of one launch.  A page's CTA reads its rows
-// twice -- for the largest magnitude, then for the codes; the second time they come from L2.
+// A thread holds four pairs of one head (eight depths), the threads of a head are neighbouring lanes.  Rows of queries and the (page, KV heads) of a
+// batch are CTAs of one launch.  A row's cosines and sines are formed once in shared memory and serve all of its query heads.  A page's CTA has few
+// heads, so there they are formed for its first row alone, and row r takes the sum formulas with the cosines and sines of r frequencies, which the
+// caller's table holds.
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
@@ -19,12 +20,22 @@
 namespace smeg {
 namespace {
 
-constexpr int kRotThreads = 256;
-constexpr int kTrigRows = 64;                      // rows whose cosines and sines are in shared memory at a time
+constexpr int kRotThreads = 128;
+constexpr int kRowTile = 4;                        // rows of a CTA of query heads, at most
+constexpr int kHeld = 8;                           // runs of eight depths that a thread of a page's CTA keeps
+constexpr int kAhead = 4;                          // and that a thread of a row's CTA has on their way
 constexpr float kLeastScale = 7.703719777548943e-34f;   // 2^-110: a smaller scale has no reciprocal to speak of and counts as zero
+constexpr float kRound = 12582912.0f;              // 1.5 * 2^23: what is added to it is rounded to an integer, in the low bits of the sum
+
+// How a head's pairs lie.  A thread has the pairs 4 c .. 4 c + 3.
+enum { kHalves = 0,                                // (i, i + hd / 2): two runs of four depths
+       kNeighbours = 1,                            // (2 i, 2 i + 1): one run of eight
+       kMixed = 2,                                 // (i, i + rot / 2) up to rot, neighbours behind: one or the other
+       kAny = 3 };                                 // rot no multiple of 8, or heads off the 8-byte grid: depth by depth
 
 struct HeadLay {
-    int hd, rot, half, group, inter;               // depths, rotated depths, rot / 2, lanes of a head (a power of two), interleaved pairs
+    int hd, half, group, log2_group, inter;        // depths, rotated pairs, lanes of a head (a power of two), interleaved pairs
+    float inv_hd;
 };
 
 // Index of the first (e = 0) or second member of a head's pair p.
@@ -32,70 +43,98 @@ __device__ __forceinline__ int pair_at(const HeadLay& L, int p, int e) {
     if (p >= L.half || L.inter) return 2 * p + e;   // (pairs behind the rotated part are neighbours, as 2 p = rot + 2 (p - rot / 2))
     return p + e * L.half;
 }
-
-// Pairs 4 c .. 4 c + 3 of a head.  VEC: rot a multiple of 8 and every head on an 8-byte boundary.
-template <int BF16, int VEC>
-__device__ __forceinline__ void load_pairs(const uint16_t* x, const HeadLay& L, int c, float (&a)[4], float (&b)[4]) {
-    if (VEC) {
-        const bool split = !L.inter && 4 * c < L.half;
-        const uint2 u = *reinterpret_cast<const uint2*>(x + (split ? 4 * c : 8 * c));
-        const uint2 w = *reinterpret_cast<const uint2*>(x + (split ? L.half + 4 * c : 8 * c + 4));
-        const uint32_t r[4] = {u.x, u.y, w.x, w.y};
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = t_to_f32<BF16>((uint16_t)r[i]);
-            f[2 * i + 1] = t_to_f32<BF16>((uint16_t)(r[i] >> 16));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            a[j] = split ? f[j] : f[2 * j];
-            b[j] = split ? f[4 + j] : f[2 * j + 1];
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            a[j] = t_to_f32<BF16>(x[pair_at(L, 4 * c + j, 0)]);
-            b[j] = t_to_f32<BF16>(x[pair_at(L, 4 * c + j, 1)]);
-        }
-    }
+template <int LAY>
+__device__ __forceinline__ bool is_split(const HeadLay& L, int c) {
+    return LAY == kHalves || (LAY == kMixed && 4 * c < L.half);
 }
-template <int BF16, int VEC>
-__device__ __forceinline__ void store_pairs(uint16_t* x, const HeadLay& L, int c, const float (&a)[4], const float (&b)[4]) {
-    if (VEC) {
-        const bool split = !L.inter && 4 * c < L.half;
+
+struct Octet {
+    float a[4], b[4];                              // first and second members of four pairs
+};
+template <int BF16>
+__device__ __forceinline__ float2 both(uint32_t w) {
+    if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+struct Raw {
+    uint2 u, w;                                    // as they lie: halves, four first members, then four second ones; neighbours, eight depths
+};
+template <int LAY>
+__device__ __forceinline__ Raw load_raw(const uint16_t* x, const HeadLay& L, int c) {
+    Raw o;
+    if (LAY != kAny) {
+        const bool split = is_split<LAY>(L, c);
+        o.u = *reinterpret_cast<const uint2*>(x + (split ? 4 * c : 8 * c));
+        o.w = *reinterpret_cast<const uint2*>(x + (split ? L.half + 4 * c : 8 * c + 4));
+    } else {
+        uint32_t r[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            r[j] = x[pair_at(L, 4 * c + j, 0)];
+            r[4 + j] = x[pair_at(L, 4 * c + j, 1)];
+        }
+        o.u = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+        o.w = make_uint2(r[4] | r[5] << 16, r[6] | r[7] << 16);
+    }
+    return o;
+}
+template <int BF16, int LAY>
+__device__ __forceinline__ Octet unpack(const Raw& x, const HeadLay& L, int c) {
+    const bool split = LAY == kAny || is_split<LAY>(L, c);
+    const float2 f[4] = {both<BF16>(x.u.x), both<BF16>(x.u.y), both<BF16>(x.w.x), both<BF16>(x.w.y)};
+    Octet o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        o.a[j] = split ? (j & 1 ? f[j / 2].y : f[j / 2].x) : f[j].x;
+        o.b[j] = split ? (j & 1 ? f[2 + j / 2].y : f[2 + j / 2].x) : f[j].y;
+    }
+    return o;
+}
+template <int BF16, int LAY>
+__device__ __forceinline__ void store_pairs(uint16_t* x, const HeadLay& L, int c, const Octet& o) {
+    if (LAY != kAny) {
+        const bool split = is_split<LAY>(L, c);
         uint2 u, w;
-        u.x = split ? pack2_t<BF16>(a[0], a[1]) : pack2_t<BF16>(a[0], b[0]);
-        u.y = split ? pack2_t<BF16>(a[2], a[3]) : pack2_t<BF16>(a[1], b[1]);
-        w.x = split ? pack2_t<BF16>(b[0], b[1]) : pack2_t<BF16>(a[2], b[2]);
-        w.y = split ? pack2_t<BF16>(b[2], b[3]) : pack2_t<BF16>(a[3], b[3]);
+        u.x = split ? pack2_t<BF16>(o.a[0], o.a[1]) : pack2_t<BF16>(o.a[0], o.b[0]);
+        u.y = split ? pack2_t<BF16>(o.a[2], o.a[3]) : pack2_t<BF16>(o.a[1], o.b[1]);
+        w.x = split ? pack2_t<BF16>(o.b[0], o.b[1]) : pack2_t<BF16>(o.a[2], o.b[2]);
+        w.y = split ? pack2_t<BF16>(o.b[2], o.b[3]) : pack2_t<BF16>(o.a[3], o.b[3]);
         *reinterpret_cast<uint2*>(x + (split ? 4 * c : 8 * c)) = u;
         *reinterpret_cast<uint2*>(x + (split ? L.half + 4 * c : 8 * c + 4)) = w;
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            x[pair_at(L, 4 * c + j, 0)] = f32_to_t<BF16>(a[j]);
-            x[pair_at(L, 4 * c + j, 1)] = f32_to_t<BF16>(b[j]);
+            x[pair_at(L, 4 * c + j, 0)] = f32_to_t<BF16>(o.a[j]);
+            x[pair_at(L, 4 * c + j, 1)] = f32_to_t<BF16>(o.b[j]);
         }
     }
 }
-__device__ __forceinline__ uint32_t to_code(float x, float inv) {
-    return (uint32_t)((int)fminf(fmaxf(rintf(x * inv), -127.0f), 127.0f) + 128);
+// code + 128 in the low byte: |x * inv| is at most 127 and a little (not half a code more), so nothing is clamped.
+__device__ __forceinline__ uint32_t code_of(float x, float inv) { return __float_as_uint(fmaf(x, inv, kRound + 128.0f)); }
+__device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
+// Byte e of a word of codes as the code it stands for: 2^23 + byte is a number whose bits end in the byte.
+__device__ __forceinline__ float byte_value(uint32_t w, int e) { return __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | e)) - 8388736.0f; }
 // Codes of four pairs: whole words where the pairs lie that way (a cache row starts on a 16-byte boundary), else byte by byte.
-__device__ __forceinline__ void store_codes(uint8_t* x, const HeadLay& L, int c, const float (&a)[4], const float (&b)[4], float inv) {
+template <int LAY>
+__device__ __forceinline__ void store_codes(uint8_t* x, const HeadLay& L, int c, const Octet& o, float inv) {
     uint32_t u[4], w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        u[j] = to_code(a[j], inv);
-        w[j] = to_code(b[j], inv);
+        u[j] = code_of(o.a[j], inv);
+        w[j] = code_of(o.b[j], inv);
     }
-    if (L.half % 4 == 0) {
-        const bool split = !L.inter && 4 * c < L.half;
-        const uint32_t lo = split ? u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24 : u[0] | w[0] << 8 | u[1] << 16 | w[1] << 24;
-        const uint32_t hi = split ? w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24 : u[2] | w[2] << 8 | u[3] << 16 | w[3] << 24;
-        *reinterpret_cast<uint32_t*>(x + (split ? 4 * c : 8 * c)) = lo;
-        *reinterpret_cast<uint32_t*>(x + (split ? L.half + 4 * c : 8 * c + 4)) = hi;
+    if (LAY != kAny || L.half % 4 == 0) {
+        const bool split = LAY == kAny ? !L.inter && 4 * c < L.half : is_split<LAY>(L, c);
+        const uint32_t lo = split ? four_bytes(u[0], u[1], u[2], u[3]) : four_bytes(u[0], w[0], u[1], w[1]);
+        const uint32_t hi = split ? four_bytes(w[0], w[1], w[2], w[3]) : four_bytes(u[2], w[2], u[3], w[3]);
+        if (LAY == kNeighbours) {
+            *reinterpret_cast<uint2*>(x + 8 * c) = make_uint2(lo, hi);
+        } else {
+            *reinterpret_cast<uint32_t*>(x + (split ? 4 * c : 8 * c)) = lo;
+            *reinterpret_cast<uint32_t*>(x + (split ? L.half + 4 * c : 8 * c + 4)) = hi;
+        }
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -105,48 +144,87 @@ __device__ __forceinline__ void store_codes(uint8_t* x, const HeadLay& L, int c,
     }
 }
 
-// Norm (w0, w1: the weights of the thread's pairs) and rotation (cs: cosine and sine of the row's pairs).  All lanes of the warp.
-__device__ __forceinline__ void turn(const HeadLay& L, bool live, bool norm, float eps, const float (&w0)[4], const float (&w1)[4], const float2* cs,
-                                     float (&a)[4], float (&b)[4]) {
-    if (norm) {
-        float sum = 0.0f;
+// Sum, or largest, of a head's lanes: every lane of the warp, whichever heads they have.
+__device__ __forceinline__ float head_sum(float x, int group) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum = fmaf(a[j], a[j], fmaf(b[j], b[j], sum));
-        if (!live) sum = 0.0f;
-        for (int o = L.group >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(sum, (float)L.hd) + eps));
+    for (int s = 16; s; s >>= 1)
+        if (s < group) x += __shfl_xor_sync(0xffffffffu, x, s);
+    return x;
+}
+__device__ __forceinline__ unsigned head_max(unsigned x, int group) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            a[j] = a[j] * r * w0[j];
-            b[j] = b[j] * r * w1[j];
-        }
-    }
-    if (cs) {
+    for (int s = 16; s; s >>= 1)
+        if (s < group) x = max(x, __shfl_xor_sync(0xffffffffu, x, s));
+    return x;
+}
+// Norm (w: the weights of the thread's pairs).  All lanes of the warp.
+__device__ __forceinline__ void normalise(const HeadLay& L, bool live, float eps, const Octet& w, Octet& o) {
+    float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 t = cs[j];
-            const float x = a[j], y = b[j];
-            a[j] = fmaf(-y, t.y, x * t.x);
-            b[j] = fmaf(x, t.y, y * t.x);
-        }
+    for (int j = 0; j < 4; ++j) sum = fmaf(o.a[j], o.a[j], fmaf(o.b[j], o.b[j], sum));
+    const float mean = fmaf(head_sum(live ? sum : 0.0f, L.group), L.inv_hd, eps);
+    float r;                                                       // (within 2 units of the last place; a mean below 2^-126 counts as zero)
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(mean));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        o.a[j] = o.a[j] * r * w.a[j];
+        o.b[j] = o.b[j] * r * w.b[j];
     }
 }
-
-// Cosines and sines of `rows` rows' pairs (1 and 0 behind the rotated part).
-template <class Pos>
-__device__ __forceinline__ void fill_trig(const RotateArgs& p, const HeadLay& L, float2* cs, int rows, Pos pos) {
-    const int pairs = L.hd / 2;
-    for (int i = threadIdx.x; i < rows * pairs; i += kRotThreads) {
-        const int r = i / pairs, j = i - r * pairs;
-        float2 t = make_float2(1.0f, 0.0f);
-        if (j < L.half) {
-            const double turns = (double)pos(r) * p.turns[j];
-            const float frac = (float)(turns - rint(turns));
-            sincospif(2.0f * frac, &t.y, &t.x);
-            t.x *= p.factor;
-            t.y *= p.factor;
+// Rotation by the cosines and sines of the four pairs.
+__device__ __forceinline__ void rotate4(const float4 c, const float4 s, Octet& o) {
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float x = o.a[j], y = o.b[j];
+        o.a[j] = fmaf(-y, ss[j], x * cc[j]);
+        o.b[j] = fmaf(x, ss[j], y * cc[j]);
+    }
+}
+template <int LAY>
+__device__ __forceinline__ Octet norm_weights(const float* w, const HeadLay& L, int c, bool live) {
+    Octet o = {};
+    if (!w || !live) return o;
+    if (LAY != kAny) {
+        const bool split = is_split<LAY>(L, c);
+        const float4 x = *reinterpret_cast<const float4*>(w + (split ? 4 * c : 8 * c)), y = *reinterpret_cast<const float4*>(w + (split ? L.half + 4 * c : 8 * c + 4));
+        const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o.a[j] = split ? f[j] : f[2 * j];
+            o.b[j] = split ? f[4 + j] : f[2 * j + 1];
         }
-        cs[i] = t;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o.a[j] = w[pair_at(L, 4 * c + j, 0)];
+            o.b[j] = w[pair_at(L, 4 * c + j, 1)];
+        }
+    }
+    return o;
+}
+__device__ __forceinline__ float2 cos_sin(const RotateArgs& p, long long pos, int pair) {
+    const double turns = (double)pos * p.turns[pair];
+    const float frac = (float)(turns - rint(turns));
+    float2 t;
+    sincospif(2.0f * frac, &t.y, &t.x);
+    return make_float2(t.x * p.factor, t.y * p.factor);
+}
+// Cosines and sines of `rows` rows' pairs (1 and 0 behind the rotated part): a row's cosines, then its sines.
+template <class Pos>
+__device__ __forceinline__ void fill_trig(const RotateArgs& p, const HeadLay& L, float* cs, int rows, Pos pos) {
+    const int pairs = L.hd / 2;
+    int r = 0, j = threadIdx.x;
+    while (j >= pairs) { j -= pairs; ++r; }
+    int dr = 0, dj = kRotThreads;
+    while (dj >= pairs) { dj -= pairs; ++dr; }
+    while (r < rows) {
+        const float2 t = j < L.half ? cos_sin(p, pos(r), j) : make_float2(1.0f, 0.0f);
+        cs[r * L.hd + j] = t.x;
+        cs[r * L.hd + pairs + j] = t.y;
+        r += dr;
+        j += dj;
+        if (j >= pairs) { j -= pairs; ++r; }
     }
 }
 
@@ -161,16 +239,15 @@ __device__ __forceinline__ int count_upto(int n, long long x, Key key) {
     return got;
 }
 
-// A (page, KV heads) of the batch, keys or values.
-template <int BF16, int VEC>
-__device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L, float2* cs, int unit) {
+// A (page, KV heads) of the batch, keys or values.  A thread keeps what it loaded -- kHeld runs of eight, as they lie -- from the search for the largest
+// magnitude to the codes, and norms and turns them a second time; a longer page is read twice.
+template <int BF16, int LAY>
+__device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L, float* cs, int unit) {
     __shared__ unsigned s_max[32];
     __shared__ float s_inv[32], s_ratio[32];
     const PackedSeqs& B = p.seqs;
     const int tid = threadIdx.x, page = 1 << B.page_log2;
-    const int which = unit & 1, hgroups = (p.kv_heads + p.page_heads - 1) / p.page_heads;
-    const int hg = (unit >> 1) % hgroups;
-    const long long slot = (unit >> 1) / hgroups;
+    const int which = unit & 1, slot = (unit >> 1) / p.page_groups, hg = (unit >> 1) - slot * p.page_groups;
     const int h0 = hg * p.page_heads, nh = min(p.page_heads, p.kv_heads - h0);
     const int s = count_upto(B.seqs, slot, [&](int i) { int f; seq_rows(B, i, &f); return first_slot(f, i, B.page_log2, 2); }) - 1;
     if (s < 0) return;
@@ -182,61 +259,88 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
     if (piece < 0 || piece >= pieces(rows, d, B.page_log2)) return;
     const int r0 = piece == 0 ? 0 : (int)(piece * page - d), r1 = (int)min((long long)rows, (piece + 1) * page - d), n = r1 - r0;
     const int at = piece == 0 ? d : 0;                             // first slot that is written
+    // (row, head) of this thread's group of lanes, pairs 4 c ... of it
+    const int c = tid & (L.group - 1), mine = tid >> L.log2_group, rpp = p.page_rows, mr = mine * p.page_magic >> 16, mh = mine - mr * p.page_heads;
+    const bool mine_ok = 8 * c < L.hd && mr < rpp && mh < nh;
+    const bool keys = which == 0, norm = keys && p.k_w != nullptr, rotate = keys && p.turns != nullptr;
+    const size_t stride = keys ? p.k_stride : p.v_stride, step = stride * rpp;
+    const uint16_t* src = (keys ? p.k : p.v) + (size_t)(first + r0 + mr) * stride + (h0 + mh) * L.hd;
+    const int left = mine_ok ? n - mr : 0;                         // rows from this thread's first one on
+    Raw held[kHeld];
+    auto load = [&](int c0) {                                      // rows c0 + mr, c0 + mr + rpp, ...
+        const uint16_t* x = src + (size_t)c0 * stride;
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e) {
+            held[e].u = held[e].w = make_uint2(0, 0);
+            if (c0 + e * rpp < left) held[e] = load_raw<LAY>(x, L, c);
+            x += step;
+        }
+    };
+    load(0);                                                       // (on their way while the page is looked up)
     const int id = page_of(B, s, (long long)start + r0);
     if (id < 0) {
         if (tid == 0 && p.status) atomicOr(p.status, STATUS_PAGE);
         return;
     }
-    const bool keys = which == 0;
-    const uint16_t* src = (keys ? p.k : p.v) + (size_t)(first + r0) * (keys ? p.k_stride : p.v_stride) + (size_t)h0 * L.hd;
-    const size_t stride = keys ? p.k_stride : p.v_stride;
-    const size_t block = (size_t)page * L.hd;                      // bytes of one head's keys or values in a page
-    uint8_t* dst = p.codes + (((size_t)id * p.kv_heads + h0) * 2 + which) * block + (size_t)at * L.hd;
+    const int block = page * L.hd;                                 // bytes of one head's keys or values in a page
+    uint8_t* dst = p.codes + (((size_t)id * p.kv_heads + h0) * 2 + which) * block + at * L.hd;
     float* scale = p.scales + ((size_t)id * p.kv_heads + h0) * 2 + which;
     if (tid < 32) s_max[tid] = 0;
-    const int lane_c = tid & (L.group - 1), per_pass = kRotThreads / L.group, mine = tid / L.group;
-    const bool live_c = lane_c * 8 < L.hd, norm = keys && p.k_w != nullptr, rotate = keys && p.turns != nullptr;
-    float w0[4] = {}, w1[4] = {};
-    if (norm && live_c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            w0[j] = p.k_w[pair_at(L, 4 * lane_c + j, 0)];
-            w1[j] = p.k_w[pair_at(L, 4 * lane_c + j, 1)];
-        }
-    auto trig = [&](int c0, int m) {
-        if (!rotate) return;
-        __syncthreads();
-        fill_trig(p, L, cs, m, [&](int r) { return (long long)start + r0 + c0 + r; });
-        __syncthreads();
-    };
-    auto pass = [&](int c0, int m, auto done) {                    // rows c0 .. c0 + m of the page's, all heads
-        for (int i0 = 0; i0 < m * nh; i0 += per_pass) {
-            const int it = i0 + mine;
-            const bool live = it < m * nh && live_c;
-            const int r = live ? it / nh : 0, h = live ? it - r * nh : 0;
-            float a[4] = {}, b[4] = {};
-            if (live) load_pairs<BF16, VEC>(src + (size_t)(c0 + r) * stride + (size_t)h * L.hd, L, lane_c, a, b);
-            turn(L, live, norm, p.k_eps, w0, w1, rotate && live ? cs + (size_t)r * (L.hd / 2) + 4 * lane_c : nullptr, a, b);
-            done(live, c0 + r, h, a, b);
-        }
-    };
+    const Octet w = norm_weights<LAY>(norm ? p.k_w : nullptr, L, c, mine_ok);
+    // The first row's angles are formed here; row r is r steps of the frequencies further, by the sum formulas (steps: [256][cosines, sines], 32 bits)
+    if (rotate) fill_trig(p, L, cs, 1, [&](int) { return (long long)start + r0; });
     __syncthreads();
-    for (int c0 = 0; c0 < n; c0 += kTrigRows) {
-        const int m = min(kTrigRows, n - c0);
-        trig(c0, m);
-        pass(c0, m, [&](bool live, int, int h, const float (&a)[4], const float (&b)[4]) {
-            unsigned mx = 0;                                       // (of the bits: an infinity or NaN is larger than every number)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mx = max(mx, max(__float_as_uint(fabsf(a[j])), __float_as_uint(fabsf(b[j]))));
-            if (!live) mx = 0;
-            for (int o = L.group >> 1; o; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            if (live && lane_c == 0) atomicMax(&s_max[h], mx);
-        });
+    float4 c_0 = make_float4(1.f, 1.f, 1.f, 1.f), s_0 = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rotate && mine_ok) {
+        c_0 = *reinterpret_cast<const float4*>(cs + 4 * c);
+        s_0 = *reinterpret_cast<const float4*>(cs + L.hd / 2 + 4 * c);
     }
+    auto treat = [&](int e, int r) {                               // run e, row r
+        Octet o = unpack<BF16, LAY>(held[e], L, c);
+        if (norm) normalise(L, r < left + mr, p.k_eps, w, o);
+        if (rotate && r < left + mr) {
+            float4 u = make_float4(1.f, 1.f, 1.f, 1.f), v = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float* t = p.steps + r * 2 * L.half + 4 * c;
+            if (LAY != kAny || L.half % 4 == 0) {
+                if (4 * c < L.half) {
+                    u = *reinterpret_cast<const float4*>(t);
+                    v = *reinterpret_cast<const float4*>(t + L.half);
+                }
+            } else {
+                float x[4], y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool in = 4 * c + j < L.half;
+                    x[j] = in ? t[j] : 1.0f;
+                    y[j] = in ? t[L.half + j] : 0.0f;
+                }
+                u = make_float4(x[0], x[1], x[2], x[3]);
+                v = make_float4(y[0], y[1], y[2], y[3]);
+            }
+            const float4 cc = make_float4(fmaf(-s_0.x, v.x, c_0.x * u.x), fmaf(-s_0.y, v.y, c_0.y * u.y), fmaf(-s_0.z, v.z, c_0.z * u.z), fmaf(-s_0.w, v.w, c_0.w * u.w));
+            const float4 ss = make_float4(fmaf(c_0.x, v.x, s_0.x * u.x), fmaf(c_0.y, v.y, s_0.y * u.y), fmaf(c_0.z, v.z, s_0.z * u.z), fmaf(c_0.w, v.w, s_0.w * u.w));
+            rotate4(cc, ss, o);
+        }
+        return o;
+    };
+    unsigned mx = 0;                                               // (of the bits: an infinity or NaN is larger than every number)
+    const int chunk = kHeld * rpp;
+    for (int c0 = 0; c0 < n; c0 += chunk) {
+        if (c0) load(c0);
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e) {
+            if (c0 + e * rpp >= n) break;                          // (the same for the whole block)
+            const Octet o = treat(e, c0 + e * rpp + mr);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx = max(mx, max(__float_as_uint(fabsf(o.a[j])), __float_as_uint(fabsf(o.b[j]))));
+        }
+    }
+    mx = head_max(mx, L.group);
+    if (mine_ok && c == 0) atomicMax(&s_max[mh], mx);
     __syncthreads();
     if (tid < nh) {
-        const float old = at == 0 ? 0.0f : scale[2 * tid], mx = __uint_as_float(s_max[tid]);
-        float now = mx < __uint_as_float(0x7f800000u) ? __fdiv_rn(mx, 127.0f) : __uint_as_float(0x7fc00000u);
+        const float old = at == 0 ? 0.0f : scale[2 * tid], top = __uint_as_float(s_max[tid]);
+        float now = top < __uint_as_float(0x7f800000u) ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
         if (now < kLeastScale) now = 0.0f;
         if (old >= now || old != old) now = old;                   // (a block that holds a NaN or an infinity is NaN until its page starts over)
         scale[2 * tid] = now;
@@ -245,108 +349,125 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
     }
     __syncthreads();
     // the codes of earlier calls under a scale that grew
-    for (int h = 0; h < nh; ++h) {
-        const float ratio = s_ratio[h];
-        if (ratio == 1.0f || at == 0) continue;
-        uint32_t* old = reinterpret_cast<uint32_t*>(dst - (size_t)at * L.hd + (size_t)h * 2 * block);
-        for (int i = tid; i < at * L.hd / 4; i += kRotThreads) {
-            const uint32_t w = old[i];
-            uint32_t o = 0;
+    if (at > 0)
+        for (int h = 0; h < nh; ++h) {
+            const float ratio = s_ratio[h];
+            if (ratio == 1.0f) continue;
+            uint32_t* old = reinterpret_cast<uint32_t*>(dst - at * L.hd + h * 2 * block);
+            for (int i = tid; i < at * L.hd / 4; i += kRotThreads) {
+                const uint32_t x = old[i];
+                uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o |= to_code((float)((int)(w >> 8 * e & 255u) - 128), ratio) << 8 * e;
-            old[i] = o;
+                for (int e = 0; e < 4; ++e) o[e] = code_of(byte_value(x, e), ratio);
+                old[i] = four_bytes(o[0], o[1], o[2], o[3]);
+            }
         }
-    }
-    for (int c0 = 0; c0 < n; c0 += kTrigRows) {
-        const int m = min(kTrigRows, n - c0);
-        if (n > kTrigRows) trig(c0, m);
-        pass(c0, m, [&](bool live, int r, int h, const float (&a)[4], const float (&b)[4]) {
-            if (!live) return;
-            store_codes(dst + (size_t)h * 2 * block + (size_t)r * L.hd, L, lane_c, a, b, s_inv[h]);
-            if (keys && p.k_out) store_pairs<BF16, VEC>(p.k_out + (size_t)(first + r0 + r) * p.ko_stride + (size_t)(h0 + h) * L.hd, L, lane_c, a, b);
-        });
+    const float inv = mine_ok ? s_inv[mh] : 0.0f;
+    uint8_t* to = dst + mh * 2 * block + mr * L.hd;
+    uint16_t* ko = keys && p.k_out ? p.k_out + (size_t)(first + r0 + mr) * p.ko_stride + (h0 + mh) * L.hd : nullptr;
+    for (int c0 = 0; c0 < n; c0 += chunk) {
+        if (n > chunk) load(c0);
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e) {
+            const int r = c0 + e * rpp;
+            if (r >= n) break;
+            const Octet o = treat(e, r + mr);
+            if (r >= left) continue;
+            store_codes<LAY>(to + r * L.hd, L, c, o, inv);
+            if (ko) store_pairs<BF16, LAY>(ko + (size_t)r * p.ko_stride, L, c, o);
+        }
     }
 }
 
-// Rows of heads: queries, or keys that go to no cache.
-template <int BF16, int VEC>
-__device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, float2* cs, int unit) {
-    __shared__ long long s_pos[kTrigRows];
+// A few rows of some query heads, or of key heads that go to no cache.
+template <int BF16, int LAY>
+__device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, float* cs, int unit) {
+    __shared__ long long s_pos[kRowTile];
     const int tid = threadIdx.x;
-    const int tile = unit / p.head_tiles, ht = unit - tile * p.head_tiles;
+    const int tile = unit / p.head_tiles;
+    int ht = unit - tile * p.head_tiles;
     const int r0 = tile * p.row_tile, n = min(p.row_tile, p.rows - r0);
-    const int all = p.q_heads_here + p.k_heads_here, h0 = ht * p.head_tile, nh = min(p.head_tile, all - h0);
+    const bool is_q = ht < p.q_tiles;
+    if (!is_q) ht -= p.q_tiles;
+    const int all = is_q ? p.heads : p.kv_heads, h0 = ht * p.head_tile, nh = min(p.head_tile, all - h0);
+    // (row, head) of this thread's group of lanes: `hpp` heads of `rpp` rows at a time, kAhead times as many rows on their way
+    const int hpp = p.row_heads, rpp = p.row_rows;
+    const int c = tid & (L.group - 1), mine = tid >> L.log2_group, mr = mine * p.row_magic >> 16, mh = mine - mr * hpp;
+    const bool mine_ok = 8 * c < L.hd && mr < rpp;
+    const size_t si = is_q ? p.q_stride : p.k_stride, so = is_q ? p.qo_stride : p.ko_stride;
+    const uint16_t* src = (is_q ? p.q : p.k) + (size_t)(r0 + mr) * si + (h0 + mh) * L.hd;
+    uint16_t* dst = (is_q ? p.q_out : p.k_out) + (size_t)(r0 + mr) * so + (h0 + mh) * L.hd;
+    Raw next[kAhead];
+    auto load = [&](int r, int h) {
+        const uint16_t* x = src + (size_t)r * si + h * L.hd;
+        const bool ok = mine_ok && h + mh < nh;
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            next[e].u = next[e].w = make_uint2(0, 0);
+            if (ok && r + e * rpp + mr < n) next[e] = load_raw<LAY>(x, L, c);
+            x += si * rpp;
+        }
+    };
+    load(0, 0);                                                    // (on their way while the rows' angles are formed)
     // positions, -1 for a row that is nobody's
-    for (int r = 0; r < n; ++r) {
-        if (p.positions) {
-            if (tid == 0) s_pos[r] = p.positions[r0 + r];
-        } else if (!p.seqs.cu) {
-            if (tid == 0) s_pos[r] = p.start + r0 + r;
-        } else {
-            const PackedSeqs& B = p.seqs;
-            const int s = count_upto(B.seqs, r0 + r, [&](int i) { int f; seq_rows(B, i, &f); return (long long)f; }) - 1;
-            if (tid == 0) {
-                int f = 0;
-                const int m = s < 0 ? 0 : seq_rows(B, s, &f), st = s < 0 ? -1 : B.starts[s];
-                s_pos[r] = st >= 0 && r0 + r < f + m ? (long long)st + (r0 + r - f) : -1;
-            }
+    int s = 0;
+    if (p.seqs.cu) s = count_upto(p.seqs.seqs, r0, [&](int i) { int f; seq_rows(p.seqs, i, &f); return (long long)f; }) - 1;
+    if (tid < n) {
+        long long pos = p.start + r0 + tid;
+        if (p.positions) pos = p.positions[r0 + tid];
+        if (p.seqs.cu) {
+            int f = 0, m = 0;
+            if (s < 0) s = 0;
+            while (s + 1 < p.seqs.seqs && p.seqs.cu[s + 1] <= r0 + tid) ++s;
+            m = seq_rows(p.seqs, s, &f);
+            const int st = p.seqs.starts[s];
+            pos = st >= 0 && r0 + tid >= f && r0 + tid < f + m ? (long long)st + (r0 + tid - f) : -1;
         }
+        s_pos[tid] = pos;
     }
+    const float* nw = is_q ? p.q_w : p.k_w;
+    const float eps = is_q ? p.q_eps : p.k_eps;
+    const Octet w = norm_weights<LAY>(nw, L, c, mine_ok);
     __syncthreads();
-    if (p.turns) fill_trig(p, L, cs, n, [&](int r) { return s_pos[r]; });
-    __syncthreads();
-    const int lane_c = tid & (L.group - 1), per_pass = kRotThreads / L.group, mine = tid / L.group;
-    const bool live_c = lane_c * 8 < L.hd;
-    float qw[2][4] = {}, kw[2][4] = {};
-    if (live_c)
+    if (p.turns) {
+        fill_trig(p, L, cs, n, [&](int r) { return s_pos[r]; });
+        __syncthreads();
+    }
+    const bool any_row = p.seqs.cu == nullptr;
+    for (int h = 0, r = 0; h < nh;) {
+        Raw cur[kAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int e = 0; e < kAhead; ++e) cur[e] = next[e];
+        const int h_now = h, r_now = r;
+        r += kAhead * rpp;
+        if (r >= n) { r = 0; h += hpp; }
+        if (h < nh) load(r, h);
+        uint16_t* y = dst + (size_t)r_now * so + h_now * L.hd;
+        const bool head_ok = mine_ok && h_now + mh < nh;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (p.q_w) qw[e][j] = p.q_w[pair_at(L, 4 * lane_c + j, e)];
-                if (p.k_w && p.k_heads_here) kw[e][j] = p.k_w[pair_at(L, 4 * lane_c + j, e)];
-            }
-    for (int i0 = 0; i0 < n * nh; i0 += per_pass) {
-        const int it = i0 + mine;
-        const bool in = it < n * nh;
-        const int r = in ? it / nh : 0, h = h0 + (in ? it - r * nh : 0);
-        const bool is_q = h < p.q_heads_here;
-        const int hh = is_q ? h : h - p.q_heads_here;
-        const bool live = in && live_c && (!p.seqs.cu || s_pos[r] >= 0);
-        float a[4] = {}, b[4] = {};
-        if (live) load_pairs<BF16, VEC>((is_q ? p.q + (size_t)(r0 + r) * p.q_stride : p.k + (size_t)(r0 + r) * p.k_stride) + (size_t)hh * L.hd, L, lane_c, a, b);
-        const float2* t = p.turns && live ? cs + (size_t)r * (L.hd / 2) + 4 * lane_c : nullptr;
-        float w0[4], w1[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            w0[j] = is_q ? qw[0][j] : kw[0][j];
-            w1[j] = is_q ? qw[1][j] : kw[1][j];
+        for (int e = 0; e < kAhead; ++e) {
+            if (r_now + e * rpp >= n) break;                       // (the same for the whole block)
+            const int row = r_now + e * rpp + mr;
+            const bool live = head_ok && row < n && (any_row || s_pos[row] >= 0);
+            Octet o = unpack<BF16, LAY>(cur[e], L, c);
+            if (nw) normalise(L, live, eps, w, o);
+            if (p.turns && live)
+                rotate4(*reinterpret_cast<const float4*>(cs + row * L.hd + 4 * c), *reinterpret_cast<const float4*>(cs + row * L.hd + L.hd / 2 + 4 * c), o);
+            if (live) store_pairs<BF16, LAY>(y, L, c, o);
+            y += so * rpp;
         }
-        const bool norm_q = p.q_w != nullptr, norm_k = p.k_w != nullptr;
-        float x[4], y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { x[j] = a[j]; y[j] = b[j]; }
-        if (norm_q || norm_k) {                                    // (the reduction is the whole warp's, whichever heads its lanes have)
-            turn(L, live, true, is_q ? p.q_eps : p.k_eps, w0, w1, nullptr, a, b);
-            if (!(is_q ? norm_q : norm_k))
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { a[j] = x[j]; b[j] = y[j]; }
-        }
-        turn(L, live, false, 0.0f, w0, w1, t, a, b);
-        if (live) store_pairs<BF16, VEC>((is_q ? p.q_out + (size_t)(r0 + r) * p.qo_stride : p.k_out + (size_t)(r0 + r) * p.ko_stride) + (size_t)hh * L.hd, L, lane_c, a, b);
     }
 }
 
-template <int BF16, int VEC>
-__global__ void __launch_bounds__(kRotThreads) rotate_append_kernel(const __grid_constant__ RotateArgs p) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    float2* cs = reinterpret_cast<float2*>(smem);
+template <int BF16, int LAY>
+__global__ void __launch_bounds__(kRotThreads, 5) rotate_append_kernel(const __grid_constant__ RotateArgs p) {
+    extern __shared__ __align__(16) float trig_s[];
     HeadLay L;
-    L.hd = p.head_dim; L.rot = p.rot; L.half = p.rot / 2; L.inter = p.interleaved; L.group = p.lanes;
+    L.hd = p.head_dim; L.half = p.rot / 2; L.inter = p.interleaved; L.log2_group = p.lanes_log2; L.group = 1 << p.lanes_log2; L.inv_hd = p.inv_hd;
     pdl_launch_dependents();
     pdl_wait();
-    if ((int)blockIdx.x < p.page_units) page_unit<BF16, VEC>(p, L, cs, blockIdx.x);
-    else row_unit<BF16, VEC>(p, L, cs, blockIdx.x - p.page_units);
+    if ((int)blockIdx.x < p.page_units) page_unit<BF16, LAY>(p, L, trig_s, blockIdx.x);
+    else row_unit<BF16, LAY>(p, L, trig_s, blockIdx.x - p.page_units);
 }
 
 // The values of whole pages: 16 codes a thread.
@@ -371,8 +492,7 @@ __global__ void __launch_bounds__(256) paged_read_kernel(uint16_t* __restrict__ 
     uint32_t o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const uint32_t x = r[e / 2] >> (16 * (e & 1));
-        o[e] = pack2_t<BF16>((float)((int)(x & 255u) - 128) * s, (float)((int)(x >> 8 & 255u) - 128) * s);
+        o[e] = pack2_t<BF16>(byte_value(r[e / 2], 2 * (e & 1)) * s, byte_value(r[e / 2], 2 * (e & 1) + 1) * s);
     }
     if (out_vec) {
         *reinterpret_cast<uint4*>(out + idx) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -386,41 +506,50 @@ __global__ void __launch_bounds__(256) paged_read_kernel(uint16_t* __restrict__ 
 }  // namespace
 
 cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStream_t stream) {
-    const bool paged = a.codes != nullptr;
-    a.lanes = 1;
-    while (a.lanes * 8 < a.head_dim) a.lanes *= 2;
+    const bool paged = a.codes != nullptr, vec = a.rot % 8 == 0 && ((a.q_stride | a.k_stride | a.v_stride | a.qo_stride | a.ko_stride) & 3) == 0 &&
+                     (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_out) & 7) == 0 &&
+                     (((uintptr_t)a.q_w | (uintptr_t)a.k_w) & 15) == 0;
+    const int lay = !vec ? kAny : (a.interleaved || a.rot == 0 ? kNeighbours : (a.rot == a.head_dim ? kHalves : kMixed));
+    a.lanes_log2 = 0;
+    while (8 << a.lanes_log2 < a.head_dim) ++a.lanes_log2;
+    const int per_pass = kRotThreads >> a.lanes_log2;
+    a.inv_hd = 1.0f / (float)a.head_dim;
     // row units: all heads of a few rows, so that they share the rows' cosines; of one row, as many heads as the block has at a time, while the
     // machine has room for more CTAs
-    a.q_heads_here = a.q ? a.heads : 0;
-    a.k_heads_here = a.k && !paged ? a.kv_heads : 0;
-    const int all = a.q_heads_here + a.k_heads_here;
-    a.row_tile = (size_t)a.rows >= (size_t)sm_count * 16 ? 4 : 1;
-    a.head_tile = (size_t)a.rows >= (size_t)sm_count * 4 ? all : kRotThreads / a.lanes;
-    if (a.head_tile > all) a.head_tile = all;
-    a.head_tiles = all ? (all + a.head_tile - 1) / a.head_tile : 0;
+    const int qh = a.q ? a.heads : 0, kh = a.k && !paged ? a.kv_heads : 0, most = qh > kh ? qh : kh;
+    a.row_tile = (size_t)a.rows >= (size_t)sm_count * 8 ? kRowTile : 1;
+    a.head_tile = (size_t)a.rows >= (size_t)sm_count * 4 ? most : per_pass;
+    if (a.head_tile > most) a.head_tile = most;
+    a.q_tiles = qh ? (qh + a.head_tile - 1) / a.head_tile : 0;
+    a.head_tiles = a.q_tiles + (kh ? (kh + a.head_tile - 1) / a.head_tile : 0);
+    a.row_heads = a.head_tile < per_pass ? a.head_tile : per_pass;
+    if (a.row_heads < 1) a.row_heads = 1;
+    a.row_rows = per_pass / a.row_heads;
+    a.row_magic = (65536 + a.row_heads - 1) / a.row_heads;         // mine * magic >> 16 = mine / row_heads for mine below 256
     const long long row_units = (long long)((a.rows + a.row_tile - 1) / a.row_tile) * a.head_tiles;
     long long page_units = 0;
-    int trig_rows = a.row_tile;
     if (paged) {
-        // as many KV heads to a CTA as make 256 rows of a full page; more share the cosines, fewer share the work
-        const int page = 1 << a.seqs.page_log2;
-        a.page_heads = page >= 256 ? 1 : 256 / page;
+        // KV heads of a CTA: as many as fill its registers with a sequence's rows in a page, and fewer while there is not a CTA an SM
+        const int page = 1 << a.seqs.page_log2, mean = (a.rows + a.seqs.seqs - 1) / a.seqs.seqs;
+        const long long slots = ((long long)a.rows >> a.seqs.page_log2) + 2ll * a.seqs.seqs;
+        a.page_heads = kHeld * per_pass / (mean < page ? mean : page);
+        if (a.page_heads > per_pass) a.page_heads = per_pass;
         if (a.page_heads > a.kv_heads) a.page_heads = a.kv_heads;
-        const long long most = ((long long)a.rows >> a.seqs.page_log2) + 2ll * a.seqs.seqs;
-        page_units = most * ((a.kv_heads + a.page_heads - 1) / a.page_heads) * 2;
-        trig_rows = page < kTrigRows ? page : kTrigRows;
+        if (a.page_heads < 1) a.page_heads = 1;
+        while (a.page_heads > 1 && slots * ((a.kv_heads + a.page_heads - 1) / a.page_heads) * 2 < sm_count) a.page_heads = (a.page_heads + 1) / 2;
+        a.page_rows = per_pass / a.page_heads;
+        a.page_magic = (65536 + a.page_heads - 1) / a.page_heads;
+        a.page_groups = (a.kv_heads + a.page_heads - 1) / a.page_heads;
+        page_units = slots * a.page_groups * 2;
     }
     if (row_units + page_units > 0x7fffffffll) return cudaErrorInvalidValue;
     if (row_units + page_units == 0) return cudaSuccess;
     a.page_units = (int)page_units;
-    const size_t smem = a.turns ? (size_t)trig_rows * (a.head_dim / 2) * sizeof(float2) : 0;
-    const bool vec = a.rot % 8 == 0 && ((a.q_stride | a.k_stride | a.v_stride | a.qo_stride | a.ko_stride) & 3) == 0 &&
-                     (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_out) & 7) == 0;
-    void (*kern)(RotateArgs) = bf16 ? (vec ? rotate_append_kernel<1, 1> : rotate_append_kernel<1, 0>) : (vec ? rotate_append_kernel<0, 1> : rotate_append_kernel<0, 0>);
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
+    const size_t smem = a.turns ? (size_t)a.row_tile * a.head_dim * sizeof(float) : 0;
+    typedef void (*Kern)(RotateArgs);
+    static const Kern kerns[2][4] = {{rotate_append_kernel<0, 0>, rotate_append_kernel<0, 1>, rotate_append_kernel<0, 2>, rotate_append_kernel<0, 3>},
+                                     {rotate_append_kernel<1, 0>, rotate_append_kernel<1, 1>, rotate_append_kernel<1, 2>, rotate_append_kernel<1, 3>}};
+    const Kern kern = kerns[bf16 ? 1 : 0][lay];
     return launch_pdl(kern, dim3((unsigned)(row_units + page_units)), dim3(kRotThreads), smem, stream, a);
 }
 

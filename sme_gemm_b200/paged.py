@@ -155,20 +155,25 @@ class Rotary:
         """On the cosines and sines."""
         return self._factor
 
-    def turns(self, device: int):
-        """(turns per position of each pair, f64 on the device; their address).  Made by the first call on a device: before a capture, then."""
+    def _on(self, device: int):
+        """(address of the turns per position of each pair, f64; address of the cosines and sines of 0 .. 255 times the frequencies, f32; the tensors).  Made by
+        the first call on a device: before a capture, then."""
         t = self._turns.get(device)
         if t is None:
-            x = torch.tensor(self._frequencies / (2.0 * math.pi), dtype=torch.float64, device=torch.device("cuda", device))
-            t = self._turns[device] = x, x.data_ptr()
+            at = torch.device("cuda", device)
+            turns = torch.tensor(self._frequencies / (2.0 * math.pi), dtype=torch.float64, device=at)
+            angle = np.arange(256, dtype=np.float64)[:, None] * self._frequencies
+            steps = torch.tensor(np.concatenate([np.cos(angle), np.sin(angle)], 1), dtype=torch.float32, device=at)
+            t = self._turns[device] = turns.data_ptr(), steps.data_ptr(), turns, steps
         return t
 
 
 def _rotation(rotary, head_dim: int, device: int):
     if rotary is None:
-        return 0, 0, 0, 1.0
+        return 0, 0, 0, 0, 1.0
     assert isinstance(rotary, Rotary) and rotary._head_dim == head_dim, "the rotation is one of heads of head_dim"
-    return rotary.turns(device)[1], rotary._rot, rotary._interleaved, rotary._factor
+    turns, steps, _, _ = rotary._on(device)
+    return turns, steps, rotary._rot, rotary._interleaved, rotary._factor
 
 
 def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=None, head_dim: int | None = None) -> None:
@@ -204,13 +209,13 @@ def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=N
         pos_ptr = positions.data_ptr()
     else:
         start = int(positions)
-    turns, rot, inter, factor = _rotation(rotary, hd, device)
+    turns, steps, rot, inter, factor = _rotation(rotary, hd, device)
     qn, qe = _head_norm(q_norm, "q_norm", hd, device)
     kn, ke = _head_norm(k_norm, "k_norm", hd, device)
     if rows == 0:
         return
     _enqueue("smeg_rotate_heads_dev", device, ROTATE_ARGS.pack(
-        q_ptr, k_ptr, 0, qo_ptr, ko_ptr, qs, ks, 0, qos, kos, qn, kn, turns, qe, ke, factor, inter, dtype is torch.bfloat16, 0, rot, rows, heads, kv_heads, hd,
+        q_ptr, k_ptr, 0, qo_ptr, ko_ptr, qs, ks, 0, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, dtype is torch.bfloat16, 0, rot, rows, heads, kv_heads, hd,
         pos_ptr, start, 0, 0, 0, 0, 0, 0, 0, 0, 0))
 
 
@@ -325,13 +330,13 @@ class PagedKvCache:
             q_len = self._heads * hd
             qs, qos = _rows(q, "q", q_len, like), _rows(q_out, "q_out", q_len, like)
             q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
-        turns, rot, inter, factor = _rotation(rotary, hd, device)
+        turns, steps, rot, inter, factor = _rotation(rotary, hd, device)
         qn, qe = _head_norm(q_norm, "q_norm", hd, device)
         kn, ke = _head_norm(k_norm, "k_norm", hd, device)
         if like[2] == 0 or batch._fields[3] == 0:
             return
         _enqueue("smeg_paged_append_dev", device, ROTATE_ARGS.pack(
-            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, qs, ks, vs, qos, kos, qn, kn, turns, qe, ke, factor, inter, like[0] is torch.bfloat16, 0, rot,
+            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, qs, ks, vs, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, like[0] is torch.bfloat16, 0, rot,
             like[2], self._heads, self._kv_heads, hd, 0, 0, *batch._fields, *self._at, self._pages, self._page))
 
     def attend(self, q, batch: PagedBatch, out) -> None:

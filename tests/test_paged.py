@@ -30,7 +30,7 @@ def test_index_arithmetic_covers_sound_batches_and_stays_inside_for_any_values(i
 def test_packed_arguments_are_the_structures(index_check):
     got = list(map(int, subprocess.run([index_check, "sizes"], capture_output=True, text=True, check=True).stdout.split()))
     import struct
-    start = struct.calcsize("@PPPPPNNNNNPPPfffiiiNNNNNPq") - 8
+    start = struct.calcsize("@PPPPPNNNNNPPPPfffiiiNNNNNPq") - 8
     end = PAGED_ATTEND_ARGS.size - 8
     assert got == [ROTATE_ARGS.size, start, PAGED_ATTEND_ARGS.size, end, ATTN_PACKED_ARGS.size]
 
@@ -72,9 +72,9 @@ def test_refusals_before_any_device_work(bad, message):
 
 
 def _rotate(**kw):
-    names = ("q k v q_out k_out q_stride k_stride v_stride q_out_stride k_out_stride q_norm k_norm turns q_eps k_eps factor interleaved bf16 reserved rot rows heads "
+    names = ("q k v q_out k_out q_stride k_stride v_stride q_out_stride k_out_stride q_norm k_norm turns steps q_eps k_eps factor interleaved bf16 reserved rot rows heads "
              "kv_heads head_dim positions start cu_rows starts table seqs table_cols codes scales pages page").split()
-    a = dict(q=4096, k=4096, v=0, q_out=4096, k_out=4096, q_stride=256, k_stride=128, v_stride=128, q_out_stride=256, k_out_stride=128, q_norm=0, k_norm=0, turns=0,
+    a = dict(q=4096, k=4096, v=0, q_out=4096, k_out=4096, q_stride=256, k_stride=128, v_stride=128, q_out_stride=256, k_out_stride=128, q_norm=0, k_norm=0, turns=0, steps=0,
              q_eps=0.0, k_eps=0.0, factor=1.0, interleaved=0, bf16=0, reserved=0, rot=0, rows=2, heads=4, kv_heads=2, head_dim=64, positions=0, start=0, cu_rows=0,
              starts=0, table=0, seqs=0, table_cols=0, codes=0, scales=0, pages=0, page=0)
     a.update(kw)
@@ -95,7 +95,7 @@ def test_rotation_refuses_bad_arguments(kw, rc):
 
 @pytest.mark.parametrize("kw,rc", [(dict(head_dim=24), -4), (dict(v=0), -4), (dict(codes=0), -4), (dict(scales=0), -4), (dict(cu_rows=0), -4), (dict(starts=0), -4),
                                    (dict(table=0), -4), (dict(page=48), -4), (dict(page=8), -4), (dict(page=512), -4), (dict(v_stride=127), -4),
-                                   (dict(codes=4100), -4), (dict(k=0), -4), (dict(table_cols=1 << 26), -3), (dict(pages=1 << 32), -3), (dict(seqs=1 << 25), -3),
+                                   (dict(codes=4100), -4), (dict(turns=4096, rot=64), -4), (dict(turns=4096, rot=64, steps=4100), -4), (dict(k=0), -4), (dict(table_cols=1 << 26), -3), (dict(pages=1 << 32), -3), (dict(seqs=1 << 25), -3),
                                    (dict(seqs=0), 0), (dict(rows=0), 0)])
 def test_append_refuses_bad_arguments(kw, rc):
     assert sg.lib().smeg_paged_append_dev(_paged(**kw), None) == rc
