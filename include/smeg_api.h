@@ -325,7 +325,8 @@ int smeg_paged_read_dev(uint16_t *out, const uint8_t *codes, const float *scales
 
 /* Attention of a batch's rows against the cache, which already holds them: row i of sequence s attends to positions 0..=starts[s] + i; per
  * head softmax(scale * q . k) @ v in 32 bits, one rounding.  Rows of idle sequences become zeros.  Query head h uses KV head h / (heads / kv_heads).
- * workspace: smeg_paged_attend_workspace(...) bytes of device memory, 16-byte aligned, that nothing else uses until the call has run. */
+ * scales lies on
+ * an 8-byte boundary.  workspace: smeg_paged_attend_workspace(...) bytes of device memory, 16-byte aligned, that nothing else uses until the call has run. */
 typedef struct smeg_paged_attend_args {
     const uint16_t *q;
     uint16_t *out;

@@ -1323,7 +1323,7 @@ static int log2_of(size_t page) {
 // Sizes that the index arithmetic of paged.h is 32 bits wide for.
 static bool too_long(size_t rows, size_t heads, size_t kv_heads, size_t seqs, size_t cols, size_t page, size_t pages) {
     if (kv_heads == 0 || page == 0) return true;
-    return rows > 0x7fffffffu / (heads / kv_heads) || heads > 65535 || seqs > 0xffffffu || cols > 0x7fffffffu / page || pages > 0x7fffffffu;
+    return rows > 0x7fffffffu / (heads / kv_heads) || heads > 65535 || seqs > 0xffffffu || cols > 0x7fffffffu / page || pages > 0x3fffffffu / kv_heads;
 }
 static int rotate_dev(const smeg_rotate_args* b, bool paged, cudaStream_t stream) {
     if (!b) return -4;
@@ -1394,9 +1394,9 @@ int smeg_paged_attend_dev(const smeg_paged_attend_args* b, void* stream) {
     if (!b) return -4;
     if (b->rows == 0 || b->seqs == 0) return 0;
     if (!heads_ok(b->heads, b->kv_heads, b->head_dim, 16) || !page_ok(b->page)) return -4;
-    if (!b->q || !b->out || !b->codes || !b->scales || !b->cu_rows || !b->starts || !b->table || ((uintptr_t)b->codes & 15) != 0) return -4;
+    if (!b->q || !b->out || !b->codes || !b->scales || !b->cu_rows || !b->starts || !b->table || ((uintptr_t)b->codes & 15) != 0 || ((uintptr_t)b->scales & 7) != 0) return -4;
     if (b->q_stride < b->heads * b->head_dim || b->out_stride < b->heads * b->head_dim) return -4;
-    if (too_long(b->rows, b->heads, b->kv_heads, b->seqs, b->table_cols, b->page, b->pages)) return -3;
+    if (too_long(b->rows, b->heads, b->kv_heads, b->seqs, b->table_cols, b->page, b->pages) || b->pages == 0) return -3;
     DeviceState* ds = dev_state();
     if (!ds) return -5;
     PagedAttendArgs a;

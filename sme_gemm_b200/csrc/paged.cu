@@ -12,25 +12,32 @@
 //   S^T (keys x rows) = K Q^T,   O^T (depths x rows) += V^T P^T
 // A byte is not converted: as the low byte of a half word it is the f16 subnormal u * 2^-24, two masks for four codes, and the 128 of its offset
 // comes off through the accumulators' start values (-128 * 2^-24 * the sum of the other operand, formed by the same instruction on a constant).
-// Operands go from global memory to the registers they are used from: a lane takes 16 consecutive depths of a key as four steps of the first product, and
-// 16 depths of its four keys as eight row tiles of the second.  A query row is scaled by a power of two into f16's range (so bf16 queries are
-// exact too); the probabilities are f16 at 2^14, a group's scaled by its page's scale over the larger of the warp's two, and each 32 keys' sums are
-// folded into 32-bit registers, since the tensor core cuts its sums off.
+// Keys and values come by tiled copies into a ring of each warp's own (32 keys a stage, the copies' swizzle, and an order of the keys that
+// keeps the operand loads off each other's banks); a lane then takes 16 consecutive depths of a key as four steps of the first product, and 16
+// depths of its four keys as eight row tiles of the second.  The ring runs ahead over the ends of items, so that the next item's keys are on their way
+// while the warps' shares of this one meet.  A query row is scaled by a power of two into f16's range (so bf16 queries are exact too); the
+// probabilities are f16 at 2^7, a group's scaled by its page's scale over the larger of the warp's two; the reference of a row's exponentials follows
+// its maximum when that is 2^8 above it; each 32 keys' sums are folded into 32-bit registers, since the tensor core cuts its sums off.
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
+#include "tc_common.cuh"
+
+#include <string.h>
 
 namespace smeg {
 namespace {
 
 constexpr int kPaThreads = 128, kPaWarps = 4;
 constexpr uint32_t kOffset = 0x00800080u;           // two f16 subnormals of 128 * 2^-24
-constexpr float kPScale = 16384.0f;
+constexpr float kPScale = 128.0f;
+constexpr float kLazy = 8.0f;                       // a row's reference follows its maximum when that is 2^8 above it
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = a b + c
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t mov_trans(uint32_t x) {
     uint32_t r;
@@ -39,15 +46,19 @@ __device__ __forceinline__ uint32_t mov_trans(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t even_bytes(uint32_t w) { return w & 0x00ff00ffu; }
 __device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return __byte_perm(w, 0, 0x4341); }
-__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
     uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ uint2 ld_stream2(const uint8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+__device__ __forceinline__ uint4 lds8(uint32_t a) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
     return v;
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -133,41 +144,156 @@ __device__ __forceinline__ void store_row4(const PagedAttendArgs& p, int row, in
     }
 }
 
+// Where a worker is: sequence, its item (row tile, KV head) and unit.
+struct Walk {
+    int s, tile, kvh, row_tile;
+    long long left;                                  // units to go
+    SeqUnits U;
+};
+__device__ __forceinline__ void walk_to(const PagedAttendArgs& p, Walk& w, int tile_rows) {   // the sequence's sizes; sequences without units are passed over
+    while (w.s < p.seqs.seqs) {
+        w.U = seq_units(p.seqs, w.s, p.heads / p.kv_heads, p.kv_heads, tile_rows);
+        if (w.U.items > 0) return;
+        ++w.s;
+    }
+    w.left = 0;
+}
+__device__ __forceinline__ void walk_on(const PagedAttendArgs& p, Walk& w, int units, int tile_rows) {   // units: no more than the item has left
+    w.left -= units;
+    w.tile += units;
+    if (w.tile < w.U.tiles) return;
+    w.tile = 0;
+    if (++w.kvh < p.kv_heads) return;
+    w.kvh = 0;
+    if ((long long)++w.row_tile * p.kv_heads < w.U.items) return;
+    w.row_tile = 0;
+    ++w.s;
+    if (w.left > 0) walk_to(p, w, tile_rows);
+}
+
+struct PagedMaps {
+    CUtensorMap codes;                               // [block][position][depth], swizzled boxes of 64 or 128 depths x 16 or 32 positions
+};
+
 // HC: depths in units of 64 (1, 2 or 4); NT: tiles of eight query rows.
 template <int BF16, int HC, int NT>
-__global__ void __launch_bounds__(kPaThreads, HC == 4 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2)) paged_attend_kernel(const __grid_constant__ PagedAttendArgs p) {
-    constexpr int G = HC == 4 ? 1 : 2;               // groups of 16 keys that a warp has at a time
-    constexpr int kKeys = 16 * G;
+__global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) paged_attend_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedAttendArgs p) {
     constexpr int MT = 4 * HC;                       // tiles of 16 depths
     constexpr int NR = 8 * NT;
-    extern __shared__ __align__(16) float part[];    // [warp][NR maxima, NR sums, NR x depths]
+    constexpr int kStages = HC == 1 ? 4 : 3;
+    constexpr int kPitch = HC == 1 ? 64 : 128, kPanel = 32 * kPitch, kPanels = HC == 4 ? 2 : 1;   // bytes of a key, of 32 keys; panels of 128 depths
+    constexpr int kHalf = kPanels * kPanel, kStage = 2 * kHalf;                                   // keys, then values
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t full[kPaWarps][kStages];
+    __shared__ int s_block[kPaWarps][kStages][2];    // of each group of 16 keys, below zero: none
+    __shared__ float s_m[kPaWarps][NR], s_l[kPaWarps][NR];
+    __shared__ int abort_word;
+    volatile int* abort_flag = &abort_word;
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int hd = p.head_dim, group = p.heads / p.kv_heads, page = 1 << p.seqs.page_log2;
-    const size_t block = (size_t)page * hd;
-    pdl_launch_dependents();
+    if (tid == 0) {
+        abort_word = 0;
+        for (int w = 0; w < kPaWarps; ++w)
+            for (int i = 0; i < kStages; ++i) mbar_init(&full[w][i], 1);
+        fence_barrier_init();
+    }
     pdl_wait();
+    pdl_launch_dependents();                         // (behind the wait: what ran before this kernel is there for the next one's index work, too)
     long long total;
     Place at;
-    if (!find_unit(p, NR, [&](long long n) { return share_begin(n, gridDim.x, blockIdx.x); }, &total, &at)) return;
-    long long left = share_begin(total, gridDim.x, blockIdx.x + 1) - share_begin(total, gridDim.x, blockIdx.x);
-    bool first_piece = true;
-    int s = at.s;
-    long long off = at.off;
-    while (left > 0 && s < p.seqs.seqs) {
-        const SeqUnits U = seq_units(p.seqs, s, group, p.kv_heads, NR);
-        if (off >= U.items * U.tiles) { ++s; off = 0; continue; }
-        const long long item = off / U.tiles;
-        const int tile0 = (int)(off - item * U.tiles), tile1 = (int)min((long long)U.tiles, tile0 + left);
-        const int kvh = (int)(item % p.kv_heads);
-        const long long row_tile = item / p.kv_heads;
-        const int n0 = (int)(row_tile * NR), nrow = (int)min((long long)NR, (long long)U.rows * group - n0);   // packed rows x heads of the tile
-        left -= tile1 - tile0;
-        off += tile1 - tile0;
+    if (!find_unit(p, NR, [&](long long n) { return share_begin(n, gridDim.x, blockIdx.x); }, &total, &at)) return;   // (with barriers: the mbarriers are set up)
+    Walk now;
+    now.s = at.s;
+    now.left = share_begin(total, gridDim.x, blockIdx.x + 1) - share_begin(total, gridDim.x, blockIdx.x);
+    walk_to(p, now, NR);
+    {
+        const long long item = at.off / now.U.tiles;
+        now.tile = (int)(at.off - item * now.U.tiles);
+        now.row_tile = (int)(item / p.kv_heads);
+        now.kvh = (int)(item - (long long)now.row_tile * p.kv_heads);
+    }
+    // ---- this warp's ring ----
+    Walk ahead = now;
+    const uint32_t ring = smem_u32(smem) + warp * kStages * kStage;
+    int put = 0, issued = 0;
+    auto issue = [&]() {                             // the next piece (32 keys) that this warp has
+        while (ahead.left > 0) {
+            const int key0 = ahead.tile * kUnitKeys + 32 * warp;
+            const bool has = key0 < ahead.U.keys;
+            if (has) {
+                int id[2];
+                id[0] = page_of(p.seqs, ahead.s, key0);
+                id[1] = key0 + 16 >= ahead.U.keys ? -2 : (page >= 32 ? id[0] : page_of(p.seqs, ahead.s, key0 + 16));
+                if (lane == 0) {
+                    if ((id[0] == -1 || id[1] == -1) && p.status) atomicOr(p.status, STATUS_PAGE);
+                    const int z0 = 2 * (id[0] * p.kv_heads + ahead.kvh), z1 = 2 * (id[1] * p.kv_heads + ahead.kvh);
+                    s_block[warp][put][0] = id[0] < 0 ? -1 : z0;
+                    s_block[warp][put][1] = id[1] < 0 ? -1 : z1;
+                    const uint32_t dst = ring + put * kStage;
+                    uint64_t* bar = &full[warp][put];
+                    const int y = key0 & (page - 1);
+                    if (page >= 32) {
+                        mbar_expect_tx(bar, id[0] < 0 ? 0 : kStage);
+                        if (id[0] >= 0)
+#pragma unroll
+                            for (int c = 0; c < kPanels; ++c) {
+                                tma_3d(dst + c * kPanel, &maps.codes, 128 * c, y, z0, bar);
+                                tma_3d(dst + kHalf + c * kPanel, &maps.codes, 128 * c, y, z0 + 1, bar);
+                            }
+                    } else {
+                        mbar_expect_tx(bar, ((id[0] >= 0) + (id[1] >= 0)) * (kStage / 2));
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+                            if (id[b] >= 0)
+#pragma unroll
+                                for (int c = 0; c < kPanels; ++c) {
+                                    tma_3d(dst + c * kPanel + b * 16 * kPitch, &maps.codes, 128 * c, 0, b ? z1 : z0, bar);
+                                    tma_3d(dst + kHalf + c * kPanel + b * 16 * kPitch, &maps.codes, 128 * c, 0, (b ? z1 : z0) + 1, bar);
+                                }
+                    }
+                }
+                __syncwarp();
+                ++issued;
+                if (++put == kStages) put = 0;
+            }
+            walk_on(p, ahead, 1, NR);
+            if (has) return;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) issue();
+
+    // Key order: row g of a group's A operand is key pi(g), so that the lanes of a quarter warp meet different banks in both products
+    const int pi_g = g & 1 ? g ^ 4 : g, pi_t = (2 * t + 1) ^ 4;
+    const uint32_t k_at = HC == 1 ? pi_g * 64 + ((t ^ ((pi_g >> 1) & 3)) << 4) : pi_g * 128 + ((t ^ pi_g) << 4);
+    const uint32_t v_even = HC == 1 ? 2 * t * 64 + (((g >> 1) ^ t) << 4) + 8 * (g & 1) : 2 * t * 128 + ((g ^ (2 * t)) << 4);
+    const uint32_t v_odd = HC == 1 ? pi_t * 64 + (((g >> 1) ^ ((pi_t >> 1) & 3)) << 4) + 8 * (g & 1) : pi_t * 128 + ((g ^ pi_t) << 4);
+    const float zero4[4] = {0.f, 0.f, 0.f, 0.f};
+    int get = 0, parity = 0, taken = 0;
+    bool first_piece = true, ok = true;
+    float sk_n[2] = {0.f, 0.f}, sv_n[2] = {0.f, 0.f};
+    auto fetch_scales = [&](int stage) {             // of the piece in `stage`, whose pages are known since it was issued
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int z = s_block[warp][stage][b];
+            const float2 x = z >= 0 ? *reinterpret_cast<const float2*>(p.scales + z) : make_float2(0.f, 0.f);
+            sk_n[b] = x.x;
+            sv_n[b] = x.y;
+        }
+    };
+    if (issued > 0) fetch_scales(0);
+
+    while (now.left > 0) {
+        const SeqUnits U = now.U;
+        const int kvh = now.kvh, tile0 = now.tile, tile1 = (int)min((long long)U.tiles, tile0 + now.left);
+        const int n0 = now.row_tile * NR, nrow = (int)min((long long)NR, (long long)U.rows * group - n0);   // packed rows x heads of the tile
 
         // ---- queries: B fragments, a power of two to each row ----
         uint32_t qf[NT][4 * HC][2];
-        float row_scale[NT][2], start0[NT][2];
+        float row_scale[NT][2], start0[NT][4];
         int limit[NT][2];                            // keys that rows 2 t and 2 t + 1 of a tile attend to
+        const int low = U.start >= 0 ? min(U.start + n0 / group + 1, U.keys) : 0;    // keys that every row of the tile attends to
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int n = n0 + 8 * j + g, i = n / group, head = kvh * group + (n - i * group);
@@ -198,7 +324,7 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? (NT == 1 ? 2 : 1) : (NT 
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             // largest magnitude to 2^14 .. 2^15: exact but for depths 2^-28 below it (f16's own range needs no more than that)
             const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-            const int up = mx > 0.0f && ex < 120 && ex > -110 ? 14 - ex : 0;
+            const int up = mx > 0.0f && ex < 100 && ex > -110 ? 14 - ex : 0;
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
             const float back = __uint_as_float((uint32_t)(127 - up) << 23) * (p.scale_log2e * 16777216.0f);
 #pragma unroll
@@ -210,17 +336,18 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? (NT == 1 ? 2 : 1) : (NT 
                 }
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < 4 * HC; ++k) mma_f16(sum, kOffset, kOffset, kOffset, kOffset, qf[j][k][0], qf[j][k][1]);
+            for (int k = 0; k < 4 * HC; ++k) mma_f16(sum, kOffset, kOffset, kOffset, kOffset, qf[j][k][0], qf[j][k][1], sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) start0[j][e] = -sum[e & 1];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                start0[j][e] = -sum[e];
                 row_scale[j][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
                 const int m = n0 + 8 * j + 2 * t + e;
                 limit[j][e] = 8 * j + 2 * t + e < nrow && U.start >= 0 ? min(U.start + m / group + 1, U.keys) : 0;
             }
         }
 
-        // ---- this warp's keys of the tiles ----
+        // ---- this warp's pieces of the units ----
         float o[NT][MT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -231,133 +358,96 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? (NT == 1 ? 2 : 1) : (NT 
 #pragma unroll
             for (int e = 0; e < 2; ++e) { m_run[j][e] = -INFINITY; l_run[j][e] = 0.0f; }
         }
-        constexpr int kPer = kUnitKeys / kPaWarps / kKeys;             // pieces of kKeys keys that a warp has of a unit
-        const int pieces_all = (tile1 - tile0) * kPer;
-        uint4 kq[G][2][HC];                                            // key g and g + 8 of a group, 16 depths a chunk
-        uint4 vq[G][4][HC == 4 ? 2 : 1];                               // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        float sk[G], sv[G];
-        float sk_n[G], sv_n[G];
-        const uint8_t* base[G];
-        bool there[G];                                                 // the group's page holds keys that some row attends to
-        auto key_of = [&](int i) { return (tile0 + i / kPer) * kUnitKeys + warp * 32 + (i % kPer) * kKeys; };
-        auto locate = [&](int i) {
-#pragma unroll
-            for (int b = 0; b < G; ++b) {
-                const int key = key_of(i) + 16 * b;
-                int id = -1;
-                if (i < pieces_all && key < U.keys) {
-                    id = page_of(p.seqs, s, key);
-                    if (id < 0 && lane == 0 && p.status) atomicOr(p.status, STATUS_PAGE);
-                }
-                there[b] = id >= 0;
-                const size_t blk = ((size_t)max(id, 0) * p.kv_heads + kvh) * 2;
-                base[b] = p.codes + blk * block + (size_t)(key & (page - 1)) * hd;
-                sk_n[b] = there[b] ? p.scales[blk] : 0.0f;
-                sv_n[b] = there[b] ? p.scales[blk + 1] : 0.0f;
-            }
-        };
-        auto load_k = [&]() {
-#pragma unroll
-            for (int b = 0; b < G; ++b)
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
-#pragma unroll
-                    for (int c = 0; c < HC; ++c) {
-                        const int d = 16 * (t + 4 * c);
-                        kq[b][r][c] = there[b] && d < hd ? ld_stream(base[b] + (size_t)(g + 8 * r) * hd + d) : make_uint4(0, 0, 0, 0);
-                    }
-        };
-        auto load_v = [&]() {
-#pragma unroll
-            for (int b = 0; b < G; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint8_t* v = base[b] + block + (size_t)(2 * t + (r & 1) + 8 * (r >> 1)) * hd;
-                    if (HC == 1) {
-                        const uint2 w = there[b] && 8 * g < hd ? ld_stream2(v + 8 * g) : make_uint2(0, 0);
-                        vq[b][r][0] = make_uint4(w.x, w.y, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < (HC == 4 ? 2 : 1); ++c) {
-                            const int d = 16 * g + 128 * c;
-                            vq[b][r][c] = there[b] && d < hd ? ld_stream(v + d) : make_uint4(0, 0, 0, 0);
-                        }
-                    }
-                }
-        };
-        locate(0);
-        load_k();
-        load_v();
-        for (int i = 0; i < pieces_all; ++i) {
-            const int key0 = key_of(i);
-#pragma unroll
-            for (int b = 0; b < G; ++b) { sk[b] = sk_n[b]; sv[b] = sv_n[b]; }
-            bool here[G];
-#pragma unroll
-            for (int b = 0; b < G; ++b) here[b] = there[b];
+        const int end = min(tile1 * kUnitKeys, U.keys);
+        int last = -1;                                                 // the stage consumed last
+        for (int key0 = tile0 * kUnitKeys + 32 * warp; key0 < end; key0 += kUnitKeys) {
+            if (last >= 0) issue();                                    // (into the stage that the piece before has left)
+            const float sk[2] = {sk_n[0], sk_n[1]}, sv[2] = {sv_n[0], sv_n[1]};
+            const bool here0 = s_block[warp][get][0] >= 0, here1 = s_block[warp][get][1] >= 0;
+            ++taken;
+            if (taken < issued) fetch_scales(get + 1 == kStages ? 0 : get + 1);
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[warp][get], parity, abort_flag, p.status));
+            const uint32_t stage = ring + get * kStage;
             // scores
-            float sc[NT][G][4];
+            float sc[NT][2][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int b = 0; b < G; ++b) {
-                    sc[j][b][0] = sc[j][b][2] = start0[j][0];
-                    sc[j][b][1] = sc[j][b][3] = start0[j][1];
-                }
-#pragma unroll
-            for (int b = 0; b < G; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int c = 0; c < HC; ++c) {
-                    const uint32_t lo[4] = {kq[b][0][c].x, kq[b][0][c].y, kq[b][0][c].z, kq[b][0][c].w};
-                    const uint32_t hi[4] = {kq[b][1][c].x, kq[b][1][c].y, kq[b][1][c].z, kq[b][1][c].w};
+                    const uint32_t a = stage + (c >> 1) * kPanel + b * 16 * kPitch + (k_at ^ (64 * (c & 1)));
+                    const uint4 x = lds16(a), y = lds16(a + 8 * kPitch);
+                    const uint32_t lo[4] = {x.x, x.y, x.z, x.w}, hi[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const uint32_t a0 = even_bytes(lo[w]), a1 = even_bytes(hi[w]), a2 = odd_bytes(lo[w]), a3 = odd_bytes(hi[w]);
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) mma_f16(sc[j][b], a0, a1, a2, a3, qf[j][4 * c + w][0], qf[j][4 * c + w][1]);
+                        for (int j = 0; j < NT; ++j)
+                            mma_f16(sc[j][b], a0, a1, a2, a3, qf[j][4 * c + w][0], qf[j][4 * c + w][1], c + w == 0 ? start0[j] : sc[j][b]);
                     }
                 }
-            // (the next keys are on their way while these are weighed; their values' addresses are kept for after this piece's values)
-            locate(i + 1);
-            load_k();
-            float st = 0.0f;                                           // (fmaxf drops a NaN: it stays with the rows that attend to it)
+            const float st = fmaxf(fmaxf(sv[0], sv[1]), 0.0f);         // (fmaxf drops a NaN: it stays with the rows that attend to it)
+            float ratio[2];
 #pragma unroll
-            for (int b = 0; b < G; ++b) st = fmaxf(st, sv[b]);
-            uint32_t pf[NT][G][2];
-            float alpha[NT][2];
+            for (int b = 0; b < 2; ++b) ratio[b] = (sv[b] == st ? 1.0f : (st > 0.0f ? __fdividef(sv[b], st) : sv[b])) * kPScale;
+            const bool whole = key0 + 32 <= low && here0 && here1;
+            uint32_t pf[NT][2][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                float mx[2] = {-INFINITY, -INFINITY};
-                bool on[G][4];
+                float f[2][2];
 #pragma unroll
-                for (int b = 0; b < G; ++b)
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) f[b][e] = row_scale[j][e] * sk[b];
+                float mx[2] = {-INFINITY, -INFINITY};
+                unsigned on = 0xffu;                                   // bit 4 b + e: element e of group b counts
+                if (!whole) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + 16 * b + pi_g + 8 * (e >> 1);
+                            if (!((b ? here1 : here0) && key < limit[j][e & 1])) on &= ~(1u << (4 * b + e));
+                        }
+                }
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + 16 * b + g + 8 * (e >> 1);
-                        on[b][e] = here[b] && key < limit[j][e & 1];
-                        sc[j][b][e] = sc[j][b][e] * (row_scale[j][e & 1] * sk[b]);
-                        if (on[b][e]) mx[e & 1] = fmaxf(mx[e & 1], sc[j][b][e]);
+                        sc[j][b][e] *= f[b][e & 1];
+                        if (!whole && !(on >> (4 * b + e) & 1)) sc[j][b][e] = -INFINITY;
+                        mx[e & 1] = fmaxf(mx[e & 1], sc[j][b][e]);
                     }
+                bool far = false;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], w));
-                    mx[e] = fmaxf(mx[e], m_run[j][e]);
-                    const float ref = mx[e] == -INFINITY ? 0.0f : mx[e];
-                    alpha[j][e] = ex2(m_run[j][e] - ref);
-                    m_run[j][e] = mx[e];
-                    mx[e] = ref;
-                    l_run[j][e] *= alpha[j][e];
+                    far = far || mx[e] > m_run[j][e] + kLazy;          // (from -inf: whatever there is)
                 }
+                if (__any_sync(0xffffffffu, far)) {
+                    float alpha[2];
 #pragma unroll
-                for (int b = 0; b < G; ++b) {
-                    const float ratio = (sv[b] == st ? 1.0f : (st > 0.0f ? __fdividef(sv[b], st) : sv[b])) * kPScale;
+                    for (int e = 0; e < 2; ++e) {
+                        const float to = fmaxf(m_run[j][e], mx[e]);
+                        alpha[e] = ex2(m_run[j][e] - (to == -INFINITY ? 0.0f : to));
+                        m_run[j][e] = to;
+                        l_run[j][e] *= alpha[e];
+                    }
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][m][e] *= alpha[e & 1];
+                }
+                const float ref[2] = {m_run[j][0] == -INFINITY ? 0.0f : m_run[j][0], m_run[j][1] == -INFINITY ? 0.0f : m_run[j][1]};
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float x = ex2(sc[j][b][e] - mx[e & 1]);
-                        l_run[j][e & 1] += on[b][e] ? x : 0.0f;
-                        w[e] = on[b][e] ? x * ratio : 0.0f;
+                        const float x = ex2(sc[j][b][e] - ref[e & 1]);
+                        l_run[j][e & 1] += x;
+                        w[e] = x * ratio[b];
+                        if (!whole && !(on >> (4 * b + e) & 1)) w[e] = 0.0f;          // (not 0 * the NaN of a page that the row does not attend to)
                     }
                     pf[j][b][0] = mov_trans(pack2_t<0>(w[0], w[1]));
                     pf[j][b][1] = mov_trans(pack2_t<0>(w[2], w[3]));
@@ -367,91 +457,97 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? (NT == 1 ? 2 : 1) : (NT 
             float off0[NT][4];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
+                mma_f16(off0[j], kOffset, kOffset, kOffset, kOffset, pf[j][0][0], pf[j][0][1], zero4);
+                mma_f16(off0[j], kOffset, kOffset, kOffset, kOffset, pf[j][1][0], pf[j][1][1], off0[j]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) off0[j][e] = 0.0f;
-#pragma unroll
-                for (int b = 0; b < G; ++b) mma_f16(off0[j], kOffset, kOffset, kOffset, kOffset, pf[j][b][0], pf[j][b][1]);
+                for (int e = 0; e < 4; ++e) off0[j][e] = -off0[j][e];
             }
 #pragma unroll
-            for (int m = 0; m < MT; m += 2) {                          // a word of four depths: tiles m and m + 1
-                float acc[2][NT][4];
+            for (int c = 0; c < (HC == 4 ? 2 : 1); ++c) {
+                uint32_t vw[2][4][4];                                  // group, key, word
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[h][j][e] = -off0[j][e];
-#pragma unroll
-                for (int b = 0; b < G; ++b) {
-                    uint32_t w[4];
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const uint4 v = vq[b][r][HC == 4 ? m / 8 : 0];
-                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                        w[r] = x[(m / 2) & 3];
+                        const uint32_t a = stage + kHalf + c * kPanel + (16 * b + 8 * (r >> 1)) * kPitch + (r & 1 ? v_odd : v_even);
+                        const uint4 v = HC == 1 ? lds8(a) : lds16(a);
+                        vw[b][r][0] = v.x; vw[b][r][1] = v.y; vw[b][r][2] = v.z; vw[b][r][3] = v.w;
                     }
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t x = __byte_perm(w[0], w[1], h ? 0x7632 : 0x5410), y = __byte_perm(w[2], w[3], h ? 0x7632 : 0x5410);
+                for (int w = 0; w < (HC == 1 ? 2 : 4); ++w)
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) mma_f16(acc[h][j], even_bytes(x), odd_bytes(x), even_bytes(y), odd_bytes(y), pf[j][b][0], pf[j][b][1]);
+                    for (int h = 0; h < 2; ++h) {                      // depths 4 w + 2 h and the next: row tile m
+                        const int m = 8 * c + 2 * w + h;
+                        float acc[NT][4];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const uint32_t x = __byte_perm(vw[b][0][w], vw[b][1][w], h ? 0x7632 : 0x5410), y = __byte_perm(vw[b][2][w], vw[b][3][w], h ? 0x7632 : 0x5410);
+                            const uint32_t a0 = even_bytes(x), a1 = odd_bytes(x), a2 = even_bytes(y), a3 = odd_bytes(y);
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) mma_f16(acc[j], a0, a1, a2, a3, pf[j][b][0], pf[j][b][1], b ? acc[j] : off0[j]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[j][m][e] = fmaf(acc[j][e], st, o[j][m][e]);
                     }
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][m + h][e] = fmaf(o[j][m + h][e], alpha[j][e & 1], acc[h][j][e] * st);
             }
-            load_v();
+            last = get;
+            if (++get == kStages) { get = 0; parity ^= 1; }
+            __syncwarp();                                              // (every lane has read the stage)
         }
 
-        // ---- the warps' shares meet, then the item's ----
-        __syncthreads();                                               // (an earlier item's have been read)
-        float* mine = part + (size_t)warp * part_floats(NR, hd);
+        // ---- the warps' shares meet in the stages they have left, then the item's ----
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float l = l_run[j][e];
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
                 if (g == 0) {
-                    mine[8 * j + 2 * t + e] = m_run[j][e];
-                    mine[NR + 8 * j + 2 * t + e] = l;
+                    s_m[warp][8 * j + 2 * t + e] = m_run[j][e];
+                    s_l[warp][8 * j + 2 * t + e] = last < 0 ? -1.0f : l;               // below zero: this warp had no keys
                 }
             }
+        // (rows one after the other where stages are as large as NR x 64 HC numbers: kStage = 4096 HC = 16 * 64 HC * 4)
+        static_assert(kStage >= NR * 64 * HC * 4, "a stage holds a warp's share");
+        __shared__ int s_last[kPaWarps];
+        if (lane == 0) s_last[warp] = last;
+        if (last >= 0) {
+            float* mine = reinterpret_cast<float*>(smem + (size_t)(warp * kStages + last) * kStage);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // row tile m's rows g and g + 8 are depths 2 m and 2 m + 1 of the lane's run
-                    const int d = HC == 1 ? 8 * g + 2 * m + (e >> 1) : 16 * g + 128 * (m / 8) + 2 * (m % 8) + (e >> 1);
-                    if (d < hd) mine[2 * NR + (8 * j + 2 * t + (e & 1)) * hd + d] = o[j][m][e];
-                }
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // row tile m's rows g and g + 8 are depths 2 m and 2 m + 1 of the lane's run
+                        const int d = HC == 1 ? 8 * g + 2 * m + (e >> 1) : 16 * g + 128 * (m / 8) + 2 * (m % 8) + (e >> 1);
+                        mine[(8 * j + 2 * t + (e & 1)) * 64 * HC + d] = o[j][m][e];
+                    }
         }
         __syncthreads();
-        const bool whole = tile0 == 0 && tile1 == U.tiles;
+        const bool all_of_it = tile0 == 0 && tile1 == U.tiles;
         float* ws = p.ws + (2 * (size_t)blockIdx.x + (first_piece ? 0 : 1)) * part_floats(NR, hd);
         first_piece = false;
         for (int it = tid; it < nrow * (hd / 4); it += kPaThreads) {
             const int n = it / (hd / 4), d = (it - n * (hd / 4)) * 4;
             float mx = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kPaWarps; ++w) mx = fmaxf(mx, part[(size_t)w * part_floats(NR, hd) + n]);
+            for (int w = 0; w < kPaWarps; ++w) mx = fmaxf(mx, s_m[w][n]);
             const float ref = mx == -INFINITY ? 0.0f : mx;
             float l = 0.0f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kPaWarps; ++w) {
-                const float* o_w = part + (size_t)w * part_floats(NR, hd);
-                const float f = ex2(o_w[n] - ref);
-                const float4 x = *reinterpret_cast<const float4*>(o_w + 2 * NR + n * hd + d);
-                l = fmaf(f, o_w[NR + n], l);
+                if (s_l[w][n] < 0.0f) continue;
+                const float f = ex2(s_m[w][n] - ref);
+                const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)(w * kStages + s_last[w]) * kStage + (n * 64 * HC + d) * 4);
+                l = fmaf(f, s_l[w][n], l);
                 v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
             }
-            if (whole) {
+            if (all_of_it) {
                 const float r = l == 0.0f ? 0.0f : __fdiv_rn(16777216.0f / kPScale, l);   // (a row that attends to nothing is zero)
                 const int i = (n0 + n) / group, head = kvh * group + (n0 + n) - i * group;
                 store_row4<BF16>(p, U.first + i, head, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
@@ -459,6 +555,12 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? (NT == 1 ? 2 : 1) : (NT 
                 if (d == 0) { ws[n] = mx; ws[NR + n] = l; }
                 *reinterpret_cast<float4*>(ws + 2 * NR + n * hd + d) = v;
             }
+        }
+        walk_on(p, now, tile1 - tile0, NR);
+        if (now.left > 0) {
+            fence_proxy_async();                                       // (the shares' place is the ring's again)
+            __syncthreads();
+            if (last >= 0) issue();
         }
     }
 }
@@ -468,8 +570,7 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? (NT == 1 ? 2 : 1) : (NT 
 template <int BF16>
 __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const __grid_constant__ PagedAttendArgs p, int workers, int tile_rows) {
     const int tid = threadIdx.x, hd = p.head_dim, group = p.heads / p.kv_heads;
-    pdl_launch_dependents();
-    pdl_wait();
+    // (the batch is there: paged_attend_kernel lets this grid go behind its own wait)
     const int cut = blockIdx.x + 1;
     long long total;
     Place at;
@@ -482,6 +583,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const __grid_con
     if (w0 != cut - 1) return;
     const int kvh = (int)(item % p.kv_heads), n0 = (int)(item / p.kv_heads * tile_rows);
     const int nrow = (int)min((long long)tile_rows, (long long)U.rows * group - n0);
+    pdl_wait();
+    pdl_launch_dependents();
     const size_t pf = part_floats(tile_rows, hd);
     const size_t slot0 = 2 * (size_t)w0 + (begin > share_begin(total, workers, w0) ? 1 : 0);
     for (int it = tid; it < nrow * (hd / 4); it += kPaThreads) {
@@ -524,7 +627,7 @@ int tile_rows_of(int group, int max_rows) { return (long long)group * max_rows >
 // CTAs: as many as the GPU holds at a time (the occupancy of the variant), no more than there can be units.
 int workers_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
-    const int per_sm = hc == 4 ? (tile_rows == 8 ? 2 : 1) : (tile_rows == 8 ? 3 : 2);
+    const int per_sm = hc == 4 ? 1 : (hc == 2 ? 2 : 3);
     const long long room = ((long long)a.seqs.cols << a.seqs.page_log2), tiles = (room + kUnitKeys - 1) / kUnitKeys;
     const long long items = ((long long)a.seqs.rows * (a.heads / a.kv_heads) / tile_rows + a.seqs.seqs) * a.kv_heads;
     const long long most = (long long)sm_count * per_sm, units = items * (tiles > 0 ? tiles : 1);
@@ -534,12 +637,21 @@ int workers_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
 template <int BF16, int HC, int NT>
 cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t stream) {
     auto kern = paged_attend_kernel<BF16, HC, NT>;
-    const size_t smem = kPaWarps * part_floats(8 * NT, a.head_dim) * sizeof(float);
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
-    return launch_pdl(kern, dim3((unsigned)workers), dim3(kPaThreads), smem, stream, a);
+    TensorMapEncodeFn enc = tensor_map_encoder();
+    if (!enc) return cudaErrorNotSupported;
+    const int page = 1 << a.seqs.page_log2;
+    PagedMaps m;
+    const cuuint64_t dim[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)page, (cuuint64_t)a.seqs.pages * a.kv_heads * 2};
+    const cuuint64_t stride[2] = {(cuuint64_t)a.head_dim, (cuuint64_t)page * a.head_dim};
+    const cuuint32_t box[3] = {HC == 1 ? 64u : 128u, page >= 32 ? 32u : 16u, 1}, ones[3] = {1, 1, 1};
+    if (dim[2] == 0) return cudaErrorInvalidValue;
+    if (enc(&m.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, (void*)a.codes, dim, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            HC == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    const size_t smem = 1024 + (size_t)kPaWarps * (HC == 1 ? 4 : 3) * 4096 * HC;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kern, dim3((unsigned)workers), dim3(kPaThreads), smem, stream, m, a);
 }
 
 }  // namespace

@@ -262,11 +262,11 @@ class PagedKvCache:
         assert head_dim % 16 == 0 and 16 <= head_dim <= 256, "head_dim must be a multiple of 16 in 16..=256"
         assert kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "heads must be a positive multiple of kv_heads"
         assert page in (16, 32, 64, 128, 256), "a page holds 16, 32, 64, 128 or 256 positions"
-        assert pages >= 0, "pages is a number of pages"
+        assert pages > 0, "a cache has pages"
         self._heads, self._kv_heads, self._head_dim, self._pages, self._page = heads, kv_heads, head_dim, pages, page
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        self._codes = torch.full((max(pages, 1), kv_heads, 2, page, head_dim), 128, dtype=torch.uint8, device=device)
-        self._scales = torch.zeros((max(pages, 1), kv_heads, 2), dtype=torch.float32, device=device)
+        self._codes = torch.full((pages, kv_heads, 2, page, head_dim), 128, dtype=torch.uint8, device=device)
+        self._scales = torch.zeros((pages, kv_heads, 2), dtype=torch.float32, device=device)
         self._device = self._codes.get_device()
         self._at = self._codes.data_ptr(), self._scales.data_ptr()
         self._scale = float(np.float32(1.0) / np.sqrt(np.float32(head_dim)))

@@ -102,7 +102,7 @@ def test_append_refuses_bad_arguments(kw, rc):
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(head_dim=40), -4), (dict(heads=5), -4), (dict(kv_heads=0), -4), (dict(page=20), -4), (dict(q=0), -4), (dict(out=0), -4),
-                                   (dict(codes=0), -4), (dict(scales=0), -4), (dict(cu=0), -4), (dict(starts=0), -4), (dict(table=0), -4), (dict(codes=4104), -4),
+                                   (dict(codes=0), -4), (dict(scales=0), -4), (dict(cu=0), -4), (dict(starts=0), -4), (dict(table=0), -4), (dict(codes=4104), -4), (dict(scales=4100), -4), (dict(pages=0), -3),
                                    (dict(q_stride=255), -4), (dict(out_stride=255), -4), (dict(cols=1 << 26), -3), (dict(rows=1 << 31), -3), (dict(rows=0), 0),
                                    (dict(seqs=0), 0)])
 def test_cache_attention_refuses_bad_arguments(kw, rc):
