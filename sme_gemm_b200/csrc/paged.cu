@@ -60,6 +60,11 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
+// (x, y) += (a, b) * s in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float s) {
+    asm("{\n\t.reg .b64 u, v, w;\n\tmov.b64 u, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 w, {%4, %4};\n\tfma.rn.f32x2 u, v, w, u;\n\tmov.b64 {%0, %1}, u;\n\t}"
+        : "+f"(x), "+f"(y) : "f"(a), "f"(b), "f"(s));
+}
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -208,9 +213,9 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
     now.left = share_begin(total, gridDim.x, blockIdx.x + 1) - share_begin(total, gridDim.x, blockIdx.x);
     walk_to(p, now, NR);
     {
-        const long long item = at.off / now.U.tiles;
+        const long long item = quotient(at.off, now.U.tiles);
         now.tile = (int)(at.off - item * now.U.tiles);
-        now.row_tile = (int)(item / p.kv_heads);
+        now.row_tile = (int)quotient(item, p.kv_heads);
         now.kvh = (int)(item - (long long)now.row_tile * p.kv_heads);
     }
     // ---- this warp's ring ----
@@ -222,9 +227,12 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
             const int key0 = ahead.tile * kUnitKeys + 32 * warp;
             const bool has = key0 < ahead.U.keys;
             if (has) {
+                // (positions below U.keys are within the table)
+                const int* row = p.seqs.table + (size_t)ahead.s * p.seqs.cols + (key0 >> p.seqs.page_log2);
                 int id[2];
-                id[0] = page_of(p.seqs, ahead.s, key0);
-                id[1] = key0 + 16 >= ahead.U.keys ? -2 : (page >= 32 ? id[0] : page_of(p.seqs, ahead.s, key0 + 16));
+                id[0] = (unsigned)row[0] < (unsigned)p.seqs.pages ? row[0] : -1;
+                id[1] = key0 + 16 >= ahead.U.keys ? -2 : id[0];
+                if (page < 32 && id[1] != -2) id[1] = (unsigned)row[1] < (unsigned)p.seqs.pages ? row[1] : -1;
                 if (lane == 0) {
                     if ((id[0] == -1 || id[1] == -1) && p.status) atomicOr(p.status, STATUS_PAGE);
                     const int z0 = 2 * (id[0] * p.kv_heads + ahead.kvh), z1 = 2 * (id[1] * p.kv_heads + ahead.kvh);
@@ -293,10 +301,10 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
         uint32_t qf[NT][4 * HC][2];
         float row_scale[NT][2], start0[NT][4];
         int limit[NT][2];                            // keys that rows 2 t and 2 t + 1 of a tile attend to
-        const int low = U.start >= 0 ? min(U.start + n0 / group + 1, U.keys) : 0;    // keys that every row of the tile attends to
+        const int low = U.start >= 0 ? min(U.start + div_by(n0, p.by_group) + 1, U.keys) : 0;    // keys that every row of the tile attends to
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int n = n0 + 8 * j + g, i = n / group, head = kvh * group + (n - i * group);
+            const int n = n0 + 8 * j + g, i = div_by(n, p.by_group), head = kvh * group + (n - i * group);
             const bool in = 8 * j + g < nrow;
             const uint16_t* q = p.q + (size_t)(U.first + i) * p.q_stride + (size_t)head * hd;
             float x[HC][16];
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
             for (int e = 0; e < 2; ++e) {
                 row_scale[j][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
                 const int m = n0 + 8 * j + 2 * t + e;
-                limit[j][e] = 8 * j + 2 * t + e < nrow && U.start >= 0 ? min(U.start + m / group + 1, U.keys) : 0;
+                limit[j][e] = 8 * j + 2 * t + e < nrow && U.start >= 0 ? min(U.start + div_by(m, p.by_group) + 1, U.keys) : 0;
             }
         }
 
@@ -487,9 +495,10 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
                             for (int j = 0; j < NT; ++j) mma_f16(acc[j], a0, a1, a2, a3, pf[j][b][0], pf[j][b][1], b ? acc[j] : off0[j]);
                         }
 #pragma unroll
-                        for (int j = 0; j < NT; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[j][m][e] = fmaf(acc[j][e], st, o[j][m][e]);
+                        for (int j = 0; j < NT; ++j) {
+                            fma2(o[j][m][0], o[j][m][1], acc[j][0], acc[j][1], st);
+                            fma2(o[j][m][2], o[j][m][3], acc[j][2], acc[j][3], st);
+                        }
                     }
             }
             last = get;
@@ -532,7 +541,7 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
         float* ws = p.ws + (2 * (size_t)blockIdx.x + (first_piece ? 0 : 1)) * part_floats(NR, hd);
         first_piece = false;
         for (int it = tid; it < nrow * (hd / 4); it += kPaThreads) {
-            const int n = it / (hd / 4), d = (it - n * (hd / 4)) * 4;
+            const int n = div_by(it, p.by_quads), d = (it - n * (hd / 4)) * 4;
             float mx = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kPaWarps; ++w) mx = fmaxf(mx, s_m[w][n]);
@@ -549,7 +558,7 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
             }
             if (all_of_it) {
                 const float r = l == 0.0f ? 0.0f : __fdiv_rn(16777216.0f / kPScale, l);   // (a row that attends to nothing is zero)
-                const int i = (n0 + n) / group, head = kvh * group + (n0 + n) - i * group;
+                const int i = div_by(n0 + n, p.by_group), head = kvh * group + (n0 + n) - i * group;
                 store_row4<BF16>(p, U.first + i, head, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
             } else {
                 if (d == 0) { ws[n] = mx; ws[NR + n] = l; }
@@ -576,19 +585,19 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const __grid_con
     Place at;
     if (!find_unit(p, tile_rows, [&](long long n) { return share_begin(n, workers, cut); }, &total, &at)) return;
     const SeqUnits U = seq_units(p.seqs, at.s, group, p.kv_heads, tile_rows);
-    const long long item = at.off / U.tiles, u = share_begin(total, workers, cut);
+    const long long item = quotient(at.off, U.tiles), u = share_begin(total, workers, cut);
     const long long begin = u - (at.off - item * U.tiles), end = begin + U.tiles;
     if (begin == u) return;                                            // the cut is between two items
     const int w0 = share_of(total, workers, begin), w1 = share_of(total, workers, end - 1);
     if (w0 != cut - 1) return;
-    const int kvh = (int)(item % p.kv_heads), n0 = (int)(item / p.kv_heads * tile_rows);
+    const int row_tile = (int)quotient(item, p.kv_heads), kvh = (int)(item - (long long)row_tile * p.kv_heads), n0 = row_tile * tile_rows;
     const int nrow = (int)min((long long)tile_rows, (long long)U.rows * group - n0);
     pdl_wait();
     pdl_launch_dependents();
     const size_t pf = part_floats(tile_rows, hd);
     const size_t slot0 = 2 * (size_t)w0 + (begin > share_begin(total, workers, w0) ? 1 : 0);
     for (int it = tid; it < nrow * (hd / 4); it += kPaThreads) {
-        const int n = it / (hd / 4), d = (it - n * (hd / 4)) * 4;
+        const int n = div_by(it, p.by_quads), d = (it - n * (hd / 4)) * 4;
         float mx = -INFINITY, l = 0.0f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int w = w0; w <= w1; w += 4) {                            // four shares' loads at a time
@@ -617,7 +626,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const __grid_con
             mx = now;
         }
         const float r = l == 0.0f ? 0.0f : __fdiv_rn(16777216.0f / kPScale, l);
-        const int i = (n0 + n) / group, head = kvh * group + (n0 + n) - i * group;
+        const int i = div_by(n0 + n, p.by_group), head = kvh * group + (n0 + n) - i * group;
         store_row4<BF16>(p, U.first + i, head, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
     }
 }
@@ -665,6 +674,8 @@ size_t paged_attend_ws_floats(const PagedAttendArgs& a, int sm_count) {
 cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaStream_t stream) {
     if (a.seqs.rows == 0 || a.seqs.seqs == 0) return cudaSuccess;
     a.q_vec = a.q_stride % 8 == 0 && ((uintptr_t)a.q & 15) == 0;
+    a.by_group = fast_div((uint32_t)(a.heads / a.kv_heads));
+    a.by_quads = fast_div((uint32_t)(a.head_dim / 4));
     a.out_vec = a.out_stride % 4 == 0 && ((uintptr_t)a.out & 7) == 0;
     const int tr = tile_rows_of(a.heads / a.kv_heads, a.max_rows), workers = workers_of(a, tr, sm_count);
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);

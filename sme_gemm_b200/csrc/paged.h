@@ -78,15 +78,34 @@ SMEG_HD SeqUnits seq_units(const PackedSeqs& p, int s, int group, int kv_heads, 
     u.items = ((long long)u.rows * group + tile_rows - 1) / tile_rows * kv_heads;
     return u;
 }
+// x / y for x not below zero, in 32 bits where that will do (a 64-bit quotient is a hundred instructions).
+SMEG_HD long long quotient(long long x, int y) { return x <= 0xffffffffll ? (long long)((uint32_t)x / (uint32_t)y) : x / y; }
 // Worker w of n takes the units from share_begin(w) to share_begin(w + 1); unit u is worker share_of(u)'s.
 SMEG_HD long long share_begin(long long total, int n, int w) {
-    const long long q = total / n, r = total - q * n;        // the first r workers have one more
+    const long long q = quotient(total, n), r = total - q * n;   // the first r workers have one more
     return q * w + (w < r ? w : r);
 }
 SMEG_HD int share_of(long long total, int n, long long u) {
-    const long long q = total / n, r = total - q * n, cut = (q + 1) * r;
-    if (u < cut) return (int)(u / (q + 1));
-    return q ? (int)(r + (u - cut) / q) : n - 1;
+    const long long q = quotient(total, n), r = total - q * n, cut = (q + 1) * r;
+    if (u < cut) return (int)(q < 0x7fffffff ? quotient(u, (int)q + 1) : u / (q + 1));
+    return q ? (int)(r + (q <= 0x7fffffff ? quotient(u - cut, (int)q) : (u - cut) / q)) : n - 1;
+}
+// n / d for n below 2^31 by a product.
+struct FastDiv {
+    uint32_t mul, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+    FastDiv f = {1, 0};
+    while ((1ull << f.shift) < d) ++f.shift;
+    if (d > 1) f.mul = (uint32_t)(((1ull << 32) * ((1ull << f.shift) - d)) / d + 1);
+    return f;
+}
+SMEG_HD int div_by(int n, FastDiv f) {
+#ifdef __CUDA_ARCH__
+    return (int)((__umulhi((uint32_t)n, f.mul) + (uint32_t)n) >> f.shift);
+#else
+    return (int)(((uint32_t)(((uint64_t)(uint32_t)n * f.mul) >> 32) + (uint32_t)n) >> f.shift);
+#endif
 }
 
 }  // namespace smeg

@@ -91,6 +91,20 @@ int main(int argc, char** argv) {
                     offsetof(smeg_paged_attend_args, workspace_bytes), sizeof(smeg_attn_packed_args));
         return 0;
     }
+    for (uint32_t d : {1u, 2u, 3u, 5u, 7u, 8u, 12u, 24u, 63u, 64u, 100u, 641u, 65535u})
+        for (uint64_t n : {0ull, 1ull, 2ull, 6ull, 7ull, 8ull, 65535ull, 1000003ull, 2147483646ull, 2147483647ull})
+            for (int e = -2; e <= 2; ++e) {
+                const long long x = (long long)(n / d * d) + e;
+                if (x >= 0 && x <= 2147483647) REQUIRE(div_by((int)x, fast_div(d)) == (int)(x / d));
+            }
+    for (long long total : {0ll, 5ll, 443ll, 444ll, 4294967295ll, 4294967296ll, 1234567890123ll})
+        for (int n : {1, 7, 444}) {
+            for (int w = 0; w <= n; ++w) REQUIRE(share_begin(total, n, w) == total / n * w + std::min<long long>(w, total % n));
+            for (int w = 0; w < n; ++w) {
+                const long long a = share_begin(total, n, w), e = share_begin(total, n, w + 1);
+                if (a < e) REQUIRE(share_of(total, n, a) == w && share_of(total, n, e - 1) == w);
+            }
+        }
     std::mt19937_64 rng(7);
     auto pick = [&](long long lo, long long hi) { return lo + (long long)(rng() % (unsigned long long)(hi - lo + 1)); };
     for (int round = 0; round < 3000; ++round) {
