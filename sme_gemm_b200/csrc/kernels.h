@@ -298,7 +298,7 @@ struct PagedAttendArgs {
     float* ws;                             // paged_attend_ws_floats()
     unsigned* status;
     int q_vec, out_vec;                    // launcher-filled
-    FastDiv by_group, by_quads;            // / heads of a group, / (head_dim / 4)
+    FastDiv by_group, by_quads, by_par;    // / heads of a group, / (head_dim / 4), / rows that the join has at a time
 };
 size_t paged_attend_ws_floats(const PagedAttendArgs& a, int sm_count);
 cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaStream_t stream);

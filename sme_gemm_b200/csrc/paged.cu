@@ -76,7 +76,8 @@ struct Place {
     int s;
     long long off;
 };
-__device__ __forceinline__ long long block_scan(long long x, long long* warp_sums, long long* all) {   // inclusive; 128 threads
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(long long x, long long* warp_sums, long long* all) {   // inclusive
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -86,12 +87,13 @@ __device__ __forceinline__ long long block_scan(long long x, long long* warp_sum
     __syncthreads();                                               // (the sums of a scan before have been read)
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    long long before = 0;
+    long long before = 0, sum = 0;
 #pragma unroll
-    for (int w = 0; w < kPaWarps; ++w) {
+    for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) before += warp_sums[w];
+        sum += warp_sums[w];
     }
-    *all = warp_sums[0] + warp_sums[1] + warp_sums[2] + warp_sums[3];
+    *all = sum;
     return x + before;
 }
 __device__ __forceinline__ long long units_of(const PagedAttendArgs& p, int s, int tile_rows) {
@@ -100,27 +102,27 @@ __device__ __forceinline__ long long units_of(const PagedAttendArgs& p, int s, i
     return u.items * u.tiles;
 }
 // The total of all units, and (find) the place of unit `at(total)`; false where there is none.
-template <class At>
+template <int THREADS, class At>
 __device__ __forceinline__ bool find_unit(const PagedAttendArgs& p, int tile_rows, At at, long long* total_out, Place* out) {
-    __shared__ long long warp_sums[kPaWarps], s_off;
+    __shared__ long long warp_sums[THREADS / 32], s_off;
     __shared__ int s_seq;
     const int tid = threadIdx.x, n = p.seqs.seqs;
-    const bool once = n <= kPaThreads;
+    const bool once = n <= THREADS;
     if (tid == 0) s_seq = -1;
     long long total = 0, mine = 0, incl = 0, all = 0;
-    for (int s0 = 0; s0 < n; s0 += kPaThreads) {
+    for (int s0 = 0; s0 < n; s0 += THREADS) {
         mine = units_of(p, s0 + tid, tile_rows);
-        incl = block_scan(mine, warp_sums, &all);
+        incl = block_scan<THREADS>(mine, warp_sums, &all);
         total += all;
     }
     *total_out = total;
     const long long u = at(total);
     if (u < 0 || u >= total) return false;                         // (uniform: the whole block)
     long long base = 0;
-    for (int s0 = 0; s0 < n; s0 += kPaThreads) {
+    for (int s0 = 0; s0 < n; s0 += THREADS) {
         if (!once) {
             mine = units_of(p, s0 + tid, tile_rows);
-            incl = block_scan(mine, warp_sums, &all);
+            incl = block_scan<THREADS>(mine, warp_sums, &all);
         }
         const long long end = base + incl;
         if (u >= end - mine && u < end) {
@@ -133,6 +135,39 @@ __device__ __forceinline__ bool find_unit(const PagedAttendArgs& p, int tile_row
     out->s = s_seq;
     out->off = s_off;
     return out->s >= 0;
+}
+
+// The sequence of item `item` of all sequences': its first item and its first unit, and the total of all units.
+template <int THREADS>
+__device__ __forceinline__ bool find_item(const PagedAttendArgs& p, int tile_rows, int item, long long* total_out, int* seq, long long* first_item, long long* first_unit) {
+    __shared__ long long warp_sums[THREADS / 32], s_item, s_unit;
+    __shared__ int s_seq;
+    const int tid = threadIdx.x, n = p.seqs.seqs;
+    if (tid == 0) s_seq = -1;
+    long long items = 0, units = 0;
+    for (int s0 = 0; s0 < n; s0 += THREADS) {
+        long long mine = 0, all_items, all_units, tiles = 0;
+        if (s0 + tid < n) {
+            const SeqUnits u = seq_units(p.seqs, s0 + tid, p.heads / p.kv_heads, p.kv_heads, tile_rows);
+            mine = u.items;
+            tiles = u.tiles;
+        }
+        const long long upto = items + block_scan<THREADS>(mine, warp_sums, &all_items);
+        const long long end = units + block_scan<THREADS>(mine * tiles, warp_sums, &all_units);
+        if (item >= upto - mine && item < upto) {
+            s_seq = s0 + tid;
+            s_item = upto - mine;
+            s_unit = end - mine * tiles;
+        }
+        items += all_items;
+        units += all_units;
+    }
+    __syncthreads();
+    *total_out = units;
+    *seq = s_seq;
+    *first_item = s_item;
+    *first_unit = s_unit;
+    return s_seq >= 0;
 }
 
 // Unnormalised sums of a share of an item: maxima, sums of the probabilities, then rows x depths.
@@ -207,7 +242,7 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
     pdl_launch_dependents();                         // (behind the wait: what ran before this kernel is there for the next one's index work, too)
     long long total;
     Place at;
-    if (!find_unit(p, NR, [&](long long n) { return share_begin(n, gridDim.x, blockIdx.x); }, &total, &at)) return;   // (with barriers: the mbarriers are set up)
+    if (!find_unit<kPaThreads>(p, NR, [&](long long n) { return share_begin(n, gridDim.x, blockIdx.x); }, &total, &at)) return;   // (with barriers: the mbarriers are set up)
     Walk now;
     now.s = at.s;
     now.left = share_begin(total, gridDim.x, blockIdx.x + 1) - share_begin(total, gridDim.x, blockIdx.x);
@@ -574,16 +609,17 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
     }
 }
 
-// CTA b: the item that the cut before worker b + 1 goes through, if that is the first one through it.  A cut item is the last of its first worker's
+// The items that were cut are joined by a kernel of their own, whose search for them runs while the shares are still being made.
+// Many items of few shares: CTA b has the item that the cut before worker b + 1 goes through, if that is the first one through it.  A cut item is the last of its first worker's
 // and the first of the others'.
 template <int BF16>
-__global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const __grid_constant__ PagedAttendArgs p, int workers, int tile_rows) {
+__global__ void __launch_bounds__(kPaThreads) paged_join_cuts_kernel(const __grid_constant__ PagedAttendArgs p, int workers, int tile_rows) {
     const int tid = threadIdx.x, hd = p.head_dim, group = p.heads / p.kv_heads;
     // (the batch is there: paged_attend_kernel lets this grid go behind its own wait)
     const int cut = blockIdx.x + 1;
     long long total;
     Place at;
-    if (!find_unit(p, tile_rows, [&](long long n) { return share_begin(n, workers, cut); }, &total, &at)) return;
+    if (!find_unit<kPaThreads>(p, tile_rows, [&](long long n) { return share_begin(n, workers, cut); }, &total, &at)) return;
     const SeqUnits U = seq_units(p.seqs, at.s, group, p.kv_heads, tile_rows);
     const long long item = quotient(at.off, U.tiles), u = share_begin(total, workers, cut);
     const long long begin = u - (at.off - item * U.tiles), end = begin + U.tiles;
@@ -631,14 +667,96 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_kernel(const __grid_con
     }
 }
 
+// Fewer items than workers, so that an item has many shares: CTAs (b, y) take `par` rows at a time of item b.  A thread takes four depths of a row and every
+// so many shares; the threads of the same depths meet in shared memory.  (131071 keys of one sequence in 37 shares an item, us in all: by cuts 61, so 51.
+// 64 sequences of 2900 in two or three shares: by cuts 71.5, with this kernel's inner part by cuts 75.)
+constexpr int kPjThreads = 256;
+template <int BF16>
+__global__ void __launch_bounds__(kPjThreads) paged_join_items_kernel(const __grid_constant__ PagedAttendArgs p, int workers, int tile_rows, int par) {
+    __shared__ float4 s_v[kPjThreads];
+    __shared__ float s_m[kPjThreads / 4], s_l[kPjThreads / 4];
+    const int tid = threadIdx.x, hd = p.head_dim, group = p.heads / p.kv_heads;
+    // (the batch is there: paged_attend_kernel lets this grid go behind its own wait)
+    long long total, first_item, begin;
+    int s;
+    if (!find_item<kPjThreads>(p, tile_rows, blockIdx.x, &total, &s, &first_item, &begin)) return;
+    const long long item = blockIdx.x - first_item;
+    const SeqUnits U = seq_units(p.seqs, s, group, p.kv_heads, tile_rows);
+    begin += item * U.tiles;
+    const int w0 = share_of(total, workers, begin), w1 = share_of(total, workers, begin + U.tiles - 1);
+    if (w0 == w1) return;                                                          // (not cut)
+    const int row_tile = (int)quotient(item, p.kv_heads), kvh = (int)(item - (long long)row_tile * p.kv_heads), n0 = row_tile * tile_rows;
+    const int nrow = (int)min((long long)tile_rows, (long long)U.rows * group - n0);
+    const size_t pf = part_floats(tile_rows, hd);
+    const size_t slot0 = 2 * (size_t)w0 + (begin > share_begin(total, workers, w0) ? 1 : 0);
+    const int quads = hd / 4, lane = div_by(tid, p.by_quads), d = (tid - lane * quads) * 4;
+    const int lanes = div_by(div_by(kPjThreads, p.by_quads), p.by_par), pg = div_by(lane, p.by_par), r = lane - pg * par;    // share, row of this thread
+    pdl_wait();
+    pdl_launch_dependents();                         // (not before: the next kernel's CTAs would take the room that this grid's wait for)
+    for (int nb = blockIdx.y * par; nb < nrow; nb += gridDim.y * par) {
+        const int n = nb + r;
+        const bool in = pg < lanes && n < nrow;
+        float mx = -INFINITY, l = 0.0f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in)
+            for (int w = w0 + pg; w <= w1; w += 4 * lanes) {           // four shares' loads at a time
+                float m[4], q[4];
+                float4 x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int k = w + e * lanes;
+                    const float* ws = p.ws + (k == w0 ? slot0 : 2 * (size_t)min(k, w1)) * pf;
+                    m[e] = k <= w1 ? ws[n] : -INFINITY;
+                    q[e] = k <= w1 ? ws[tile_rows + n] : 0.0f;
+                    x[e] = k <= w1 ? *reinterpret_cast<const float4*>(ws + 2 * tile_rows + n * hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                const float now = fmaxf(fmaxf(fmaxf(mx, m[0]), fmaxf(m[1], m[2])), m[3]);
+                const float ref = now == -INFINITY ? 0.0f : now, f0 = ex2(mx - ref);
+                l *= f0;
+                v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float f = ex2(m[e] - ref);
+                    l = fmaf(f, q[e], l);
+                    v.x = fmaf(f, x[e].x, v.x); v.y = fmaf(f, x[e].y, v.y); v.z = fmaf(f, x[e].z, v.z); v.w = fmaf(f, x[e].w, v.w);
+                }
+                mx = now;
+            }
+        s_v[tid] = v;
+        if (d == 0 && in) { s_m[lane] = mx; s_l[lane] = l; }
+        __syncthreads();
+        if (pg == 0 && in) {
+            float top = -INFINITY;
+            for (int e = 0; e < lanes; ++e) top = fmaxf(top, s_m[e * par + r]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            l = 0.0f;
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int e = 0; e < lanes; ++e) {
+                const float f = ex2(s_m[e * par + r] - ref);
+                const float4 x = s_v[e * par * quads + tid];
+                l = fmaf(f, s_l[e * par + r], l);
+                v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+            }
+            const float scale = l == 0.0f ? 0.0f : __fdiv_rn(16777216.0f / kPScale, l);
+            const int i = div_by(n0 + n, p.by_group), head = kvh * group + (n0 + n) - i * group;
+            store_row4<BF16>(p, U.first + i, head, d, make_float4(v.x * scale, v.y * scale, v.z * scale, v.w * scale));
+        }
+        __syncthreads();
+    }
+}
+
 int tile_rows_of(int group, int max_rows) { return (long long)group * max_rows > 8 ? 16 : 8; }
+
+long long items_bound(const PagedAttendArgs& a, int tile_rows) {
+    return ((long long)a.seqs.rows * (a.heads / a.kv_heads) / tile_rows + a.seqs.seqs) * a.kv_heads;
+}
 
 // CTAs: as many as the GPU holds at a time (the occupancy of the variant), no more than there can be units.
 int workers_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
     const int per_sm = hc == 4 ? 1 : (hc == 2 ? 2 : 3);
     const long long room = ((long long)a.seqs.cols << a.seqs.page_log2), tiles = (room + kUnitKeys - 1) / kUnitKeys;
-    const long long items = ((long long)a.seqs.rows * (a.heads / a.kv_heads) / tile_rows + a.seqs.seqs) * a.kv_heads;
+    const long long items = items_bound(a, tile_rows);
     const long long most = (long long)sm_count * per_sm, units = items * (tiles > 0 ? tiles : 1);
     return (int)(units < most ? (units > 0 ? units : 1) : most);
 }
@@ -690,8 +808,18 @@ cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaS
     }
 #undef SMEG_PA
     if (e != cudaSuccess || workers == 1) return e;
-    return bf16 ? launch_pdl(paged_join_kernel<1>, dim3((unsigned)workers - 1), dim3(kPaThreads), 0, stream, a, workers, tr)
-                : launch_pdl(paged_join_kernel<0>, dim3((unsigned)workers - 1), dim3(kPaThreads), 0, stream, a, workers, tr);
+    const long long items = items_bound(a, tr);
+    if (items >= workers)
+        return bf16 ? launch_pdl(paged_join_cuts_kernel<1>, dim3((unsigned)workers - 1), dim3(kPaThreads), 0, stream, a, workers, tr)
+                    : launch_pdl(paged_join_cuts_kernel<0>, dim3((unsigned)workers - 1), dim3(kPaThreads), 0, stream, a, workers, tr);
+    // a row a CTA while that is no more than two CTAs an SM
+    const int lanes = kPjThreads / (a.head_dim / 4), rows = (int)min((long long)tr, (long long)a.max_rows * (a.heads / a.kv_heads));
+    int par = 1;
+    while (par * 2 <= lanes && par < rows && items * ((rows + par - 1) / par) > 2 * sm_count) par *= 2;
+    a.by_par = fast_div((uint32_t)par);
+    const dim3 grid((unsigned)items, (unsigned)((rows + par - 1) / par));
+    return bf16 ? launch_pdl(paged_join_items_kernel<1>, grid, dim3(kPjThreads), 0, stream, a, workers, tr, par)
+                : launch_pdl(paged_join_items_kernel<0>, grid, dim3(kPjThreads), 0, stream, a, workers, tr, par);
 }
 
 }  // namespace smeg
