@@ -610,6 +610,10 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
 }
 
 // The items that were cut are joined by a kernel of their own, whose search for them runs while the shares are still being made.
+// (A grid whose CTAs all left without waiting could end before the grid that it depends on, and the next one would not wait for that.)
+__device__ __forceinline__ void leave() {
+    if (blockIdx.x == 0) pdl_wait();
+}
 // Many items of few shares: CTA b has the item that the cut before worker b + 1 goes through, if that is the first one through it.  A cut item is the last of its first worker's
 // and the first of the others'.
 template <int BF16>
@@ -619,13 +623,13 @@ __global__ void __launch_bounds__(kPaThreads) paged_join_cuts_kernel(const __gri
     const int cut = blockIdx.x + 1;
     long long total;
     Place at;
-    if (!find_unit<kPaThreads>(p, tile_rows, [&](long long n) { return share_begin(n, workers, cut); }, &total, &at)) return;
+    if (!find_unit<kPaThreads>(p, tile_rows, [&](long long n) { return share_begin(n, workers, cut); }, &total, &at)) return leave();
     const SeqUnits U = seq_units(p.seqs, at.s, group, p.kv_heads, tile_rows);
     const long long item = quotient(at.off, U.tiles), u = share_begin(total, workers, cut);
     const long long begin = u - (at.off - item * U.tiles), end = begin + U.tiles;
-    if (begin == u) return;                                            // the cut is between two items
+    if (begin == u) return leave();                                            // the cut is between two items
     const int w0 = share_of(total, workers, begin), w1 = share_of(total, workers, end - 1);
-    if (w0 != cut - 1) return;
+    if (w0 != cut - 1) return leave();
     const int row_tile = (int)quotient(item, p.kv_heads), kvh = (int)(item - (long long)row_tile * p.kv_heads), n0 = row_tile * tile_rows;
     const int nrow = (int)min((long long)tile_rows, (long long)U.rows * group - n0);
     pdl_wait();
@@ -679,12 +683,12 @@ __global__ void __launch_bounds__(kPjThreads) paged_join_items_kernel(const __gr
     // (the batch is there: paged_attend_kernel lets this grid go behind its own wait)
     long long total, first_item, begin;
     int s;
-    if (!find_item<kPjThreads>(p, tile_rows, blockIdx.x, &total, &s, &first_item, &begin)) return;
+    if (!find_item<kPjThreads>(p, tile_rows, blockIdx.x, &total, &s, &first_item, &begin)) return leave();
     const long long item = blockIdx.x - first_item;
     const SeqUnits U = seq_units(p.seqs, s, group, p.kv_heads, tile_rows);
     begin += item * U.tiles;
     const int w0 = share_of(total, workers, begin), w1 = share_of(total, workers, begin + U.tiles - 1);
-    if (w0 == w1) return;                                                          // (not cut)
+    if (w0 == w1) return leave();                                                          // (not cut)
     const int row_tile = (int)quotient(item, p.kv_heads), kvh = (int)(item - (long long)row_tile * p.kv_heads), n0 = row_tile * tile_rows;
     const int nrow = (int)min((long long)tile_rows, (long long)U.rows * group - n0);
     const size_t pf = part_floats(tile_rows, hd);
