@@ -308,6 +308,28 @@ struct PromptTc {
     int slots;                                     // K / V ring
     long long pieces;                              // work slots of a KV head
 };
+// A work item: rows tok0 .. of a sequence, two query tiles of them, for one KV head.
+struct PromptItem {
+    int first, rows, tok0, kvh;                    // the sequence; rows below zero: there is no more
+};
+
+// The grid has a CTA for every work slot, and a CTA that has finished its own takes over the next one that has not been launched: the barriers and the
+// tensor memory are set up once, and the next item's queries and keys are on their way while this one's last blocks are weighed and its results stored.
+__device__ __forceinline__ void take_next_cta(uint32_t answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ int taken_cta(uint32_t answer) {        // its index, -1: all have been launched or taken
+    uint32_t ok, x;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+        : "=r"(ok), "=r"(x) : "r"(answer) : "memory");
+    return ok ? (int)x : -1;
+}
 
 template <int BF16, int NCH>
 __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptTc a) {
@@ -315,45 +337,31 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     const PromptArgs& p = a.p;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
-    __shared__ __align__(8) uint64_t bars[2 * kPtMaxSlots + 7];
+    __shared__ __align__(16) uint4 answer;
+    __shared__ __align__(8) uint64_t bars[2 * kPtMaxSlots + 13];
+    __shared__ PromptItem items[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
-    uint64_t *full = bars, *empty = full + kPtMaxSlots, *q_full = empty + kPtMaxSlots, *s_full = q_full + 1, *p_full = s_full + 2, *o_done = p_full + 2;
+    uint64_t *full = bars, *empty = full + kPtMaxSlots, *q_full = empty + kPtMaxSlots, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2, *o_done = p_full + 2,
+             *item_full = o_done + 2, *item_empty = item_full + 2, *taken = item_empty + 2;
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     const int hd = p.head_dim, hd16 = (hd + 15) & ~15, group = p.heads / p.kv_heads, tt = a.tokens;
-    const int kvh = (int)(blockIdx.x % (unsigned)p.kv_heads);
-    const long long slot_id = a.pieces - 1 - blockIdx.x / (unsigned)p.kv_heads;        // the pieces with the most keys first
-    pdl_wait();
-    int first = 0, rows = 0;
-    long long piece = 0;
-    {
-        int n = 0;
-        for (int s0 = 0; s0 < p.seqs.seqs; s0 += kPtThreads) {
-            const int s = s0 + tid;
-            int f = 0;
-            const bool at = s < p.seqs.seqs && (seq_rows(p.seqs, s, &f), first_slot_of(f, s, 2 * tt) <= slot_id);
-            n += __syncthreads_count(at);
-        }
-        if (n > 0) {
-            rows = seq_rows(p.seqs, n - 1, &first);
-            piece = slot_id - first_slot_of(first, n - 1, 2 * tt);
-        }
-        if (n == 0 || piece < 0 || piece >= pieces_of(rows, 2 * tt)) return;
-    }
-    const int tok0 = (int)(piece * 2 * tt);                        // tile x: the sequence's rows tok0 + x * tt ...
-    const int ntok[2] = {min(tt, rows - tok0), max(0, min(tt, rows - tok0 - tt))};
-    const int nblk[2] = {(tok0 + ntok[0] - 1) / kPtKeys + 1, ntok[1] ? (tok0 + tt + ntok[1] - 1) / kPtKeys + 1 : 0};
-    const int nmax = max(nblk[0], nblk[1]);
     unsigned char *q_s = smem, *ring = smem + 2 * kTile;
 
     if (tid == 0) {
         abort_word = 0;
         for (int i = 0; i < a.slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(q_full, 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+        mbar_init(q_empty, 1);
+        mbar_init(taken, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1);
+            mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 9);
+        }
         fence_barrier_init();
     }
+    pdl_wait();                                                    // (before the allocation: the kernel ahead may still hold tensor memory)
     if (warp == 9) {
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
@@ -364,30 +372,96 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     pdl_launch_dependents();
     const uint32_t tmem = tmem_slot;
 
-    if (warp == 8) {                                               // ---- loads ----
-        if (elect_one()) {
-            const int tiles = ntok[1] ? 2 : 1;
-            mbar_expect_tx(q_full, tiles * NCH * tt * group * 128);
-            for (int x = 0; x < tiles; ++x)
-                for (int c = 0; c < NCH; ++c) tma_4d(q_s + x * kTile + c * kPtChunk, &a.q, c * 64, 0, kvh, first + tok0 + x * tt, q_full);
-            int slot = 0, round = 0;
-            auto load = [&](const CUtensorMap* map, int j) {
-                if (round && !mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, p.status)) return false;
-                mbar_expect_tx(&full[slot], kTile);
-                for (int c = 0; c < NCH; ++c) tma_3d(ring + (size_t)slot * kTile + c * kPtChunk, map, c * 64, kvh, first + j * kPtKeys, &full[slot]);
-                if (++slot == a.slots) { slot = 0; ++round; }
-                return true;
-            };
-            for (int j = 0; j < nmax; ++j)
-                if (!load(&a.k, j) || !load(&a.v, j)) break;
-        }
+    // Item `it` of this CTA, for the warps that work on it: its place is free again once all of them have read it.
+    auto next_item = [&](int it, PromptItem& w) {
+        const int k = it & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&item_full[k], (it >> 1) & 1, abort_flag, p.status))) return false;
+        w = items[k];
         __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[k]);
+        return w.rows >= 0;
+    };
+    auto tokens_of = [&](const PromptItem& w, int x) { return max(0, min(tt, w.rows - w.tok0 - x * tt)); };
+    auto blocks_of = [&](const PromptItem& w, int x) {
+        const int n = tokens_of(w, x);
+        return n ? (w.tok0 + x * tt + n - 1) / kPtKeys + 1 : 0;
+    };
+
+    if (warp == 8) {                                               // ---- items and loads ----
+        int cta = blockIdx.x, slot = 0, round = 0, it = 0, asked = 0;
+        bool ok = true;
+        auto load = [&](const CUtensorMap* map, const PromptItem& w, int j) {
+            if (round && !__all_sync(0xffffffffu, mbar_wait(&empty[slot], (round - 1) & 1, abort_flag, p.status))) return false;
+            if (elect_one()) {
+                mbar_expect_tx(&full[slot], kTile);
+                for (int c = 0; c < NCH; ++c) tma_3d(ring + (size_t)slot * kTile + c * kPtChunk, map, c * 64, w.kvh, w.first + j * kPtKeys, &full[slot]);
+            }
+            __syncwarp();
+            if (++slot == a.slots) { slot = 0; ++round; }
+            return true;
+        };
+        while (ok) {
+            // the slot's sequence and piece; the pieces with the most keys first
+            PromptItem w = {0, -1, 0, 0};
+            if (cta >= 0) {
+                const int q = cta / p.kv_heads;
+                const long long slot_id = a.pieces - 1 - q;
+                w.kvh = cta - q * p.kv_heads;
+                int n = 0;
+                for (int s0 = 0; s0 < p.seqs.seqs; s0 += 32) {
+                    const int s = s0 + lane;
+                    int f = 0;
+                    n += __popc(__ballot_sync(0xffffffffu, s < p.seqs.seqs && (seq_rows(p.seqs, s, &f), first_slot_of(f, s, 2 * tt) <= slot_id)));
+                }
+                if (n > 0) {
+                    const int rows = seq_rows(p.seqs, n - 1, &w.first);
+                    const long long piece = slot_id - first_slot_of(w.first, n - 1, 2 * tt);
+                    if (piece >= 0 && piece < pieces_of(rows, 2 * tt)) {
+                        w.rows = rows;
+                        w.tok0 = (int)(piece * 2 * tt);
+                    }
+                }
+            }
+            if (cta < 0 || w.rows > 0) {                           // (a slot may be nobody's)
+                const int k = it & 1;
+                if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[k], ((it >> 1) - 1) & 1, abort_flag, p.status));
+                if (!ok) break;
+                if (lane == 0) {
+                    items[k] = w;
+                    mbar_arrive(&item_full[k]);
+                }
+                __syncwarp();
+                if (cta < 0) break;
+                if (it > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (it - 1) & 1, abort_flag, p.status));
+                if (!ok) break;
+                ++it;
+                const int tiles = tokens_of(w, 1) ? 2 : 1, n = max(blocks_of(w, 0), blocks_of(w, 1));
+                if (elect_one()) {
+                    mbar_expect_tx(q_full, tiles * NCH * tt * group * 128);
+                    for (int x = 0; x < tiles; ++x)
+                        for (int c = 0; c < NCH; ++c) tma_4d(q_s + x * kTile + c * kPtChunk, &a.q, c * 64, 0, w.kvh, w.first + w.tok0 + x * tt, q_full);
+                }
+                __syncwarp();
+                for (int j = 0; ok && j < n; ++j) ok = load(&a.k, w, j) && load(&a.v, w, j);
+                if (!ok) break;
+            }
+            if (elect_one()) {
+                fence_proxy_async();                               // (the last answer has been read)
+                mbar_expect_tx(taken, 16);
+                take_next_cta(smem_u32(&answer), taken);
+            }
+            __syncwarp();
+            ok = __all_sync(0xffffffffu, mbar_wait(taken, asked & 1, abort_flag, p.status));
+            ++asked;
+            cta = taken_cta(smem_u32(&answer));
+            __syncwarp();
+        }
     } else if (warp == 9) {                                        // ---- products ----
         const uint32_t idesc_s = umma_idesc(BF16, 128, kPtKeys), idesc_o = umma_idesc(BF16, 128, hd16) | (1u << 16);
         const int ksteps = hd16 >> 4;
         const uint32_t q_a = smem_u32(q_s), ring_a = smem_u32(ring);
-        int slot = 0, par = 0;
-        bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag, p.status));
+        int slot = 0, par = 0, done[2] = {0, 0};                   // blocks of the two tiles so far
+        bool ok = true;
         auto take = [&](uint32_t& addr, int& at) {
             at = slot;
             addr = ring_a + (uint32_t)slot * kTile;
@@ -405,150 +479,166 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             }
             __syncwarp();
         };
-        uint32_t k_addr = 0, v_addr = 0;
-        int k_slot = 0, v_slot = 0;
-        if (ok) take(k_addr, k_slot);
-        if (ok) {
-            scores(0, k_addr);
-            if (nblk[1]) scores(1, k_addr);
-            if (elect_one()) umma_commit(&empty[k_slot]);
-            __syncwarp();
-        }
-        for (int j = 0; ok && j < nmax; ++j) {
-            take(v_addr, v_slot);
-            const bool more = j + 1 < nmax;
-            if (ok && more) take(k_addr, k_slot);
-            for (int x = 0; ok && x < 2; ++x) {
-                if (j >= nblk[x]) continue;
-                ok = __all_sync(0xffffffffu, mbar_wait_poll(&p_full[x], j & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
-                if (!ok) break;
-                tc_fence_after();
+        PromptItem w;
+        for (int it = 0; ok && next_item(it, w); ++it) {
+            const int nblk[2] = {blocks_of(w, 0), blocks_of(w, 1)}, nmax = max(nblk[0], nblk[1]);
+            ok = __all_sync(0xffffffffu, mbar_wait(q_full, it & 1, abort_flag, p.status));
+            uint32_t k_addr = 0, v_addr = 0;
+            int k_slot = 0, v_slot = 0;
+            if (ok) take(k_addr, k_slot);
+            if (ok) {
+                scores(0, k_addr);
+                if (nblk[1]) scores(1, k_addr);
                 if (elect_one()) {
-                    for (int s = 0; s < kPtKeys / 16; ++s)
-                        umma_f16_ts(tmem + kPtO + 128 * x, tmem + 128 * x + 8 * s, desc_mn(v_addr + s * 2048), idesc_o, j > 0 || s > 0);
-                    if (j + 1 == nblk[x]) umma_commit(&o_done[x]);
+                    umma_commit(&empty[k_slot]);
+                    if (nmax == 1) umma_commit(q_empty);
                 }
                 __syncwarp();
-                if (j + 1 < nblk[x]) scores(x, k_addr);
             }
-            if (ok && elect_one()) {
-                umma_commit(&empty[v_slot]);
-                if (more) umma_commit(&empty[k_slot]);
+            for (int j = 0; ok && j < nmax; ++j) {
+                take(v_addr, v_slot);
+                const bool more = j + 1 < nmax;
+                if (ok && more) take(k_addr, k_slot);
+                for (int x = 0; ok && x < 2; ++x) {
+                    if (j >= nblk[x]) continue;
+                    ok = __all_sync(0xffffffffu, mbar_wait_poll(&p_full[x], done[x] & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+                    if (!ok) break;
+                    ++done[x];
+                    tc_fence_after();
+                    if (elect_one()) {
+                        for (int s = 0; s < kPtKeys / 16; ++s)
+                            umma_f16_ts(tmem + kPtO + 128 * x, tmem + 128 * x + 8 * s, desc_mn(v_addr + s * 2048), idesc_o, j > 0 || s > 0);
+                        if (j + 1 == nblk[x]) umma_commit(&o_done[x]);
+                    }
+                    __syncwarp();
+                    if (j + 1 < nblk[x]) scores(x, k_addr);
+                }
+                if (ok && elect_one()) {
+                    umma_commit(&empty[v_slot]);
+                    if (more) umma_commit(&empty[k_slot]);
+                    if (j + 2 == nmax) umma_commit(q_empty);       // (the last scores have been formed)
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
     } else {                                                       // ---- softmax ----
         const int x = warp >> 2, row = (warp & 3) * 32 + lane;
-        const int t = row / group, tok = tok0 + x * tt + min(t, ntok[x] - 1), n = nblk[x], head = kvh * group + row - t * group;
-        const bool in = t < ntok[x];
-        const int low = tok0 + x * tt;                             // the tile's first row
-        const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * x, to = ts - 128 * x + kPtO + 128 * x;
+        const int t = row / group, g = row - t * group;
+        const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * x, to = ts + kPtO;
         const float sc = p.scale_log2e;
-        float m = -kInf, l = 0.0f;
+        const bool vec = (((uintptr_t)p.out | (p.out_stride * 2)) & 15) == 0;
+        int done = 0, tiles = 0;                                   // blocks and tiles so far
         bool ok = true;
-        for (int j = 0; j < n; ++j) {
-            ok = __all_sync(0xffffffffu, mbar_wait_poll(&s_full[x], j & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t s[4][32];
+        PromptItem w;
+        for (int it = 0; ok && next_item(it, w); ++it) {
+            const int ntok = tokens_of(w, x), n = blocks_of(w, x), low = w.tok0 + x * tt;      // low: the tile's first row
+            const int tok = low + min(t, max(ntok, 1) - 1), head = w.kvh * group + g;
+            const bool in = t < ntok;
+            float m = -kInf, l = 0.0f;
+            for (int j = 0; j < n; ++j, ++done) {
+                ok = __all_sync(0xffffffffu, mbar_wait_poll(&s_full[x], done & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t s[4][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
-            tmem_ld_wait();
-            const int key0 = j * kPtKeys;
-            if (key0 + kPtKeys - 1 > low) {                        // keys behind some row's own
-                const int lim = tok - key0;
+                for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+                tmem_ld_wait();
+                const int key0 = j * kPtKeys;
+                if (key0 + kPtKeys - 1 > low) {                    // keys behind some row's own
+                    const int lim = tok - key0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[c][i] = 32 * c + i <= lim ? s[c][i] : 0xff800000u;
+                }
+                float mx[4] = {m, m, m, m};
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c][i] = 32 * c + i <= lim ? s[c][i] : 0xff800000u;
-            }
-            float mx[4] = {m, m, m, m};
+                    for (int i = 0; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                const float now = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+                const bool far = (now - m) * sc > kLazy;           // (from -inf: inf; -inf to -inf: NaN, no)
+                if (j == 0) {
+                    m = now;
+                } else if (__any_sync(0xffffffffu, far)) {
+                    const float f = far ? ex2((m - now) * sc) : 1.0f;
+                    if (far) m = now;
+                    l *= f;
+                    const uint64_t f2 = pack64(f, f);
+                    for (int c = 0; c < hd16; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(to + c, o);
+                        tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-            const float now = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-            const bool far = j == 0 ? true : (now - m) * sc > kLazy;              // (from -inf: inf; -inf to -inf: NaN, no)
-            if (j == 0) {
-                m = now;
-            } else if (__any_sync(0xffffffffu, far)) {
-                const float f = far ? ex2((m - now) * sc) : 1.0f;
-                if (far) m = now;
-                l *= f;
-                const uint64_t f2 = pack64(f, f);
-                for (int c = 0; c < hd16; c += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(to + c, o);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float u, v;
-                        unpack64(mul2(pack64(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), f2), u, v);
-                        o[i] = __float_as_uint(u);
-                        o[i + 1] = __float_as_uint(v);
+                        for (int i = 0; i < 16; i += 2) {
+                            float u, v;
+                            unpack64(mul2(pack64(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), f2), u, v);
+                            o[i] = __float_as_uint(u);
+                            o[i + 1] = __float_as_uint(v);
+                        }
+                        tmem_st16(to + c, o);
                     }
-                    tmem_st16(to + c, o);
                 }
-            }
-            const float ref = m == -kInf ? 0.0f : m * sc;
-            const uint64_t sc2 = pack64(sc, sc), ref2 = pack64(-ref, -ref);
-            uint64_t sum[2] = {0, 0};
+                const float ref = m == -kInf ? 0.0f : m * sc;
+                const uint64_t sc2 = pack64(sc, sc), ref2 = pack64(-ref, -ref);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t w[16];
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t e[16];
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    float u, v;
-                    unpack64(fma2(pack64(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, ref2), u, v);
-                    u = ex2(u);
-                    v = ex2(v);
-                    sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack64(u, v));
-                    w[i / 2] = pack2_t<BF16>(u, v);
+                    for (int i = 0; i < 32; i += 2) {
+                        float u, v;
+                        unpack64(fma2(pack64(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, ref2), u, v);
+                        u = ex2(u);
+                        v = ex2(v);
+                        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack64(u, v));
+                        e[i / 2] = pack2_t<BF16>(u, v);
+                    }
+                    tmem_st16(ts + 16 * c, e);
                 }
-                tmem_st16(ts + 16 * c, w);
+                tmem_st_wait();
+                float u, v;
+                unpack64(add2(sum[0], sum[1]), u, v);
+                l += u + v;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x]);
             }
-            tmem_st_wait();
-            float u, v;
-            unpack64(add2(sum[0], sum[1]), u, v);
-            l += u + v;
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[x]);
-        }
-        if (n > 0) {
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(&o_done[x], 0, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+            if (!ok || n == 0) continue;
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], tiles & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+            ++tiles;
+            if (!ok) break;
             tc_fence_after();
             const float inv = __fdiv_rn(1.0f, l);
-            uint16_t* dst = p.out + (size_t)(first + tok) * p.out_stride + (size_t)head * hd;
+            uint16_t* dst = p.out + (size_t)(w.first + tok) * p.out_stride + (size_t)head * hd;
             bool bad = false;
-            const bool vec = (((uintptr_t)p.out | (p.out_stride * 2)) & 15) == 0;
-            for (int c = 0; ok && c < hd16; c += 16) {
+            for (int c = 0; c < hd16; c += 16) {
                 uint32_t o[16];
                 tmem_ld16(to + c, o);
                 tmem_ld_wait();
-                uint32_t w[8];
+                uint32_t e[8];
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float u = __uint_as_float(o[i]) * inv, v = __uint_as_float(o[i + 1]) * inv;
                     bad = bad || !(fabsf(u) <= 3.402823466e38f) || !(fabsf(v) <= 3.402823466e38f);
-                    w[i / 2] = pack2_t<BF16>(u, v);
+                    e[i / 2] = pack2_t<BF16>(u, v);
                 }
                 if (!in) continue;
                 if (vec) {
-                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                    if (c + 8 < hd) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(e[0], e[1], e[2], e[3]);
+                    if (c + 8 < hd) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(e[4], e[5], e[6], e[7]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (c + i < hd) dst[c + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+                        if (c + i < hd) dst[c + i] = (uint16_t)(e[i / 2] >> (16 * (i & 1)));
                 }
             }
-            unsigned mask = __ballot_sync(0xffffffffu, ok && in && bad && l > 0.0f);
-            if (mask && any_bad_value(p, kvh, first + low + 1, min(first + n * kPtKeys, p.rows)))
+            unsigned mask = __ballot_sync(0xffffffffu, in && bad && l > 0.0f);
+            if (mask && any_bad_value(p, w.kvh, w.first + low + 1, min(w.first + n * kPtKeys, p.rows)))
                 for (; mask; mask &= mask - 1) {
                     const int r = __ffs(mask) - 1, tk = __shfl_sync(0xffffffffu, tok, r), h = __shfl_sync(0xffffffffu, head, r);
                     __syncwarp();
-                    exact_row<BF16>(p, first, first + tk, h);
+                    exact_row<BF16>(p, w.first, w.first + tk, h);
                 }
         }
         tc_fence_before();
