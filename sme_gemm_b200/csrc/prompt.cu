@@ -301,29 +301,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// 2^x of two numbers on the multiply-add pipe: x = n + f with n the nearest integer (Cody and Waite's reduction, by adding 1.5 * 2^23), the
-// polynomial of degree 4 with the least relative error of 2^f over [-1/2, 1/2] (2.6e-6, fitted by iteratively reweighted least squares), times 2^n
-// put together as bits.  Below 2^-126 it is 2^-126; a NaN stays one.  The exponential unit takes a warp's instruction every eight cycles, which for a block's
-// 16384 scores is as long as its products take; two of 16 pairs go this way instead
-// (us at none, two, four, six of 16 pairs: eleven prompts of 640 rows 81, 73, 77, 83; 8192 rows, under the power cap, 462, 473, 488, 498).
-constexpr unsigned kPoly = 0x0808;                // which ones of 16 pairs, bit by bit
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-    const uint64_t magic = pack64(12582912.0f, 12582912.0f), back = pack64(-12582912.0f, -12582912.0f);
-    float a, b;
-    unpack64(x, a, b);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.0f));
-    x = pack64(a, b);
-    const uint64_t r = add2(x, magic), n = add2(r, back);
-    const uint64_t f = fma2(n, pack64(-1.0f, -1.0f), x);
-    uint64_t y = fma2(pack64(0.00957010143f, 0.00957010143f), f, pack64(0.0559178603f, 0.0559178603f));
-    y = fma2(y, f, pack64(0.240247448f, 0.240247448f));
-    y = fma2(y, f, pack64(0.693121815f, 0.693121815f));
-    y = fma2(y, f, pack64(0.999999261f, 0.999999261f));
-    unpack64(r, a, b);
-    return mul2(y, pack64(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
-}
-
 struct PromptTc {
     CUtensorMap q, k, v;
     PromptArgs p;
@@ -610,18 +587,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                     uint32_t e[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        uint64_t y = fma2(pack64(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, ref2);
+                        const uint64_t y = fma2(pack64(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, ref2);
                         float u, v;
-                        if (kPoly >> (i / 2) & 1) {
-                            y = exp2_poly(y);
-                            unpack64(y, u, v);
-                        } else {
-                            unpack64(y, u, v);
-                            u = ex2(u);
-                            v = ex2(v);
-                            y = pack64(u, v);
-                        }
-                        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], y);
+                        unpack64(y, u, v);
+                        u = ex2(u);
+                        v = ex2(v);
+                        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack64(u, v));
                         e[i / 2] = pack2_t<BF16>(u, v);
                     }
                     tmem_st16(ts + 16 * c, e);
