@@ -1117,13 +1117,26 @@ class SelfAttention:
     """A transformer self-attention block added into a residual stream (SelfAttention, src/self_attention.rs:66-231, its
     separate-steps path): the fused qkv projection ([q | k | v] in head order), the new positions' keys and values
     appended to a KvCache, causal attention over the cache, and the out projection: y += out(attention(q, K, V)).  No
-    rotary embedding, as there."""
+    rotary embedding, as there, unless with_rotary gives one; accumulate_batch runs a packed batch of sequences against an
+    8-bit PagedKvCache."""
 
     def __init__(self, qkv: Linear, out: Linear, heads: int, kv_heads: int, head_dim: int):
         assert kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "heads must be a positive multiple of kv_heads"
         assert qkv.n() == (heads + 2 * kv_heads) * head_dim, "qkv has (heads + 2 * kv_heads) * head_dim outputs"
         assert out.k() == heads * head_dim, "out takes heads * head_dim inputs"
         self.qkv, self.out, self._heads, self._kv_heads, self._head_dim = qkv, out, heads, kv_heads, head_dim
+        self.rotary = self.q_norm = self.k_norm = None
+        self._turns = False                                  # rotated or normalised heads
+
+    def with_rotary(self, rotary, q_norm=None, k_norm=None) -> "SelfAttention":
+        """The queries and keys of the block normalised per head (q_norm, k_norm: RMS norms of head_dim weights, or None) and rotated by
+        their positions (a Rotary, or None: the norms alone)."""
+        assert rotary is None or (isinstance(rotary, _paged.Rotary) and rotary.head_dim() == self._head_dim), "the rotation is one of heads of head_dim"
+        for norm in (q_norm, k_norm):
+            assert norm is None or (norm.is_rms and norm.width() == self._head_dim), "the heads' norms are RMS norms of head_dim weights"
+        self.rotary, self.q_norm, self.k_norm = rotary, q_norm, k_norm
+        self._turns = any(x is not None for x in (rotary, q_norm, k_norm))
+        return self
 
     @staticmethod
     def new(qkv: Linear, out: Linear, heads: int, kv_heads: int, head_dim: int) -> "SelfAttention":
@@ -1150,6 +1163,9 @@ class SelfAttention:
         w = q_len + 2 * kv_len
         qkv = torch.empty((m, w), dtype=torch.float16, device=x.device)
         self.qkv.forward(x, qkv, m)
+        if self._turns and m:
+            q, k = qkv[:, :q_len], qkv[:, q_len:q_len + kv_len]
+            _paged.rotate_heads(q, k, cache.len(), self.rotary, q, k, q_norm=self.q_norm, k_norm=self.k_norm, head_dim=self._head_dim)
         cache.extend_from(qkv, w, q_len, q_len + kv_len, m)
         att = torch.empty((m, q_len), dtype=torch.float16, device=x.device)
         cache._attend(qkv, w, m, att)                       # the queries are the first q_len values of each projected row
@@ -1159,6 +1175,37 @@ class SelfAttention:
         """y (m x out.n f32) += out(attention(qkv(x))) for m rows of f16 x at the cache's next positions, which this appends."""
         assert _numel(y) == m * self.out.n(), "y is m * out.n()"
         self.out.accumulate(self.attend(x, cache, m), y, m)
+
+    def paged_cache(self, pages: int, page: int = 64) -> "_paged.PagedKvCache":
+        """An 8-bit cache of pages for this block's heads."""
+        return _paged.PagedKvCache(self._heads, self._kv_heads, self._head_dim, pages, page)
+
+    def attend_batch(self, x, cache, batch, m: int, fresh: bool = False):
+        """attend() for the m packed rows of a PagedBatch against a PagedKvCache: their heads normalised and rotated at the sequences' positions, keys and
+        values appended to the pages.  fresh: every sequence starts at position 0, so that the rows attend to one another's 16-bit keys and
+        values and not to the codes.  Rows behind the last sequence come out as zeros."""
+        assert _is_torch(x) and x.dtype == torch.float16 and _numel(x) == m * self.width(), "x is m * width"
+        assert cache.heads() == self._heads and cache.kv_heads() == self._kv_heads and cache.head_dim() == self._head_dim, \
+            "the cache's heads match the block's"
+        q_len, kv_len = self._heads * self._head_dim, self._kv_heads * self._head_dim
+        qkv = torch.empty((m, q_len + 2 * kv_len), dtype=torch.float16, device=x.device)
+        self.qkv.forward(x, qkv, m)
+        q, k, v = qkv[:, :q_len], qkv[:, q_len:q_len + kv_len], qkv[:, q_len + kv_len:]
+        if self._turns:
+            cache.append(k, v, batch, self.rotary, q=q, q_out=q, k_out=k if fresh else None, q_norm=self.q_norm, k_norm=self.k_norm)
+        else:
+            cache.append(k, v, batch)
+        att = torch.zeros((m, q_len), dtype=torch.float16, device=x.device)
+        if fresh:
+            _paged.attend_packed(q, k, v, batch.cu_rows, att, self._heads, self._kv_heads, scale=cache.scale())
+        else:
+            cache.attend(q, batch, att)
+        return att
+
+    def accumulate_batch(self, x, cache, batch, y, m: int, fresh: bool = False) -> None:
+        """y (m x out.n f32) += out(attention(qkv(x))) for the m packed rows of a batch (attend_batch)."""
+        assert _numel(y) == m * self.out.n(), "y is m * out.n()"
+        self.out.accumulate(self.attend_batch(x, cache, batch, m, fresh), y, m)
 
 
 class Block:
@@ -1190,7 +1237,7 @@ class Block:
         device); False leaves every other form to its parts.  The same kernels in the same order, without a Python call and
         an allocation around each: a 384-wide layer at one row is 8 launches of 2-3 us."""
         n1, attn, n2, mlp = self.norm1, self.attn, self.norm2, self.mlp
-        if type(attn) is not SelfAttention or type(mlp) is not Mlp or type(n1) is not Norm or type(n2) is not Norm:
+        if type(attn) is not SelfAttention or type(mlp) is not Mlp or type(n1) is not Norm or type(n2) is not Norm or attn._turns:
             return False
         up = mlp.up
         gated = type(up) is GatedLinear
@@ -1234,6 +1281,16 @@ class Block:
         self.norm2.forward(x, h)
         self.mlp.accumulate(h, x, rows)
 
+    def accumulate_batch(self, x, cache, batch, rows: int, fresh: bool = False) -> None:
+        """accumulate for the packed rows of a PagedBatch against a PagedKvCache (SelfAttention.accumulate_batch)."""
+        assert _is_torch(x) and x.dtype == torch.float32 and x.numel() == rows * self.width(), "x is rows * width"
+        assert self.attn is not None, "this block was built without its attention half"
+        h = torch.empty((rows, self.width()), dtype=torch.float16, device=x.device)
+        self.norm1.forward(x, h)
+        self.attn.accumulate_batch(h, cache, batch, x, rows, fresh)
+        self.norm2.forward(x, h)
+        self.mlp.accumulate(h, x, rows)
+
 
 def last_status() -> int:
     return int(lib().smeg_last_status())
@@ -1243,3 +1300,6 @@ def device_info():
     sm, mem = C.c_int(), C.c_size_t()
     check("smeg_device_info", lib().smeg_device_info(C.byref(sm), C.byref(mem)))
     return sm.value, mem.value
+
+
+from . import paged as _paged  # noqa: E402  (its classes build on the ones above)

@@ -619,6 +619,94 @@ def test_two_streams_at_once_and_a_repeat_give_the_same_bits():
     assert all(torch.equal(o, outs[0]) for o in outs)
 
 
+def _layer(gen, d, heads, kv, hd, rotary, norms):
+    w = lambda n, k: (torch.randn(n, k, generator=gen, device="cuda") * k ** -0.5).cpu().numpy()  # noqa: E731
+    lin = lambda n, k: sg.Linear.quantize(w(n, k), sg.WeightLayout.OutIn, n, k)  # noqa: E731
+    attn = sg.SelfAttention.new(lin((heads + 2 * kv) * hd, d), lin(d, heads * hd), heads, kv, hd)
+    if rotary is not None or norms:
+        attn.with_rotary(rotary, *((_norm(gen, hd), _norm(gen, hd)) if norms else (None, None)))
+    n1, n2 = (sg.Norm.rms(np.ones(d, np.float32), 1e-6) for _ in range(2))
+    mlp = sg.Mlp.gated(sg.GatedLinear.quantize(w(3 * d // 2, d), w(3 * d // 2, d), sg.WeightLayout.OutIn, 3 * d // 2, d, sg.Gate.Silu), lin(d, 3 * d // 2))
+    return sg.Block.new(n1, attn, n2, mlp)
+
+
+@pytest.mark.parametrize("rotate,norms", [(True, True), (True, False), (False, True), (False, False)])
+def test_layer_on_a_packed_batch_is_its_parts(rotate, norms):
+    """Block.accumulate_batch: prompts, then a step with an idle sequence and a padded row, the same bits as its parts run in turn."""
+    gen = _gen(51)
+    d, heads, kv, hd, page = 256, 4, 2, 64, 16
+    block = _layer(gen, d, heads, kv, hd, sg.Rotary(hd) if rotate else None, norms)
+    attn = block.attn
+    cache, parts = attn.paged_cache(40, page), attn.paged_cache(40, page)
+    table = torch.randperm(40, generator=gen, device="cuda")[:30].reshape(3, 10).to(torch.int32)
+    have = [0, 0, 0]
+    for rows, pad, idle, fresh in (([20, 1, 70], 0, (), True), ([1, 1, 1], 1, (1,), False), ([5, 0, 2], 2, (), False)):
+        m = sum(rows) + pad
+        batch = sg.PagedBatch(_int([0] + np.cumsum(rows).tolist()), _int([-1 if s in idle else n for s, n in enumerate(have)]), table)
+        x = torch.randn(m, d, generator=gen, device="cuda")
+        y = x.clone()
+        block.accumulate_batch(x, cache, batch, m, fresh)
+        h = torch.empty(m, d, dtype=F16, device="cuda")
+        block.norm1.forward(y, h)
+        qkv = torch.empty(m, (heads + 2 * kv) * hd, dtype=F16, device="cuda")
+        attn.qkv.forward(h, qkv, m)
+        q, k, v = qkv.split([heads * hd, kv * hd, kv * hd], 1)
+        q2, k2 = q.clone(), k.clone()
+        parts.append(k, v, batch, attn.rotary, q=q, q_out=q2, k_out=k2, q_norm=attn.q_norm, k_norm=attn.k_norm)
+        att = torch.zeros(m, heads * hd, dtype=F16, device="cuda")
+        if fresh:
+            sg.attend_packed(q2, k2, v, batch.cu_rows, att, heads, kv)
+        else:
+            parts.attend(q2, batch, att)
+        attn.out.accumulate(att, y, m)
+        block.norm2.forward(y, h)
+        block.mlp.accumulate(h, y, m)
+        assert torch.equal(x, y) and torch.equal(cache.codes, parts.codes) and torch.equal(cache.scales, parts.scales)
+        assert not att[sum(rows):].any()
+        have = [n + (0 if s in idle else r) for s, (n, r) in enumerate(zip(have, rows))]
+
+
+def test_rotated_layer_on_the_f16_cache():
+    """SelfAttention.with_rotary on a KvCache: prompt, then tokens, against the packed form of the whole sequence (the same rotated 16-bit rows; the f16 cache's attention is
+    within 2e-5 of the packed one's 64-bit result, whose own bound holds), and a Block of it, which runs by its parts."""
+    gen = _gen(52)
+    d, heads, kv, hd, n = 256, 4, 2, 64, 50
+    block = _layer(gen, d, heads, kv, hd, sg.Rotary(hd, rotary_dim=32).linear(2.0), True)
+    attn = block.attn
+    x = _randn(gen, n, d)
+    cache = attn.cache(n)
+    got = torch.cat([attn.attend(x[:41], cache, 41)] + [attn.attend(x[i:i + 1], cache, 1) for i in range(41, n)])
+    k, v = cache.keys(), cache.values()                          # rotated, as cached
+    qkv = torch.cat([torch.empty(0, (heads + 2 * kv) * hd, dtype=F16, device="cuda")] + [_forward(attn.qkv, x[a:b]) for a, b in [(0, 41)] + [(i, i + 1) for i in range(41, n)]])
+    pos = torch.arange(n, device="cuda")
+    want_k, tol_k = _turned(qkv[:, heads * hd:(heads + kv) * hd], hd, pos, attn.rotary, attn.k_norm)
+    _near(k, want_k, tol_k, F16)
+    q = torch.empty(n, heads * hd, dtype=F16, device="cuda")
+    sg.rotate_heads(qkv[:, :heads * hd], None, 0, attn.rotary, q, None, q_norm=attn.q_norm)
+    want, tol = _prompt(q, k, v, [n], heads, kv)
+    _near(got, want, tol + 2e-5 * (1 + want.abs()), F16)
+    # a whole layer: the native form does not take it, its parts do
+    y = torch.randn(9, d, generator=gen, device="cuda")
+    z, c1, c2 = y.clone(), block.cache(9), block.cache(9)
+    block.accumulate(y, c1, 9)
+    h = torch.empty(9, d, dtype=F16, device="cuda")
+    block.norm1.forward(z, h)
+    attn.accumulate(h, c2, z, 9)
+    block.norm2.forward(z, h)
+    block.mlp.accumulate(h, z, 9)
+    assert torch.equal(y, z)
+    with pytest.raises(AssertionError, match="heads of head_dim"):
+        attn.with_rotary(sg.Rotary(128))
+    with pytest.raises(AssertionError, match="RMS norms"):
+        attn.with_rotary(None, sg.Norm.rms(np.ones(32, np.float32), 1e-6))
+
+
+def _forward(lin, x):
+    y = torch.empty(len(x), lin.n(), dtype=F16, device="cuda")
+    lin.forward(x.contiguous(), y, len(x))
+    return y
+
+
 def test_refusals_with_tensors_on_the_device():
     cache = sg.PagedKvCache(4, 2, 32, 5, 16)
     assert (cache.heads(), cache.kv_heads(), cache.head_dim(), cache.pages(), cache.page(), cache.row_len(), cache.query_len()) == (4, 2, 32, 5, 16, 64, 128)
