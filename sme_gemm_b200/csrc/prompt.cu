@@ -249,7 +249,9 @@ __global__ void __launch_bounds__(kPwThreads) prompt_mma_kernel(const __grid_con
     }
 }
 
-// ---- heads of up to 128 depths, rows on 16-byte boundaries: tcgen05 ----
+// ---- rows on 16-byte boundaries: tcgen05 ----
+// Up to 128 depths two query tiles take turns: while one's scores are weighed, the other's products run.  Above, tensor memory holds the result of one tile and
+// two blocks of its scores: the next block's are formed while this one's are weighed.
 constexpr int kPtThreads = 320;                    // warps 0-3 and 4-7: softmax of the two query tiles, 8: TMA, 9: MMA
 constexpr int kPtKeys = 128;
 constexpr int kPtChunk = 128 * 128;                // bytes of 128 rows x 64 depths
@@ -333,7 +335,7 @@ __device__ __forceinline__ int taken_cta(uint32_t answer) {        // its index,
 
 template <int BF16, int NCH>
 __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptTc a) {
-    constexpr int kTile = NCH * kPtChunk;
+    constexpr int kTile = NCH * kPtChunk, kTiles = NCH <= 2 ? 2 : 1;
     const PromptArgs& p = a.p;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
              *item_full = o_done + 2, *item_empty = item_full + 2, *taken = item_empty + 2;
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     const int hd = p.head_dim, hd16 = (hd + 15) & ~15, group = p.heads / p.kv_heads, tt = a.tokens;
-    unsigned char *q_s = smem, *ring = smem + 2 * kTile;
+    unsigned char *q_s = smem, *ring = smem + kTiles * kTile;
 
     if (tid == 0) {
         abort_word = 0;
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         if (lane == 0) mbar_arrive(&item_empty[k]);
         return w.rows >= 0;
     };
-    auto tokens_of = [&](const PromptItem& w, int x) { return max(0, min(tt, w.rows - w.tok0 - x * tt)); };
+    auto tokens_of = [&](const PromptItem& w, int x) { return kTiles == 1 && x ? 0 : max(0, min(tt, w.rows - w.tok0 - x * tt)); };
     auto blocks_of = [&](const PromptItem& w, int x) {
         const int n = tokens_of(w, x);
         return n ? (w.tok0 + x * tt + n - 1) / kPtKeys + 1 : 0;
@@ -411,14 +413,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 for (int s0 = 0; s0 < p.seqs.seqs; s0 += 32) {
                     const int s = s0 + lane;
                     int f = 0;
-                    n += __popc(__ballot_sync(0xffffffffu, s < p.seqs.seqs && (seq_rows(p.seqs, s, &f), first_slot_of(f, s, 2 * tt) <= slot_id)));
+                    n += __popc(__ballot_sync(0xffffffffu, s < p.seqs.seqs && (seq_rows(p.seqs, s, &f), first_slot_of(f, s, kTiles * tt) <= slot_id)));
                 }
                 if (n > 0) {
                     const int rows = seq_rows(p.seqs, n - 1, &w.first);
-                    const long long piece = slot_id - first_slot_of(w.first, n - 1, 2 * tt);
-                    if (piece >= 0 && piece < pieces_of(rows, 2 * tt)) {
+                    const long long piece = slot_id - first_slot_of(w.first, n - 1, kTiles * tt);
+                    if (piece >= 0 && piece < pieces_of(rows, kTiles * tt)) {
                         w.rows = rows;
-                        w.tok0 = (int)(piece * 2 * tt);
+                        w.tok0 = (int)(piece * kTiles * tt);
                     }
                 }
             }
@@ -442,7 +444,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                         for (int c = 0; c < NCH; ++c) tma_4d(q_s + x * kTile + c * kPtChunk, &a.q, c * 64, 0, w.kvh, w.first + w.tok0 + x * tt, q_full);
                 }
                 __syncwarp();
-                for (int j = 0; ok && j < n; ++j) ok = load(&a.k, w, j) && load(&a.v, w, j);
+                if (kTiles == 2) {
+                    for (int j = 0; ok && j < n; ++j) ok = load(&a.k, w, j) && load(&a.v, w, j);
+                } else {
+                    ok = load(&a.k, w, 0);
+                    for (int j = 0; ok && j < n; ++j) ok = (j + 1 == n || load(&a.k, w, j + 1)) && load(&a.v, w, j);
+                }
                 if (!ok) break;
             }
             if (elect_one()) {
@@ -469,13 +476,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             if (++slot == a.slots) { slot = 0; par ^= 1; }
             tc_fence_after();
         };
-        auto scores = [&](int x, uint32_t k_addr) {
+        auto scores = [&](int x, int buf, uint32_t k_addr) {           // of query tile x, into the columns of buffer buf
             if (elect_one()) {
                 for (int s = 0; s < ksteps; ++s) {
                     const uint32_t off = (uint32_t)((s >> 2) * kPtChunk + (s & 3) * 32);
-                    umma_f16(tmem + 128 * x, umma_desc_sw128(q_a + x * kTile + off), umma_desc_sw128(k_addr + off), idesc_s, s > 0);
+                    umma_f16(tmem + 128 * buf, umma_desc_sw128(q_a + x * kTile + off), umma_desc_sw128(k_addr + off), idesc_s, s > 0);
                 }
-                umma_commit(&s_full[x]);
+                umma_commit(&s_full[buf]);
             }
             __syncwarp();
         };
@@ -487,15 +494,41 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             int k_slot = 0, v_slot = 0;
             if (ok) take(k_addr, k_slot);
             if (ok) {
-                scores(0, k_addr);
-                if (nblk[1]) scores(1, k_addr);
+                scores(0, kTiles == 2 ? 0 : done[0] & 1, k_addr);
+                if (nblk[1]) scores(1, 1, k_addr);
                 if (elect_one()) {
                     umma_commit(&empty[k_slot]);
                     if (nmax == 1) umma_commit(q_empty);
                 }
                 __syncwarp();
             }
-            for (int j = 0; ok && j < nmax; ++j) {
+            if (kTiles == 1)
+                for (int j = 0; ok && j < nmax; ++j) {
+                    const int buf = done[0] & 1;
+                    if (j + 1 < nmax) {
+                        take(k_addr, k_slot);
+                        if (!ok) break;
+                        scores(0, buf ^ 1, k_addr);                // (behind the product that read this buffer's probabilities)
+                        if (elect_one()) {
+                            umma_commit(&empty[k_slot]);
+                            if (j + 2 == nmax) umma_commit(q_empty);
+                        }
+                        __syncwarp();
+                    }
+                    take(v_addr, v_slot);
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait_poll(&p_full[buf], (done[0] >> 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+                    if (!ok) break;
+                    ++done[0];
+                    tc_fence_after();
+                    if (elect_one()) {
+                        for (int s = 0; s < kPtKeys / 16; ++s)
+                            umma_f16_ts(tmem + kPtO, tmem + 128 * buf + 8 * s, desc_mn(v_addr + s * 2048), idesc_o, j > 0 || s > 0);
+                        umma_commit(&empty[v_slot]);
+                        umma_commit(&o_done[0]);
+                    }
+                    __syncwarp();
+                }
+            for (int j = 0; kTiles == 2 && ok && j < nmax; ++j) {
                 take(v_addr, v_slot);
                 const bool more = j + 1 < nmax;
                 if (ok && more) take(k_addr, k_slot);
@@ -511,7 +544,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                         if (j + 1 == nblk[x]) umma_commit(&o_done[x]);
                     }
                     __syncwarp();
-                    if (j + 1 < nblk[x]) scores(x, k_addr);
+                    if (j + 1 < nblk[x]) scores(x, x, k_addr);
                 }
                 if (ok && elect_one()) {
                     umma_commit(&empty[v_slot]);
@@ -524,7 +557,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     } else {                                                       // ---- softmax ----
         const int x = warp >> 2, row = (warp & 3) * 32 + lane;
         const int t = row / group, g = row - t * group;
-        const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * x, to = ts + kPtO;
+        const uint32_t ts0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * x, to = ts0 + kPtO;
         const float sc = p.scale_log2e;
         const bool vec = (((uintptr_t)p.out | (p.out_stride * 2)) & 15) == 0;
         int done = 0, tiles = 0;                                   // blocks and tiles so far
@@ -536,7 +569,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             const bool in = t < ntok;
             float m = -kInf, l = 0.0f;
             for (int j = 0; j < n; ++j, ++done) {
-                ok = __all_sync(0xffffffffu, mbar_wait_poll(&s_full[x], done & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+                // (one tile: the buffers take turns, the blocks before are done with where o_done says so)
+                const int buf = kTiles == 2 ? x : done & 1;
+                const uint32_t ts = kTiles == 2 ? ts0 : ts0 + 128 * buf;
+                ok = __all_sync(0xffffffffu, mbar_wait_poll(&s_full[buf], (kTiles == 2 ? done : done >> 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t s[4][32];
@@ -561,6 +597,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 if (j == 0) {
                     m = now;
                 } else if (__any_sync(0xffffffffu, far)) {
+                    if (kTiles == 1) {                             // (with two tiles the product before was done with when these scores were)
+                        ok = __all_sync(0xffffffffu, mbar_wait_poll(&o_done[0], (done - 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
                     const float f = far ? ex2((m - now) * sc) : 1.0f;
                     if (far) m = now;
                     l *= f;
@@ -603,10 +644,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 l += u + v;
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[x]);
+                if (lane == 0) mbar_arrive(&p_full[buf]);
             }
             if (!ok || n == 0) continue;
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], tiles & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], (kTiles == 2 ? tiles : done - 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
             ++tiles;
             if (!ok) break;
             tc_fence_after();
@@ -661,9 +702,9 @@ cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
     memset(&a, 0, sizeof(a));
     a.p = p;
     a.tokens = 128 / group;
-    a.slots = (int)((227 * 1024 - 2048 - 2 * NCH * kPtChunk) / (NCH * kPtChunk));
+    a.slots = (int)((227 * 1024 - 2048 - (NCH <= 2 ? 2 : 1) * NCH * kPtChunk) / (NCH * kPtChunk));
     if (a.slots > kPtMaxSlots) a.slots = kPtMaxSlots;
-    a.pieces = p.rows / (2 * a.tokens) + (long long)p.seqs.seqs;
+    a.pieces = p.rows / ((NCH <= 2 ? 2 : 1) * a.tokens) + (long long)p.seqs.seqs;
     if (a.pieces * p.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;
     const CUtensorMapDataType type = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const cuuint64_t hd = (cuuint64_t)p.head_dim;
@@ -679,7 +720,7 @@ cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaSuccess;
     auto kern = prompt_tc_kernel<BF16, NCH>;
-    const size_t smem = 1024 + (size_t)(2 + a.slots) * NCH * kPtChunk;
+    const size_t smem = 1024 + (size_t)((NCH <= 2 ? 2 : 1) + a.slots) * NCH * kPtChunk;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     *taken = true;
@@ -706,11 +747,11 @@ cudaError_t prompt_launch(PromptArgs a, int sm_count, cudaStream_t stream) {
     // rows and heads on 16-byte boundaries (what a tensor map needs), strides that it can hold, a positive scale (the maximum is taken before it)
     const bool aligned = ((a.q_stride | a.k_stride | a.v_stride) & 7) == 0 && (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0 &&
                          ((a.q_stride | a.k_stride | a.v_stride) >> 38) == 0;
-    if (aligned && a.head_dim <= 128 && a.scale_log2e > 0.0f && a.scale_log2e < 1e30f) {
+    if (aligned && a.scale_log2e > 0.0f && a.scale_log2e < 1e30f) {
         bool taken = false;
-        cudaError_t e;
-        if (a.bf16) e = a.head_dim <= 64 ? tc_launch<1, 1>(a, stream, &taken) : tc_launch<1, 2>(a, stream, &taken);
-        else e = a.head_dim <= 64 ? tc_launch<0, 1>(a, stream, &taken) : tc_launch<0, 2>(a, stream, &taken);
+        typedef cudaError_t (*Launch)(const PromptArgs&, cudaStream_t, bool*);
+        static const Launch launches[2][4] = {{tc_launch<0, 1>, tc_launch<0, 2>, tc_launch<0, 3>, tc_launch<0, 4>}, {tc_launch<1, 1>, tc_launch<1, 2>, tc_launch<1, 3>, tc_launch<1, 4>}};
+        const cudaError_t e = launches[a.bf16 ? 1 : 0][(a.head_dim + 63) / 64 - 1](a, stream, &taken);
         if (taken || e != cudaSuccess) return e;
     }
     if (a.bf16) return a.head_dim <= 64 ? mma_launch<1, 64>(a, stream) : (a.head_dim <= 128 ? mma_launch<1, 128>(a, stream) : mma_launch<1, 256>(a, stream));
