@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(kPwThreads) prompt_mma_kernel(const __grid_con
 constexpr int kPtThreads = 320;                    // warps 0-3 and 4-7: softmax of the two query tiles, 8: TMA, 9: MMA
 constexpr int kPtKeys = 128;
 constexpr int kPtChunk = 128 * 128;                // bytes of 128 rows x 64 depths
+constexpr int kPtStage = 32 * 128;                 // bytes of 32 rows x 64 results, where a softmax warp's turn from a row a lane to rows side by side
 constexpr int kPtMaxSlots = 10;
 constexpr uint32_t kPtO = 256;                     // tensor memory: scores / probabilities at columns 0 and 128, results behind them
 constexpr float kLazy = 8.0f;                      // a row's reference follows its maximum when that is 2^8 above it
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
              *item_full = o_done + 2, *item_empty = item_full + 2, *taken = item_empty + 2;
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     const int hd = p.head_dim, hd16 = (hd + 15) & ~15, group = p.heads / p.kv_heads, tt = a.tokens;
-    unsigned char *q_s = smem, *ring = smem + kTiles * kTile;
+    unsigned char *q_s = smem, *out_s = smem + kTiles * kTile, *ring = out_s + kTiles * 4 * kPtStage;
 
     if (tid == 0) {
         abort_word = 0;
@@ -652,29 +653,53 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             if (!ok) break;
             tc_fence_after();
             const float inv = __fdiv_rn(1.0f, l);
-            uint16_t* dst = p.out + (size_t)(w.first + tok) * p.out_stride + (size_t)head * hd;
-            bool bad = false;
-            for (int c = 0; c < hd16; c += 16) {
-                uint32_t o[16];
-                tmem_ld16(to + c, o);
+            const uint64_t inv2 = pack64(inv, inv);
+            const bool vec = (((uintptr_t)p.out | (p.out_stride * 2)) & 15) == 0;
+            const long long at = (long long)(w.first + tok) * (long long)p.out_stride + (long long)head * hd;
+            const unsigned rows_in = __ballot_sync(0xffffffffu, in);
+            const uint32_t mine = smem_u32(out_s) + warp * kPtStage;
+            uint64_t zero = 0;                                     // 0 * every result: not a number where one of them is not finite
+            for (int c0 = 0; c0 < hd; c0 += 64) {
+                uint32_t o[2][32];
+                tmem_ld32(to + c0, o[0]);                          // (what lies behind the head's depths is not used)
+                tmem_ld32(to + c0 + 32, o[1]);
                 tmem_ld_wait();
-                uint32_t e[8];
+                __syncwarp();                                      // (the stage's last reader is through)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float u = __uint_as_float(o[i]) * inv, v = __uint_as_float(o[i + 1]) * inv;
-                    bad = bad || !(fabsf(u) <= 3.402823466e38f) || !(fabsf(v) <= 3.402823466e38f);
-                    e[i / 2] = pack2_t<BF16>(u, v);
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint64_t y = mul2(pack64(__uint_as_float(o[c / 4][8 * (c % 4) + 2 * i]), __uint_as_float(o[c / 4][8 * (c % 4) + 2 * i + 1])), inv2);
+                        if (c0 + 8 * c < hd) zero = fma2(y, 0, zero);
+                        float u, v;
+                        unpack64(y, u, v);
+                        e[i] = pack2_t<BF16>(u, v);
+                    }
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]) : "memory");
                 }
-                if (!in) continue;
-                if (vec) {
-                    *reinterpret_cast<uint4*>(dst + c) = make_uint4(e[0], e[1], e[2], e[3]);
-                    if (c + 8 < hd) *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(e[4], e[5], e[6], e[7]);
-                } else {
+                __syncwarp();
+                const int c = c0 + 8 * (lane & 7);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (c + i < hd) dst[c + i] = (uint16_t)(e[i / 2] >> (16 * (i & 1)));
+                for (int i = 0; i < 8; ++i) {                      // four rows of 128 bytes at a time
+                    const int r = 4 * i + (lane >> 3);
+                    uint4 e;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(e.x), "=r"(e.y), "=r"(e.z), "=r"(e.w) : "r"(mine + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) : "memory");
+                    const long long to_row = __shfl_sync(0xffffffffu, at, r);
+                    if (!(rows_in >> r & 1) || c >= hd) continue;
+                    uint16_t* dst = p.out + to_row + c;
+                    if (vec) {
+                        *reinterpret_cast<uint4*>(dst) = e;
+                    } else {
+                        const uint32_t x4[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) dst[k] = (uint16_t)(x4[k / 2] >> (16 * (k & 1)));
+                    }
                 }
             }
+            float z0, z1;
+            unpack64(zero, z0, z1);
+            const bool bad = !(z0 + z1 == 0.0f);
             unsigned mask = __ballot_sync(0xffffffffu, in && bad && l > 0.0f);
             if (mask && any_bad_value(p, w.kvh, w.first + low + 1, min(w.first + n * kPtKeys, p.rows)))
                 for (; mask; mask &= mask - 1) {
@@ -694,6 +719,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
 
 template <int BF16, int NCH>
 cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
+    constexpr int kTiles = NCH <= 2 ? 2 : 1;
     *taken = false;
     TensorMapEncodeFn enc = tensor_map_encoder();
     const int group = p.heads / p.kv_heads;
@@ -702,9 +728,9 @@ cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
     memset(&a, 0, sizeof(a));
     a.p = p;
     a.tokens = 128 / group;
-    a.slots = (int)((227 * 1024 - 2048 - (NCH <= 2 ? 2 : 1) * NCH * kPtChunk) / (NCH * kPtChunk));
+    a.slots = (int)((227 * 1024 - 2048 - kTiles * (NCH * kPtChunk + 4 * kPtStage)) / (NCH * kPtChunk));
     if (a.slots > kPtMaxSlots) a.slots = kPtMaxSlots;
-    a.pieces = p.rows / ((NCH <= 2 ? 2 : 1) * a.tokens) + (long long)p.seqs.seqs;
+    a.pieces = p.rows / (kTiles * a.tokens) + (long long)p.seqs.seqs;
     if (a.pieces * p.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;
     const CUtensorMapDataType type = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const cuuint64_t hd = (cuuint64_t)p.head_dim;
@@ -720,7 +746,7 @@ cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaSuccess;
     auto kern = prompt_tc_kernel<BF16, NCH>;
-    const size_t smem = 1024 + (size_t)((NCH <= 2 ? 2 : 1) + a.slots) * NCH * kPtChunk;
+    const size_t smem = 1024 + (size_t)(kTiles + a.slots) * NCH * kPtChunk + kTiles * 4 * kPtStage;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     *taken = true;
