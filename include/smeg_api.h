@@ -320,8 +320,15 @@ int smeg_rotate_heads_dev(const smeg_rotate_args *a, void *stream);
  * as they are in q_out and k_out too. */
 int smeg_paged_append_dev(const smeg_rotate_args *a, void *stream);
 /* The values of n whole pages as 16-bit rows, out [n][kv_heads][keys, values][page][head_dim]; a page id outside the pool reads as zeros. */
-int smeg_paged_read_dev(uint16_t *out, const uint8_t *codes, const float *scales, const int32_t *ids, size_t n, size_t pages, size_t page,
-                        size_t kv_heads, size_t head_dim, int bf16, void *stream);
+typedef struct smeg_paged_read_args {
+    uint16_t *out;
+    const uint8_t *codes;
+    const float *scales;
+    const int32_t *ids;
+    size_t n, pages, page, kv_heads, head_dim;
+    int bf16, reserved;
+} smeg_paged_read_args;
+int smeg_paged_read_dev(const smeg_paged_read_args *a, void *stream);
 
 /* Attention of a batch's rows against the cache, which already holds them: row i of sequence s attends to positions 0..=starts[s] + i; per
  * head softmax(scale * q . k) @ v in 32 bits, one rounding.  Rows of idle sequences become zeros.  Query head h uses KV head h / (heads / kv_heads).

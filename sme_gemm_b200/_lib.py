@@ -50,9 +50,10 @@ class BlockArgs(C.Structure):
 # The same fields, packed by one call (0.3 us where filling a structure takes 1.6, of some 25 us of host work a layer at one row).
 BLOCK_ARGS = struct.Struct("@PNNPPPPffiiPPNNNPPNPPPfI")
 
-# smeg_rotate_args, smeg_paged_attend_args and smeg_attn_packed_args, packed the same way.
+# smeg_rotate_args, smeg_paged_attend_args, smeg_paged_read_args and smeg_attn_packed_args, packed the same way.
 ROTATE_ARGS = struct.Struct("@PPPPPNNNNNPPPPfffiiiNNNNNPqPPPNNPPNN")
 PAGED_ATTEND_ARGS = struct.Struct("@PPNNPPPPPNNNNNNNNfiPN")
+READ_ARGS = struct.Struct("@PPPPNNNNNii")
 ATTN_PACKED_ARGS = struct.Struct("@PPPPNNNNPNNNNNfi")
 
 assert BLOCK_ARGS.size == C.sizeof(BlockArgs) and BlockArgs.act.offset == BLOCK_ARGS.size - 4
@@ -134,7 +135,7 @@ SIGNATURES = {
     "smeg_attn_kv_causal_f16_dev": (_i, [_vp, _vp, _i, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, C.c_float, _vp]),
     "smeg_rotate_heads_dev": (_i, [_vp, _vp]),
     "smeg_paged_append_dev": (_i, [_vp, _vp]),
-    "smeg_paged_read_dev": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _i, _vp]),
+    "smeg_paged_read_dev": (_i, [_vp, _vp]),
     "smeg_paged_attend_workspace": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz, _sz]),
     "smeg_paged_attend_dev": (_i, [_vp, _vp]),
     "smeg_attn_packed_dev": (_i, [_vp, _vp]),

@@ -1362,14 +1362,16 @@ static int rotate_dev(const smeg_rotate_args* b, bool paged, cudaStream_t stream
 }
 int smeg_rotate_heads_dev(const smeg_rotate_args* a, void* stream) { return rotate_dev(a, false, (cudaStream_t)stream); }
 int smeg_paged_append_dev(const smeg_rotate_args* a, void* stream) { return rotate_dev(a, true, (cudaStream_t)stream); }
-int smeg_paged_read_dev(uint16_t* out, const uint8_t* codes, const float* scales, const int32_t* ids, size_t n, size_t pages, size_t page, size_t kv_heads,
-                        size_t head_dim, int bf16, void* stream) {
-    if (n == 0) return 0;
-    if (!out || !codes || !scales || !ids || !page_ok(page) || kv_heads == 0 || head_dim % 16 != 0 || head_dim < 16 || head_dim > 256 || ((uintptr_t)codes & 15) != 0) return -4;
-    if (kv_heads > 65535 || pages > 0x7fffffffu || n > 0x7fffffffu) return -3;
+int smeg_paged_read_dev(const smeg_paged_read_args* b, void* stream) {
+    if (!b) return -4;
+    if (b->n == 0) return 0;
+    if (!b->out || !b->codes || !b->scales || !b->ids || !page_ok(b->page) || b->kv_heads == 0) return -4;
+    if (b->head_dim % 16 != 0 || b->head_dim < 16 || b->head_dim > 256 || ((uintptr_t)b->codes & 15) != 0) return -4;
+    if (b->kv_heads > 65535 || b->pages > 0x7fffffffu || b->n > 0x7fffffffu) return -3;
     DeviceState* ds = dev_state();
     if (!ds) return -5;
-    const cudaError_t e = paged_read_launch(out, codes, scales, ids, n, (int)pages, (int)page, (int)kv_heads, (int)head_dim, bf16 != 0, ds->status, (cudaStream_t)stream);
+    const cudaError_t e = paged_read_launch(b->out, b->codes, b->scales, b->ids, b->n, (int)b->pages, (int)b->page, (int)b->kv_heads, (int)b->head_dim, b->bf16 != 0,
+                                            ds->status, (cudaStream_t)stream);
     return e == cudaSuccess ? 0 : (e == cudaErrorInvalidValue ? -3 : -6);
 }
 

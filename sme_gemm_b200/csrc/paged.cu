@@ -25,6 +25,8 @@
 
 #include <string.h>
 
+#include <atomic>
+
 namespace smeg {
 namespace {
 
@@ -780,8 +782,14 @@ cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t st
             HC == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
     const size_t smem = 1024 + (size_t)kPaWarps * (HC == 1 ? 4 : 3) * 4096 * HC;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+    static std::atomic<int> attr_dev{-1};          // the opt-in is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (attr_dev.load() != dev) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        attr_dev.store(dev);
+    }
     return launch_pdl(kern, dim3((unsigned)workers), dim3(kPaThreads), smem, stream, m, a);
 }
 

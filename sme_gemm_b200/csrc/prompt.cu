@@ -11,6 +11,8 @@
 
 #include <string.h>
 
+#include <atomic>
+
 namespace smeg {
 namespace {
 
@@ -747,8 +749,14 @@ cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
         return cudaSuccess;
     auto kern = prompt_tc_kernel<BF16, NCH>;
     const size_t smem = 1024 + (size_t)(kTiles + a.slots) * NCH * kPtChunk + kTiles * 4 * kPtStage;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+    static std::atomic<int> attr_dev{-1};          // the opt-in is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (attr_dev.load() != dev) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        attr_dev.store(dev);
+    }
     *taken = true;
     return launch_pdl(kern, dim3((unsigned)(a.pieces * p.kv_heads)), dim3(kPtThreads), smem, stream, a);
 }
@@ -757,8 +765,14 @@ template <int BF16, int HD>
 cudaError_t mma_launch(const PromptArgs& a, cudaStream_t stream) {
     auto kern = prompt_mma_kernel<BF16, HD>;
     const size_t smem = (size_t)(kPwRows + 2 * kPwKeys) * (HD + 8) * 2;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+    static std::atomic<int> attr_dev{-1};          // the opt-in is per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (attr_dev.load() != dev) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        attr_dev.store(dev);
+    }
     const long long slots = ((long long)a.rows * (a.heads / a.kv_heads) >> 6) + a.seqs.seqs;
     if (slots > 0x7fffffffll || a.kv_heads > 65535) return cudaErrorInvalidValue;
     const int vec_q = a.q_stride % 8 == 0 && ((uintptr_t)a.q & 15) == 0;

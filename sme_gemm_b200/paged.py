@@ -12,10 +12,11 @@ import math
 
 import numpy as np
 
-from ._lib import ATTN_PACKED_ARGS, PAGED_ATTEND_ARGS, ROTATE_ARGS, check, lib
+from ._lib import ATTN_PACKED_ARGS, PAGED_ATTEND_ARGS, READ_ARGS, ROTATE_ARGS, check, lib
 from .host import Norm, torch
 
-_DTYPES = (torch.float16, torch.bfloat16)
+_Tensor, _F16, _BF16 = torch.Tensor, torch.float16, torch.bfloat16
+_get_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 class _On:
@@ -34,40 +35,48 @@ class _On:
             torch.cuda.set_device(self._was)
 
 
+_FNS: dict = {}                                             # entry points by name
+
+
 def _enqueue(name: str, device: int, args: bytes) -> None:
     """Calls `name` with the packed arguments on the current stream of `device`."""
-    fn = getattr(lib(), name)
-    if torch._C._cuda_getDevice() == device:
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
+    fn = _FNS.get(name)
+    if fn is None:
+        fn = _FNS[name] = getattr(lib(), name)
+    if _get_device() == device:
+        rc = fn(args, _raw_stream(device))
     else:
         with _On(device):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
+            rc = fn(args, _raw_stream(device))
     if rc:
         check(name, rc)
 
 
 def _first_rows(x, what: str):
-    """(type, device index, number) of the rows that the other tensors of a call have to be like."""
+    """((type, device index), number, length) of the rows that the other tensors of a call have to be like."""
+    if type(x) is _Tensor:
+        dtype, shape, device = x.dtype, x.shape, x.get_device()
+        if (dtype is _F16 or dtype is _BF16) and device >= 0 and len(shape) == 2:
+            return (dtype, device), shape[0], shape[1]
     assert isinstance(x, torch.Tensor) and x.is_cuda, f"{what} is a CUDA tensor"
-    assert x.dtype in _DTYPES, f"{what} is f16 or bf16"
+    assert x.dtype in (_F16, _BF16), f"{what} is f16 or bf16"
     assert x.dim() == 2, f"{what} has rows"
-    return x.dtype, x.get_device(), x.shape[0]
+    return (x.dtype, x.get_device()), x.shape[0], x.shape[1]
 
 
-def _rows(x, what: str, width: int, like) -> int:
-    """Checks a tensor of rows; their stride in elements.  (A call is some eight of these checks, and a small one is over in the time they take: the
+def _rows(x, what: str, rows: int, width: int, like) -> int:
+    """Checks a tensor of rows; their stride in elements.  (A call is some five of these checks, and a small one is over in the time they take: the
     sound case is one condition, what is wrong is found afterwards.)"""
-    dtype, device, rows = like
-    if type(x) is torch.Tensor and x.dtype is dtype and x.get_device() == device and x.shape == (rows, width):
+    if type(x) is _Tensor and x.shape == (rows, width) and (x.dtype, x.get_device()) == like:
         stride, one = x.stride()
         if one == 1 and stride >= width:
             return stride
         if rows <= 1 and (one == 1 or width == 1):
             return width
     assert isinstance(x, torch.Tensor) and x.is_cuda, f"{what} is a CUDA tensor"
-    assert x.dtype in _DTYPES, f"{what} is f16 or bf16"
+    assert x.dtype in (_F16, _BF16), f"{what} is f16 or bf16"
     assert x.dim() == 2 and x.shape[1] == width, f"{what} has rows of {width} values"
-    assert x.dtype is dtype and x.get_device() == device, f"{what} has the same type and device as the other rows"
+    assert (x.dtype, x.get_device()) == like, f"{what} has the same type and device as the other rows"
     assert x.shape[0] == rows, f"{what} has as many rows as the others"
     stride, one = x.stride()
     assert rows <= 1 or stride >= width and one == 1 or width == 1, f"{what} has its rows' values side by side"
@@ -187,21 +196,24 @@ def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=N
     assert q is not None or k is not None, "there are queries or keys"
     assert (q is None) == (q_out is None), "q and q_out come together"
     assert (k is None) == (k_out is None), "k and k_out come together"
-    like = dtype, device, rows = _first_rows(q, "q") if q is not None else _first_rows(k, "k")
     q_ptr = k_ptr = qo_ptr = ko_ptr = qs = ks = qos = kos = heads = kv_heads = 0
+    like = None
     if q is not None:
-        width = q.shape[1]
+        like, rows, width = _first_rows(q, "q")
         heads = width // hd
         assert heads * hd == width and heads > 0, "q has rows of whole heads"
-        qs, qos = _rows(q, "q", width, like), _rows(q_out, "q_out", width, like)
+        qs, qos = _rows(q, "q", rows, width, like), _rows(q_out, "q_out", rows, width, like)
         q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     if k is not None:
-        _first_rows(k, "k")
-        width = k.shape[1]
+        if like is None:
+            like, rows, width = _first_rows(k, "k")
+        else:
+            width = _first_rows(k, "k")[2]
         kv_heads = width // hd
         assert kv_heads * hd == width and kv_heads > 0, "k has rows of whole heads"
-        ks, kos = _rows(k, "k", width, like), _rows(k_out, "k_out", width, like)
+        ks, kos = _rows(k, "k", rows, width, like), _rows(k_out, "k_out", rows, width, like)
         k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
+    dtype, device = like
     pos_ptr, start = 0, 0
     if isinstance(positions, torch.Tensor):
         _ints(positions, "positions", device)
@@ -215,7 +227,7 @@ def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=N
     if rows == 0:
         return
     _enqueue("smeg_rotate_heads_dev", device, ROTATE_ARGS.pack(
-        q_ptr, k_ptr, 0, qo_ptr, ko_ptr, qs, ks, 0, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, dtype is torch.bfloat16, 0, rot, rows, heads, kv_heads, hd,
+        q_ptr, k_ptr, 0, qo_ptr, ko_ptr, qs, ks, 0, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, dtype is _BF16, 0, rot, rows, heads, kv_heads, hd,
         pos_ptr, start, 0, 0, 0, 0, 0, 0, 0, 0, 0))
 
 
@@ -309,10 +321,10 @@ class PagedKvCache:
         return self._heads * self._head_dim
 
     def _like(self, x, what: str, batch):
-        like = _first_rows(x, what)
+        like, rows, _ = _first_rows(x, what)
         assert like[1] == self._device, "the rows are on the cache's device"
         assert isinstance(batch, PagedBatch) and batch._device == self._device, "the batch is on the cache's device"
-        return like
+        return like, rows
 
     def append(self, k, v, batch: PagedBatch, rotary: Rotary | None = None, *, k_norm=None, k_out=None, q=None, q_out=None, q_norm=None) -> None:
         """The rows k and v (kv_heads * head_dim values) to the pages of their sequences' positions; keys are normalised (k_norm) and rotated on the way.
@@ -320,32 +332,32 @@ class PagedKvCache:
         may be the inputs.  Rows of idle sequences and rows behind the last sequence are left as they are."""
         hd = self._head_dim
         row, device = self._kv_heads * hd, self._device
-        like = self._like(k, "k", batch)
-        ks, vs = _rows(k, "k", row, like), _rows(v, "v", row, like)
+        like, rows = self._like(k, "k", batch)
+        ks, vs = _rows(k, "k", rows, row, like), _rows(v, "v", rows, row, like)
         q_ptr = qo_ptr = ko_ptr = qs = qos = kos = 0
         if k_out is not None:
-            kos, ko_ptr = _rows(k_out, "k_out", row, like), k_out.data_ptr()
+            kos, ko_ptr = _rows(k_out, "k_out", rows, row, like), k_out.data_ptr()
         assert (q is None) == (q_out is None), "q and q_out come together"
         if q is not None:
             q_len = self._heads * hd
-            qs, qos = _rows(q, "q", q_len, like), _rows(q_out, "q_out", q_len, like)
+            qs, qos = _rows(q, "q", rows, q_len, like), _rows(q_out, "q_out", rows, q_len, like)
             q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
         turns, steps, rot, inter, factor = _rotation(rotary, hd, device)
         qn, qe = _head_norm(q_norm, "q_norm", hd, device)
         kn, ke = _head_norm(k_norm, "k_norm", hd, device)
-        if like[2] == 0 or batch._fields[3] == 0:
+        if rows == 0 or batch._fields[3] == 0:
             return
         _enqueue("smeg_paged_append_dev", device, ROTATE_ARGS.pack(
-            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, qs, ks, vs, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, like[0] is torch.bfloat16, 0, rot,
-            like[2], self._heads, self._kv_heads, hd, 0, 0, *batch._fields, *self._at, self._pages, self._page))
+            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, qs, ks, vs, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, like[0] is _BF16, 0, rot,
+            rows, self._heads, self._kv_heads, hd, 0, 0, *batch._fields, *self._at, self._pages, self._page))
 
     def attend(self, q, batch: PagedBatch, out) -> None:
         """out = the attention of the query rows (heads * head_dim values) against their sequences' cached positions, which already hold the rows' own
         (append, then attend, with the same batch): row i of a sequence attends to positions 0..=start + i.  Rows of idle sequences become
         zeros, rows behind the last sequence stay as they are."""
-        like = dtype, device, rows = self._like(q, "q", batch)
-        width = self._heads * self._head_dim
-        qs, os_ = _rows(q, "q", width, like), _rows(out, "out", width, like)
+        like, rows = self._like(q, "q", batch)
+        width, device = self._heads * self._head_dim, self._device
+        qs, os_ = _rows(q, "q", rows, width, like), _rows(out, "out", rows, width, like)
         cu, starts, table, seqs, cols = batch._fields
         if rows == 0 or seqs == 0:
             return
@@ -359,25 +371,19 @@ class PagedKvCache:
         ws = self._codes.new_empty(need) if need else None
         _enqueue("smeg_paged_attend_dev", device, PAGED_ATTEND_ARGS.pack(
             q.data_ptr(), out.data_ptr(), qs, os_, *self._at, cu, starts, table, seqs, cols, self._pages, self._page, rows, self._heads, self._kv_heads,
-            self._head_dim, self._scale, dtype is torch.bfloat16, ws.data_ptr() if need else 0, need))
+            self._head_dim, self._scale, like[0] is _BF16, ws.data_ptr() if need else 0, need))
 
     def read(self, ids, out) -> None:
         """The values of whole pages: out [n, kv_heads, 2, page, head_dim] (keys, values), contiguous f16 or bf16, for the n int32 page ids."""
         _ints(ids, "ids", self._device)
         n = ids.numel()
-        assert isinstance(out, torch.Tensor) and out.get_device() == self._device and out.dtype in _DTYPES and out.is_contiguous(), "out is contiguous f16 or bf16"
+        assert isinstance(out, torch.Tensor) and out.get_device() == self._device and out.dtype in (_F16, _BF16) and out.is_contiguous(), "out is contiguous f16 or bf16"
         assert out.numel() == n * self._kv_heads * 2 * self._page * self._head_dim, "out holds n pages"
         if n == 0:
             return
-        fn, device = lib().smeg_paged_read_dev, self._device
-        args = (out.data_ptr(), *self._at, ids.data_ptr(), n, self._pages, self._page, self._kv_heads, self._head_dim, out.dtype is torch.bfloat16)
-        if torch._C._cuda_getDevice() == device:
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
-        else:
-            with _On(device):
-                rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
-        if rc:
-            check("smeg_paged_read_dev", rc)
+        device = self._device
+        _enqueue("smeg_paged_read_dev", device, READ_ARGS.pack(out.data_ptr(), *self._at, ids.data_ptr(), n, self._pages, self._page, self._kv_heads, self._head_dim,
+                                                               out.dtype is _BF16, 0))
 
 
 def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float | None = None) -> None:
@@ -385,13 +391,13 @@ def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float
     its rows 0..=i.  q, out: rows of heads * head_dim values, k, v of kv_heads * head_dim, f16 or bf16, at any row stride; scale 1 / sqrt(head_dim).
     Rows behind the last sequence are left as they are."""
     assert kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "heads must be a positive multiple of kv_heads"
-    like = dtype, device, rows = _first_rows(q, "q")
-    width = q.shape[1]
+    like, rows, width = _first_rows(q, "q")
+    dtype, device = like
     hd = width // heads
     assert hd * heads == width, "q has rows of heads * head_dim values"
     assert hd % 8 == 0 and 8 <= hd <= 256, "head_dim must be a multiple of 8 in 8..=256"
     row = kv_heads * hd
-    qs, ks, vs, os_ = _rows(q, "q", width, like), _rows(k, "k", row, like), _rows(v, "v", row, like), _rows(out, "out", width, like)
+    qs, ks, vs, os_ = _rows(q, "q", rows, width, like), _rows(k, "k", rows, row, like), _rows(v, "v", rows, row, like), _rows(out, "out", rows, width, like)
     _ints(cu_rows, "cu_rows", device)
     seqs = cu_rows.numel() - 1
     assert seqs >= 0, "cu_rows has one value more than there are sequences"
@@ -399,4 +405,4 @@ def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float
         return
     _enqueue("smeg_attn_packed_dev", device, ATTN_PACKED_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, vs, os_, cu_rows.data_ptr(), seqs, rows, heads, kv_heads, hd,
-        hd ** -0.5 if scale is None else scale, dtype is torch.bfloat16))
+        hd ** -0.5 if scale is None else scale, dtype is _BF16))

@@ -87,8 +87,8 @@ static int shares(Batch& b, int group, int kv, int tile, int workers) {
 
 int main(int argc, char** argv) {
     if (argc > 1 && !std::strcmp(argv[1], "sizes")) {
-        std::printf("%zu %zu %zu %zu %zu\n", sizeof(smeg_rotate_args), offsetof(smeg_rotate_args, start), sizeof(smeg_paged_attend_args),
-                    offsetof(smeg_paged_attend_args, workspace_bytes), sizeof(smeg_attn_packed_args));
+        std::printf("%zu %zu %zu %zu %zu %zu\n", sizeof(smeg_rotate_args), offsetof(smeg_rotate_args, start), sizeof(smeg_paged_attend_args),
+                    offsetof(smeg_paged_attend_args, workspace_bytes), sizeof(smeg_attn_packed_args), sizeof(smeg_paged_read_args));
         return 0;
     }
     for (uint32_t d : {1u, 2u, 3u, 5u, 7u, 8u, 12u, 24u, 63u, 64u, 100u, 641u, 65535u})

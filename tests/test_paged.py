@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import sme_gemm_b200 as sg
-from sme_gemm_b200._lib import ATTN_PACKED_ARGS, PAGED_ATTEND_ARGS, ROTATE_ARGS
+from sme_gemm_b200._lib import ATTN_PACKED_ARGS, PAGED_ATTEND_ARGS, READ_ARGS, ROTATE_ARGS
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -32,7 +32,7 @@ def test_packed_arguments_are_the_structures(index_check):
     import struct
     start = struct.calcsize("@PPPPPNNNNNPPPPfffiiiNNNNNPq") - 8
     end = PAGED_ATTEND_ARGS.size - 8
-    assert got == [ROTATE_ARGS.size, start, PAGED_ATTEND_ARGS.size, end, ATTN_PACKED_ARGS.size]
+    assert got == [ROTATE_ARGS.size, start, PAGED_ATTEND_ARGS.size, end, ATTN_PACKED_ARGS.size, READ_ARGS.size]
 
 
 def test_frequencies_follow_their_definitions():
@@ -125,5 +125,7 @@ def test_prompt_attention_refuses_bad_arguments(kw, rc):
 def test_null_argument_structures_are_refused():
     L = sg.lib()
     assert [f(None, None) for f in (L.smeg_rotate_heads_dev, L.smeg_paged_append_dev, L.smeg_paged_attend_dev, L.smeg_attn_packed_dev)] == [-4] * 4
-    assert L.smeg_paged_read_dev(4096, 4096, 4096, 4096, 1, 5, 24, 2, 64, 0, None) == -4
-    assert L.smeg_paged_read_dev(4096, 4096, 4096, 4096, 0, 5, 64, 2, 64, 0, None) == 0
+    assert L.smeg_paged_read_dev(None, None) == -4
+    read = dict(out=4096, codes=4096, scales=4096, ids=4096, n=1, pages=5, page=64, kv_heads=2, head_dim=64, bf16=0, reserved=0)
+    for kw, rc in ((dict(page=24), -4), (dict(n=0), 0), (dict(out=0), -4), (dict(codes=4104), -4), (dict(head_dim=40), -4), (dict(kv_heads=0), -4), (dict(n=1 << 31), -3)):
+        assert L.smeg_paged_read_dev(READ_ARGS.pack(*{**read, **kw}.values()), None) == rc
