@@ -59,7 +59,32 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if rebuilt or not os.path.exists(LIB):
         cmd = [NVCC, "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-lpthread"]
         subprocess.check_call(cmd)
+    build_binding(force, verbose)
     return LIB
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """The Python module behind paged.py (csrc/binding.cc): links against torch, takes the library's entry points by address."""
+    import sysconfig
+
+    import torch                                               # (the one its headers belong to; it needs no GPU)
+    src = os.path.join(CSRC, "binding.cc")
+    api = os.path.join(os.path.dirname(HERE), "include", "smeg_api.h")
+    out = os.path.join(HERE, "_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(api)):
+        return out
+    root = os.path.dirname(torch.__file__)
+    inc = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    libs = os.path.join(root, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[x for i in inc for x in ("-isystem", i)], src, "-o", out, f"-L{libs}", f"-Wl,-rpath,{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if verbose or r.returncode:
+        sys.stderr.write(r.stdout)
+    if r.returncode:
+        raise RuntimeError("g++ failed on binding.cc")
+    return out
 
 
 if __name__ == "__main__":

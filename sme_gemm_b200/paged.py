@@ -8,80 +8,31 @@ captured into a graph (row offsets, starts and page tables are device memory).
 """
 from __future__ import annotations
 
+import ctypes
+import importlib
 import math
 
 import numpy as np
 
-from ._lib import ATTN_PACKED_ARGS, PAGED_ATTEND_ARGS, READ_ARGS, ROTATE_ARGS, check, lib
+from ._lib import check, lib
 from .host import Norm, torch
 
-_Tensor, _F16, _BF16 = torch.Tensor, torch.float16, torch.bfloat16
-_get_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_CALLS = None                                                # the compiled side of the calls: reads and checks tensors (csrc/binding.cc)
+_NO_ROTATION_YET = -1000                                     # from it: the rotation's table is not on the rows' device
 
 
-class _On:
-    """The tensors' device as the current one, for a call from elsewhere."""
-
-    def __init__(self, device: int):
-        self._device = device
-
-    def __enter__(self):
-        self._was = torch.cuda.current_device()
-        if self._was != self._device:
-            torch.cuda.set_device(self._device)
-
-    def __exit__(self, *exc):
-        if self._was != self._device:
-            torch.cuda.set_device(self._was)
-
-
-_FNS: dict = {}                                             # entry points by name
-
-
-def _enqueue(name: str, device: int, args: bytes) -> None:
-    """Calls `name` with the packed arguments on the current stream of `device`."""
-    fn = _FNS.get(name)
-    if fn is None:
-        fn = _FNS[name] = getattr(lib(), name)
-    if _get_device() == device:
-        rc = fn(args, _raw_stream(device))
-    else:
-        with _On(device):
-            rc = fn(args, _raw_stream(device))
-    if rc:
-        check(name, rc)
-
-
-def _first_rows(x, what: str):
-    """((type, device index), number, length) of the rows that the other tensors of a call have to be like."""
-    if type(x) is _Tensor:
-        dtype, shape, device = x.dtype, x.shape, x.get_device()
-        if (dtype is _F16 or dtype is _BF16) and device >= 0 and len(shape) == 2:
-            return (dtype, device), shape[0], shape[1]
-    assert isinstance(x, torch.Tensor) and x.is_cuda, f"{what} is a CUDA tensor"
-    assert x.dtype in (_F16, _BF16), f"{what} is f16 or bf16"
-    assert x.dim() == 2, f"{what} has rows"
-    return (x.dtype, x.get_device()), x.shape[0], x.shape[1]
-
-
-def _rows(x, what: str, rows: int, width: int, like) -> int:
-    """Checks a tensor of rows; their stride in elements.  (A call is some five of these checks, and a small one is over in the time they take: the
-    sound case is one condition, what is wrong is found afterwards.)"""
-    if type(x) is _Tensor and x.shape == (rows, width) and (x.dtype, x.get_device()) == like:
-        stride, one = x.stride()
-        if one == 1 and stride >= width:
-            return stride
-        if rows <= 1 and (one == 1 or width == 1):
-            return width
-    assert isinstance(x, torch.Tensor) and x.is_cuda, f"{what} is a CUDA tensor"
-    assert x.dtype in (_F16, _BF16), f"{what} is f16 or bf16"
-    assert x.dim() == 2 and x.shape[1] == width, f"{what} has rows of {width} values"
-    assert (x.dtype, x.get_device()) == like, f"{what} has the same type and device as the other rows"
-    assert x.shape[0] == rows, f"{what} has as many rows as the others"
-    stride, one = x.stride()
-    assert rows <= 1 or stride >= width and one == 1 or width == 1, f"{what} has its rows' values side by side"
-    assert one == 1 or width == 1 or rows == 0, f"{what} has its rows' values side by side"
-    return max(stride, width)
+def _calls():
+    global _CALLS
+    if _CALLS is None:
+        L = lib()
+        try:
+            m = importlib.import_module("._binding", __package__)
+        except ImportError as e:
+            raise RuntimeError("sme_gemm_b200/_binding is missing: build it with `python -m sme_gemm_b200.build`") from e
+        m.bind(*(ctypes.cast(getattr(L, "smeg_" + n), ctypes.c_void_p).value for n in (
+            "rotate_heads_dev", "paged_append_dev", "paged_attend_dev", "paged_attend_workspace", "attn_packed_dev", "paged_read_dev")))
+        _CALLS = m
+    return _CALLS
 
 
 def _ints(x, what: str, device: int) -> None:
@@ -89,14 +40,12 @@ def _ints(x, what: str, device: int) -> None:
     assert device is None or x.get_device() == device, f"{what} is on the rows' device"
 
 
-def _head_norm(norm, what: str, head_dim: int, device: int):
+def _head_norm(norm, what: str):
+    """(weights, eps) of a norm of the heads."""
     if norm is None:
-        return 0, 0.0
+        return None, 0.0
     assert isinstance(norm, Norm) and norm.is_rms, f"{what} is an RMS norm"
-    w = norm.weight
-    assert w.numel() == head_dim, f"{what} has head_dim weights"
-    assert w.get_device() == device, f"{what} is on the rows' device"
-    return w.data_ptr(), norm.eps
+    return norm.weight, norm.eps
 
 
 class Rotary:
@@ -115,6 +64,7 @@ class Rotary:
     def _set(self, frequencies, factor: float) -> None:
         self._frequencies, self._factor = frequencies, float(factor)
         self._turns = {}                                       # device -> turns per position, and where they are
+        self._call = self._turns, self._rot, self._interleaved, self._factor
 
     def _scaled(self, frequencies, factor: float = 1.0) -> "Rotary":
         r = Rotary(self._head_dim, self._base, self._rot, self._interleaved)
@@ -177,12 +127,11 @@ class Rotary:
         return t
 
 
-def _rotation(rotary, head_dim: int, device: int):
+def _rotation(rotary, head_dim: int):
     if rotary is None:
-        return 0, 0, 0, 0, 1.0
+        return None
     assert isinstance(rotary, Rotary) and rotary._head_dim == head_dim, "the rotation is one of heads of head_dim"
-    turns, steps, _, _ = rotary._on(device)
-    return turns, steps, rotary._rot, rotary._interleaved, rotary._factor
+    return rotary._call
 
 
 def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=None, head_dim: int | None = None) -> None:
@@ -193,42 +142,13 @@ def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=N
     hd = rotary._head_dim if rotary is not None else head_dim
     assert head_dim is None or head_dim == hd, "the rotation is one of heads of head_dim"
     assert hd % 8 == 0 and 8 <= hd <= 256, "head_dim must be a multiple of 8 in 8..=256"
-    assert q is not None or k is not None, "there are queries or keys"
-    assert (q is None) == (q_out is None), "q and q_out come together"
-    assert (k is None) == (k_out is None), "k and k_out come together"
-    q_ptr = k_ptr = qo_ptr = ko_ptr = qs = ks = qos = kos = heads = kv_heads = 0
-    like = None
-    if q is not None:
-        like, rows, width = _first_rows(q, "q")
-        heads = width // hd
-        assert heads * hd == width and heads > 0, "q has rows of whole heads"
-        qs, qos = _rows(q, "q", rows, width, like), _rows(q_out, "q_out", rows, width, like)
-        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
-    if k is not None:
-        if like is None:
-            like, rows, width = _first_rows(k, "k")
-        else:
-            width = _first_rows(k, "k")[2]
-        kv_heads = width // hd
-        assert kv_heads * hd == width and kv_heads > 0, "k has rows of whole heads"
-        ks, kos = _rows(k, "k", rows, width, like), _rows(k_out, "k_out", rows, width, like)
-        k_ptr, ko_ptr = k.data_ptr(), k_out.data_ptr()
-    dtype, device = like
-    pos_ptr, start = 0, 0
-    if isinstance(positions, torch.Tensor):
-        _ints(positions, "positions", device)
-        assert positions.numel() == rows, "positions has one value a row"
-        pos_ptr = positions.data_ptr()
-    else:
-        start = int(positions)
-    turns, steps, rot, inter, factor = _rotation(rotary, hd, device)
-    qn, qe = _head_norm(q_norm, "q_norm", hd, device)
-    kn, ke = _head_norm(k_norm, "k_norm", hd, device)
-    if rows == 0:
-        return
-    _enqueue("smeg_rotate_heads_dev", device, ROTATE_ARGS.pack(
-        q_ptr, k_ptr, 0, qo_ptr, ko_ptr, qs, ks, 0, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, dtype is _BF16, 0, rot, rows, heads, kv_heads, hd,
-        pos_ptr, start, 0, 0, 0, 0, 0, 0, 0, 0, 0))
+    args = (q, k, positions, q_out, k_out, *_head_norm(q_norm, "q_norm"), *_head_norm(k_norm, "k_norm"), _rotation(rotary, hd), hd)
+    rc = (_CALLS or _calls()).rotate(*args)
+    if rc == _NO_ROTATION_YET:
+        rotary._on((k if q is None else q).get_device())
+        rc = _CALLS.rotate(*args)
+    if rc:
+        check("smeg_rotate_heads_dev", rc)
 
 
 class PagedBatch:
@@ -245,7 +165,7 @@ class PagedBatch:
         assert table.dim() == 2 and table.shape[0] == n, "table has a row of pages for each sequence"
         self._tensors = cu_rows, starts, table
         self._device = starts.get_device()
-        self._fields = cu_rows.data_ptr(), starts.data_ptr(), table.data_ptr(), n, table.shape[1]
+        self._fields = cu_rows.data_ptr(), starts.data_ptr(), table.data_ptr(), n, table.shape[1], self._device
 
     @property
     def cu_rows(self):
@@ -280,9 +200,12 @@ class PagedKvCache:
         self._codes = torch.full((pages, kv_heads, 2, page, head_dim), 128, dtype=torch.uint8, device=device)
         self._scales = torch.zeros((pages, kv_heads, 2), dtype=torch.float32, device=device)
         self._device = self._codes.get_device()
-        self._at = self._codes.data_ptr(), self._scales.data_ptr()
-        self._scale = float(np.float32(1.0) / np.sqrt(np.float32(head_dim)))
-        self._ws_bytes = {}
+        self._set_scale(1.0 / np.sqrt(np.float32(head_dim)))
+
+    def _set_scale(self, scale: float) -> None:
+        self._scale = float(np.float32(scale))
+        self._fields = (self._codes.data_ptr(), self._scales.data_ptr(), self._pages, self._page, self._heads, self._kv_heads, self._head_dim, self._device,
+                        self._scale)
 
     @property
     def codes(self):
@@ -293,7 +216,7 @@ class PagedKvCache:
         return self._scales
 
     def with_scale(self, scale: float) -> "PagedKvCache":
-        self._scale = float(np.float32(scale))
+        self._set_scale(scale)
         return self
 
     def heads(self) -> int:
@@ -320,70 +243,33 @@ class PagedKvCache:
     def query_len(self) -> int:
         return self._heads * self._head_dim
 
-    def _like(self, x, what: str, batch):
-        like, rows, _ = _first_rows(x, what)
-        assert like[1] == self._device, "the rows are on the cache's device"
-        assert isinstance(batch, PagedBatch) and batch._device == self._device, "the batch is on the cache's device"
-        return like, rows
-
     def append(self, k, v, batch: PagedBatch, rotary: Rotary | None = None, *, k_norm=None, k_out=None, q=None, q_out=None, q_norm=None) -> None:
         """The rows k and v (kv_heads * head_dim values) to the pages of their sequences' positions; keys are normalised (k_norm) and rotated on the way.
         k_out: the keys so treated as 16-bit rows as well.  q, q_out: the queries, normalised (q_norm) and rotated, in the same pass.  The outputs
         may be the inputs.  Rows of idle sequences and rows behind the last sequence are left as they are."""
-        hd = self._head_dim
-        row, device = self._kv_heads * hd, self._device
-        like, rows = self._like(k, "k", batch)
-        ks, vs = _rows(k, "k", rows, row, like), _rows(v, "v", rows, row, like)
-        q_ptr = qo_ptr = ko_ptr = qs = qos = kos = 0
-        if k_out is not None:
-            kos, ko_ptr = _rows(k_out, "k_out", rows, row, like), k_out.data_ptr()
-        assert (q is None) == (q_out is None), "q and q_out come together"
-        if q is not None:
-            q_len = self._heads * hd
-            qs, qos = _rows(q, "q", rows, q_len, like), _rows(q_out, "q_out", rows, q_len, like)
-            q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
-        turns, steps, rot, inter, factor = _rotation(rotary, hd, device)
-        qn, qe = _head_norm(q_norm, "q_norm", hd, device)
-        kn, ke = _head_norm(k_norm, "k_norm", hd, device)
-        if rows == 0 or batch._fields[3] == 0:
-            return
-        _enqueue("smeg_paged_append_dev", device, ROTATE_ARGS.pack(
-            q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, qs, ks, vs, qos, kos, qn, kn, turns, steps, qe, ke, factor, inter, like[0] is _BF16, 0, rot,
-            rows, self._heads, self._kv_heads, hd, 0, 0, *batch._fields, *self._at, self._pages, self._page))
+        assert isinstance(batch, PagedBatch), "batch is a PagedBatch"
+        args = (k, v, k_out, q, q_out, *_head_norm(q_norm, "q_norm"), *_head_norm(k_norm, "k_norm"), _rotation(rotary, self._head_dim), batch._fields, self._fields)
+        rc = (_CALLS or _calls()).append(*args)
+        if rc == _NO_ROTATION_YET:
+            rotary._on(self._device)
+            rc = _CALLS.append(*args)
+        if rc:
+            check("smeg_paged_append_dev", rc)
 
     def attend(self, q, batch: PagedBatch, out) -> None:
         """out = the attention of the query rows (heads * head_dim values) against their sequences' cached positions, which already hold the rows' own
         (append, then attend, with the same batch): row i of a sequence attends to positions 0..=start + i.  Rows of idle sequences become
         zeros, rows behind the last sequence stay as they are."""
-        like, rows = self._like(q, "q", batch)
-        width, device = self._heads * self._head_dim, self._device
-        qs, os_ = _rows(q, "q", rows, width, like), _rows(out, "out", rows, width, like)
-        cu, starts, table, seqs, cols = batch._fields
-        if rows == 0 or seqs == 0:
-            return
-        size = rows, seqs, cols
-        need = self._ws_bytes.get(size)
-        if need is None:
-            with _On(device):
-                need = lib().smeg_paged_attend_workspace(rows, seqs, cols, self._page, self._heads, self._kv_heads, self._head_dim)
-            self._ws_bytes[size] = need
-        # the call's own memory, from the stream's pool: two streams, or two captured graphs, never share it
-        ws = self._codes.new_empty(need) if need else None
-        _enqueue("smeg_paged_attend_dev", device, PAGED_ATTEND_ARGS.pack(
-            q.data_ptr(), out.data_ptr(), qs, os_, *self._at, cu, starts, table, seqs, cols, self._pages, self._page, rows, self._heads, self._kv_heads,
-            self._head_dim, self._scale, like[0] is _BF16, ws.data_ptr() if need else 0, need))
+        assert isinstance(batch, PagedBatch), "batch is a PagedBatch"
+        rc = (_CALLS or _calls()).attend(q, out, batch._fields, self._fields)
+        if rc:
+            check("smeg_paged_attend_dev", rc)
 
     def read(self, ids, out) -> None:
         """The values of whole pages: out [n, kv_heads, 2, page, head_dim] (keys, values), contiguous f16 or bf16, for the n int32 page ids."""
-        _ints(ids, "ids", self._device)
-        n = ids.numel()
-        assert isinstance(out, torch.Tensor) and out.get_device() == self._device and out.dtype in (_F16, _BF16) and out.is_contiguous(), "out is contiguous f16 or bf16"
-        assert out.numel() == n * self._kv_heads * 2 * self._page * self._head_dim, "out holds n pages"
-        if n == 0:
-            return
-        device = self._device
-        _enqueue("smeg_paged_read_dev", device, READ_ARGS.pack(out.data_ptr(), *self._at, ids.data_ptr(), n, self._pages, self._page, self._kv_heads, self._head_dim,
-                                                               out.dtype is _BF16, 0))
+        rc = (_CALLS or _calls()).read(ids, out, self._fields)
+        if rc:
+            check("smeg_paged_read_dev", rc)
 
 
 def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float | None = None) -> None:
@@ -391,18 +277,6 @@ def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float
     its rows 0..=i.  q, out: rows of heads * head_dim values, k, v of kv_heads * head_dim, f16 or bf16, at any row stride; scale 1 / sqrt(head_dim).
     Rows behind the last sequence are left as they are."""
     assert kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "heads must be a positive multiple of kv_heads"
-    like, rows, width = _first_rows(q, "q")
-    dtype, device = like
-    hd = width // heads
-    assert hd * heads == width, "q has rows of heads * head_dim values"
-    assert hd % 8 == 0 and 8 <= hd <= 256, "head_dim must be a multiple of 8 in 8..=256"
-    row = kv_heads * hd
-    qs, ks, vs, os_ = _rows(q, "q", rows, width, like), _rows(k, "k", rows, row, like), _rows(v, "v", rows, row, like), _rows(out, "out", rows, width, like)
-    _ints(cu_rows, "cu_rows", device)
-    seqs = cu_rows.numel() - 1
-    assert seqs >= 0, "cu_rows has one value more than there are sequences"
-    if rows == 0 or seqs == 0:
-        return
-    _enqueue("smeg_attn_packed_dev", device, ATTN_PACKED_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs, ks, vs, os_, cu_rows.data_ptr(), seqs, rows, heads, kv_heads, hd,
-        hd ** -0.5 if scale is None else scale, dtype is _BF16))
+    rc = (_CALLS or _calls()).packed(q, k, v, cu_rows, out, heads, kv_heads, scale)
+    if rc:
+        check("smeg_attn_packed_dev", rc)
