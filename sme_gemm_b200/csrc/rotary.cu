@@ -23,6 +23,7 @@ namespace {
 constexpr int kRotThreads = 128;
 constexpr int kRowTile = 4;                        // rows of a CTA of query heads, at most
 constexpr int kHeld = 8;                           // runs of eight depths that a thread of a page's CTA keeps
+constexpr int kPageHeads = 32;                     // heads of a page's CTA, at most
 constexpr int kAhead = 4;                          // and that a thread of a row's CTA has on their way
 constexpr float kLeastScale = 7.703719777548943e-34f;   // 2^-110: a smaller scale has no reciprocal to speak of and counts as zero
 constexpr float kRound = 12582912.0f;              // 1.5 * 2^23: what is added to it is rounded to an integer, in the low bits of the sum
@@ -243,8 +244,8 @@ __device__ __forceinline__ int count_upto(int n, long long x, Key key) {
 // magnitude to the codes, and norms and turns them a second time; a longer page is read twice.
 template <int BF16, int LAY>
 __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L, float* cs, int unit) {
-    __shared__ unsigned s_max[32];
-    __shared__ float s_inv[32], s_ratio[32];
+    __shared__ unsigned s_max[kPageHeads];
+    __shared__ float s_inv[kPageHeads], s_ratio[kPageHeads];
     const PackedSeqs& B = p.seqs;
     const int tid = threadIdx.x, page = 1 << B.page_log2;
     const int which = unit & 1, slot = (unit >> 1) / p.page_groups, hg = (unit >> 1) - slot * p.page_groups;
@@ -285,7 +286,7 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
     const int block = page * L.hd;                                 // bytes of one head's keys or values in a page
     uint8_t* dst = p.codes + (((size_t)id * p.kv_heads + h0) * 2 + which) * block + at * L.hd;
     float* scale = p.scales + ((size_t)id * p.kv_heads + h0) * 2 + which;
-    if (tid < 32) s_max[tid] = 0;
+    if (tid < kPageHeads) s_max[tid] = 0;
     const Octet w = norm_weights<LAY>(norm ? p.k_w : nullptr, L, c, mine_ok);
     // The first row's angles are formed here; row r is r steps of the frequencies further, by the sum formulas (steps: [256][cosines, sines], 32 bits)
     if (rotate) fill_trig(p, L, cs, 1, [&](int) { return (long long)start + r0; });
@@ -534,6 +535,7 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
         const long long slots = ((long long)a.rows >> a.seqs.page_log2) + 2ll * a.seqs.seqs;
         a.page_heads = kHeld * per_pass / (mean < page ? mean : page);
         if (a.page_heads > per_pass) a.page_heads = per_pass;
+        if (a.page_heads > kPageHeads) a.page_heads = kPageHeads;
         if (a.page_heads > a.kv_heads) a.page_heads = a.kv_heads;
         if (a.page_heads < 1) a.page_heads = 1;
         while (a.page_heads > 1 && slots * ((a.kv_heads + a.page_heads - 1) / a.page_heads) * 2 < sm_count) a.page_heads = (a.page_heads + 1) / 2;

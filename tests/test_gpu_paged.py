@@ -738,3 +738,16 @@ def test_refusals_with_tensors_on_the_device():
     cache.read(_int([]), r(0, 1))
     sg.attend_packed(r(0, 128), r(0, 64), r(0, 64), _int([0]), r(0, 128), 4, 2)
     sg.rotate_heads(r(0, 128), None, 0, sg.Rotary(32), r(0, 128), None)
+
+
+# ------------------------------------------------------------------------------------------------ calls at the edges
+
+def test_more_narrow_heads_than_a_warp_has_lanes():
+    """Heads of 16 depths are two lanes each: 64 of them in a block at a time, and 40 are more than a page's CTA takes."""
+    seqs = 80
+    pool = Pool(80, 40, 16, 16, seqs, 3, seed=40)
+    rotary, kn = sg.Rotary(16), _norm(pool.gen, 16)
+    pool.append([3] * seqs, (), rotary, kn)
+    pool.append([1] * seqs, (7,), rotary, kn)
+    pool.append([20] * seqs, (), rotary, kn)
+    pool.check(times=3)
