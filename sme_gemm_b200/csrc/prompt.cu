@@ -29,19 +29,34 @@ __device__ __forceinline__ float ex2(float x) {
 // infinity or NaN there makes NaNs (0 * inf).  So a row whose result is not finite although its probabilities are is formed again, key by key over
 // what it attends to, where the blocks that it shares with later rows hold such a value.
 
-// Whether any value of keys [from, to) of a KV head is an infinity or NaN.  A warp.
-__device__ __noinline__ bool any_bad_value(const PromptArgs& p, int kvh, int from, int to) {
+// Whether rows that attend to keys [first, low] and not to all of (low, to) may have to be: a value of (low, to) is an infinity or NaN at a depth that is not
+// lost to them anyway.  (A depth at which they attend to a NaN, or to infinities of both signs, is; the 64 keys up to low tell where values are lost altogether, and
+// rows of thousands of keys need not be formed again one by one.)  A warp; a lane has eight depths.
+__device__ __noinline__ bool spoilt_by_later(const PromptArgs& p, int kvh, int first, int low, int to) {
     const unsigned expo = p.bf16 ? 0x7f80u : 0x7c00u;
-    bool bad = false;
-    for (int j = from; j < to; ++j) {
-        const uint16_t* v = p.v + (size_t)j * p.v_stride + (size_t)kvh * p.head_dim;
-        for (int d = threadIdx.x & 31; d < p.head_dim; d += 32) bad = bad || (v[d] & expo) == expo;
+    const int d0 = (threadIdx.x & 31) * 8;
+    unsigned later = 0, nan = 0, up = 0, down = 0;                 // a bit a depth
+    if (d0 < p.head_dim) {
+        const uint16_t* v = p.v + (size_t)kvh * p.head_dim + d0;
+        for (int j = low + 1; j < to; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) later |= (unsigned)((v[(size_t)j * p.v_stride + e] & expo) == expo) << e;
+        if (later)
+            for (int j = low; j >= max(first, low - 63); --j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const unsigned x = v[(size_t)j * p.v_stride + e];
+                    nan |= (unsigned)((x & 0x7fffu) > expo) << e;
+                    up |= (unsigned)(x == expo) << e;
+                    down |= (unsigned)(x == (expo | 0x8000u)) << e;
+                }
     }
-    return __any_sync(0xffffffffu, bad);
+    return __any_sync(0xffffffffu, (later & ~(nan | (up & down))) != 0);
 }
-// Row `row` (of the packed batch) of query head `head` over keys [first, row].  A warp; a lane has eight depths.
+// Row `row` (of the packed batch) of query head `head` over keys [first, row].  A warp; a lane has eight depths, and four keys are on their way at a time.
 template <int BF16>
 __device__ __noinline__ void exact_row(const PromptArgs& p, int first, int row, int head) {
+    constexpr int kAhead = 4;
     const int lane = threadIdx.x & 31, d = lane * 8, hd = p.head_dim, kvh = head / (p.heads / p.kv_heads);
     const bool in = d < hd;
     float q[8], acc[8], m = -kInf, l = 0.0f;
@@ -50,21 +65,41 @@ __device__ __noinline__ void exact_row(const PromptArgs& p, int first, int row, 
         q[e] = in ? t_to_f32<BF16>(p.q[(size_t)row * p.q_stride + (size_t)head * hd + d + e]) : 0.0f;
         acc[e] = 0.0f;
     }
-    for (int j = first; j <= row; ++j) {
-        const uint16_t *k = p.k + (size_t)j * p.k_stride + (size_t)kvh * hd + d, *v = p.v + (size_t)j * p.v_stride + (size_t)kvh * hd + d;
-        float s = 0.0f;
-        if (in)
+    for (int j0 = first; j0 <= row; j0 += kAhead) {
+        float s[kAhead];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = fmaf(q[e], t_to_f32<BF16>(k[e]), s);
+        for (int i = 0; i < kAhead; ++i) {
+            const uint16_t* k = p.k + (size_t)min(j0 + i, row) * p.k_stride + (size_t)kvh * hd + d;
+            s[i] = 0.0f;
+            if (in)
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= p.scale_log2e;
-        const float now = fmaxf(m, s), ref = now == -kInf ? 0.0f : now, a = ex2(m - ref), w = ex2(s - ref);
+                for (int e = 0; e < 8; ++e) s[i] = fmaf(q[e], t_to_f32<BF16>(k[e]), s[i]);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+        float now = m;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            s[i] *= p.scale_log2e;
+            now = fmaxf(now, s[i]);                                // (the last key again, where there are no four)
+        }
+        const float ref = now == -kInf ? 0.0f : now, a = ex2(m - ref);
         m = now;
-        l = fmaf(l, a, w);
-        if (in)
+        l *= a;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, t_to_f32<BF16>(v[e]), acc[e] * a);
+        for (int e = 0; e < 8; ++e) acc[e] *= a;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (j0 + i > row) break;
+            const float w = ex2(s[i] - ref);
+            l += w;
+            const uint16_t* v = p.v + (size_t)(j0 + i) * p.v_stride + (size_t)kvh * hd + d;
+            if (in)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, t_to_f32<BF16>(v[e]), acc[e]);
+        }
     }
     if (in)
 #pragma unroll
@@ -241,7 +276,7 @@ __global__ void __launch_bounds__(kPwThreads) prompt_mma_kernel(const __grid_con
     for (int e = 0; e < 2; ++e) {
         unsigned mask = __ballot_sync(0xffffffffu, bad[e]);
         mask = (mask | mask >> 1 | mask >> 2 | mask >> 3) & 0x11111111u;      // one bit a row
-        if (!mask || !any_bad_value(p, kvh, first + i_first + 1, first + keys)) continue;
+        if (!mask || !spoilt_by_later(p, kvh, first, first + i_first, first + keys)) continue;
         for (; mask; mask &= mask - 1) {
             const long long n = n0 + 16 * warp + (__ffs(mask) - 1) / 4 + 8 * e;
             const int i = (int)(n / group);
@@ -703,7 +738,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             unpack64(zero, z0, z1);
             const bool bad = !(z0 + z1 == 0.0f);
             unsigned mask = __ballot_sync(0xffffffffu, in && bad && l > 0.0f);
-            if (mask && any_bad_value(p, w.kvh, w.first + low + 1, min(w.first + n * kPtKeys, p.rows)))
+            if (mask && spoilt_by_later(p, w.kvh, w.first, w.first + low, min(w.first + n * kPtKeys, p.rows)))
                 for (; mask; mask &= mask - 1) {
                     const int r = __ffs(mask) - 1, tk = __shfl_sync(0xffffffffu, tok, r), h = __shfl_sync(0xffffffffu, head, r);
                     __syncwarp();

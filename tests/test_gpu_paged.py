@@ -751,3 +751,24 @@ def test_more_narrow_heads_than_a_warp_has_lanes():
     pool.append([1] * seqs, (7,), rotary, kn)
     pool.append([20] * seqs, (), rotary, kn)
     pool.check(times=3)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_values_that_are_lost_altogether(hd):
+    """From position 100 on no value is finite: NaNs, infinities of one sign, of both in turn.  A row has what the sum over what it attends to has."""
+    gen = _gen(hd + 1)
+    heads, kv, n = 4, 2, 700
+    q, k, v0 = _randn(gen, n, heads * hd), _randn(gen, n, kv * hd), _randn(gen, n, kv * hd)
+    want, tol = _prompt(q[:100], k[:100], v0[:100], [100], heads, kv)
+    for kind in ("nan", "inf", "both"):
+        v = v0.clone()
+        v[100:] = math.nan if kind == "nan" else math.inf
+        if kind == "both":
+            v[101::2] = -math.inf
+        out = torch.empty_like(q)
+        sg.attend_packed(q, k, v, _int([0, n]), out, heads, kv)
+        _near(out[:100], want, tol, F16)
+        if kind == "inf":
+            assert torch.all(out[100:] == math.inf)
+        else:
+            assert torch.isnan(out[101:]).all() and torch.all(out[100] == math.inf if kind == "both" else torch.isnan(out[100]))
