@@ -369,9 +369,10 @@ __global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) p
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             // largest magnitude to 2^14 .. 2^15: exact but for depths 2^-28 below it (f16's own range needs no more than that)
             const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-            const int up = mx > 0.0f && ex < 100 && ex > -110 ? 14 - ex : 0;
+            const int up = mx > 0.0f && ex < 128 && ex > -110 ? 14 - ex : 0;
             const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-            const float back = __uint_as_float((uint32_t)(127 - up) << 23) * (p.scale_log2e * 16777216.0f);
+            // (from 2^100 on the scores come out 2^(ex - 99) too small, which leaves a softmax of such scores as it is: their products with 2^24 stay numbers)
+            const float back = __uint_as_float((uint32_t)(127 - max(up, 14 - 99)) << 23) * (p.scale_log2e * 16777216.0f);
 #pragma unroll
             for (int c = 0; c < HC; ++c)
 #pragma unroll

@@ -772,3 +772,25 @@ def test_values_that_are_lost_altogether(hd):
             assert torch.all(out[100:] == math.inf)
         else:
             assert torch.isnan(out[101:]).all() and torch.all(out[100] == math.inf if kind == "both" else torch.isnan(out[100]))
+
+
+@pytest.mark.parametrize("size", [1e25, 1e31, 1e37])
+def test_queries_near_the_largest_numbers(size):
+    """bf16 queries so large that a row's best key has all the weight: the result is that key's value, to a rounding and the offset's error."""
+    pool = Pool(8, 2, 64, 16, 1, 4, seed=5, dtype=BF16)
+    pool.append([50])
+    q = _randn(pool.gen, 4, 512, dtype=BF16) * size
+    assert torch.isfinite(q).all()
+    out = torch.empty_like(q)
+    pool.cache.attend(q, pool.batch([4], starts=[46]), out)
+    assert torch.isfinite(out).all()
+    x, sc = pool.values(0)
+    k, v = x.repeat_interleave(4, 2)
+    z = torch.einsum("rhd,nhd->rhn", q.double().reshape(4, 8, 64), k)
+    z = z.masked_fill(torch.arange(50, device="cuda")[None, None, :] > 46 + torch.arange(4, device="cuda")[:, None, None], -math.inf)
+    top = z.topk(2, -1)
+    clear = (top.values[..., 0] - top.values[..., 1]) > 2.0 ** -10 * z.masked_fill(z == -math.inf, 0).abs().amax(-1)
+    assert clear.sum() > 16
+    best = v[top.indices[..., 0], torch.arange(8, device="cuda")[None, :]]
+    room = best.abs() * (2.0 ** -8 + 2.0 ** -10) + 2.0 ** -18 * 255 * sc.amax()
+    assert torch.all(((out.double().reshape(4, 8, 64) - best).abs() <= room)[clear])
