@@ -348,6 +348,7 @@ PyObject* packed(PyObject*, PyObject* const* v, Py_ssize_t n) {
         a.k = rows_of(v[1], "k", row, like, &a.k_stride);
         a.v = rows_of(v[2], "v", row, like, &a.v_stride);
         a.out = rows_of(v[4], "out", width, like, &a.out_stride);
+        require(like.rows == 0 || (a.out != a.q && a.out != a.k && a.out != a.v), "out", " is none of the inputs");
         int64_t count;
         a.cu_rows = ints(v[3], "cu_rows", like.device, &count);
         require(count >= 1, "", "cu_rows has one value more than there are sequences");

@@ -51,6 +51,7 @@ def _head_norm(norm, what: str):
 class Rotary:
     """The rotation of heads by position: pair i of the first `rotary_dim` depths turns by position * frequency_i, frequency_i =
     base^(-2 i / rotary_dim).  A pair is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) interleaved; the depths behind rotary_dim stay as they are.
+    The first call with it on a device places its tables there, and so cannot be one that a graph captures.
     linear(), by_wavelength() and yarn() give the same rotation with its frequencies scaled for contexts longer than the trained one."""
 
     def __init__(self, head_dim: int, base: float = 10000.0, rotary_dim: int | None = None, interleaved: bool = False):
@@ -115,15 +116,17 @@ class Rotary:
         return self._factor
 
     def _on(self, device: int):
-        """(address of the turns per position of each pair, f64; address of the cosines and sines of 0 .. 255 times the frequencies, f32; the tensors).  Made by
-        the first call on a device: before a capture, then."""
+        """(address of the turns per position of each pair, f64; address of the cosines and sines of 0 .. 255 times the frequencies, f32; the tensors)."""
         t = self._turns.get(device)
         if t is None:
+            with torch.cuda.device(device):
+                capturing = torch.cuda.is_current_stream_capturing()
+            assert not capturing, "the first call with a rotation on a device lies before a capture"
             at = torch.device("cuda", device)
             turns = torch.tensor(self._frequencies / (2.0 * math.pi), dtype=torch.float64, device=at)
             angle = np.arange(256, dtype=np.float64)[:, None] * self._frequencies
             steps = torch.tensor(np.concatenate([np.cos(angle), np.sin(angle)], 1), dtype=torch.float32, device=at)
-            t = self._turns[device] = turns.data_ptr(), steps.data_ptr(), turns, steps
+            t = self._turns.setdefault(device, (turns.data_ptr(), steps.data_ptr(), turns, steps))     # (another thread's, if that was first)
         return t
 
 
@@ -163,6 +166,7 @@ class PagedBatch:
         n = starts.numel()
         assert cu_rows.numel() == n + 1, "cu_rows has one value more than there are sequences"
         assert table.dim() == 2 and table.shape[0] == n, "table has a row of pages for each sequence"
+        assert n == 0 or table.shape[1] > 0, "table has a page for each sequence"
         self._tensors = cu_rows, starts, table
         self._device = starts.get_device()
         self._fields = cu_rows.data_ptr(), starts.data_ptr(), table.data_ptr(), n, table.shape[1], self._device
@@ -259,7 +263,7 @@ class PagedKvCache:
     def attend(self, q, batch: PagedBatch, out) -> None:
         """out = the attention of the query rows (heads * head_dim values) against their sequences' cached positions, which already hold the rows' own
         (append, then attend, with the same batch): row i of a sequence attends to positions 0..=start + i.  Rows of idle sequences become
-        zeros, rows behind the last sequence stay as they are."""
+        zeros, rows behind the last sequence stay as they are.  out shares no memory with q."""
         assert isinstance(batch, PagedBatch), "batch is a PagedBatch"
         rc = (_CALLS or _calls()).attend(q, out, batch._fields, self._fields)
         if rc:
@@ -275,7 +279,7 @@ class PagedKvCache:
 def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float | None = None) -> None:
     """out = causal attention over whole packed prompts: rows cu_rows[s] .. cu_rows[s + 1] (int32 CUDA tensor) are a sequence's, row i of it attends to
     its rows 0..=i.  q, out: rows of heads * head_dim values, k, v of kv_heads * head_dim, f16 or bf16, at any row stride; scale 1 / sqrt(head_dim).
-    Rows behind the last sequence are left as they are."""
+    Rows behind the last sequence are left as they are.  out shares no memory with the inputs."""
     assert kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "heads must be a positive multiple of kv_heads"
     rc = (_CALLS or _calls()).packed(q, k, v, cu_rows, out, heads, kv_heads, scale)
     if rc:

@@ -794,3 +794,29 @@ def test_queries_near_the_largest_numbers(size):
     best = v[top.indices[..., 0], torch.arange(8, device="cuda")[None, :]]
     room = best.abs() * (2.0 ** -8 + 2.0 ** -10) + 2.0 ** -18 * 255 * sc.amax()
     assert torch.all(((out.double().reshape(4, 8, 64) - best).abs() <= room)[clear])
+
+
+def test_the_first_call_with_a_rotation_is_not_captured():
+    rotary, q, out = sg.Rotary(32), torch.ones(2, 64, dtype=F16, device="cuda"), torch.zeros(2, 64, dtype=F16, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(AssertionError, match="before a capture"):
+            sg.rotate_heads(q, None, 0, rotary, out, None)
+        out.add_(1.0)
+    g.replay()
+    assert torch.all(out == 1.0)
+    sg.rotate_heads(q, None, 0, rotary, out, None)
+    again, h = torch.zeros_like(out), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(h):
+        sg.rotate_heads(q, None, 0, rotary, again, None)
+    h.replay()
+    assert torch.equal(again, out)
+
+
+def test_refusals_of_overlaps_and_of_tables_without_pages():
+    q, k = torch.zeros(4, 128, dtype=F16, device="cuda"), torch.zeros(4, 64, dtype=F16, device="cuda")
+    with pytest.raises(AssertionError, match="none of the inputs"):
+        sg.attend_packed(q, k, k, _int([0, 4]), q, 4, 2)
+    with pytest.raises(AssertionError, match="a page for each"):
+        sg.PagedBatch(_int([0, 4]), _int([0]), torch.zeros(1, 0, dtype=torch.int32, device="cuda"))
+    assert sg.PagedBatch(_int([0]), torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, 3, dtype=torch.int32, device="cuda")).seqs() == 0
