@@ -501,97 +501,87 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             cta = taken_cta(smem_u32(&answer));
             __syncwarp();
         }
-    } else if (warp == 9) {                                        // ---- products ----
-        const uint32_t idesc_s = umma_idesc(BF16, 128, kPtKeys), idesc_o = umma_idesc(BF16, 128, hd16) | (1u << 16);
-        const int ksteps = hd16 >> 4;
-        const uint32_t q_a = smem_u32(q_s), ring_a = smem_u32(ring);
-        int slot = 0, par = 0, done[2] = {0, 0};                   // blocks of the two tiles so far
-        bool ok = true;
-        auto take = [&](uint32_t& addr, int& at) {
-            at = slot;
-            addr = ring_a + (uint32_t)slot * kTile;
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[slot], par, abort_flag, p.status));
-            if (++slot == a.slots) { slot = 0; par ^= 1; }
-            tc_fence_after();
-        };
-        auto scores = [&](int x, int buf, uint32_t k_addr) {           // of query tile x, into the columns of buffer buf
-            if (elect_one()) {
-                for (int s = 0; s < ksteps; ++s) {
-                    const uint32_t off = (uint32_t)((s >> 2) * kPtChunk + (s & 3) * 32);
-                    umma_f16(tmem + 128 * buf, umma_desc_sw128(q_a + x * kTile + off), umma_desc_sw128(k_addr + off), idesc_s, s > 0);
-                }
+    } else if (warp == 9) {                                        // ---- products: one lane, so that nothing but the waits stands between them ----
+        if (elect_one()) {
+            const uint32_t idesc_s = umma_idesc(BF16, 128, kPtKeys), idesc_o = umma_idesc(BF16, 128, hd16) | (1u << 16);
+            const int ksteps = hd16 >> 4;
+            const uint64_t q_d = umma_desc_sw128(smem_u32(q_s)), k_d = umma_desc_sw128(smem_u32(ring)), v_d = desc_mn(smem_u32(ring));   // (an address is its low 14 bits, in 16 bytes)
+            int slot = 0, par = 0, done[2] = {0, 0};               // blocks of the two tiles so far
+            bool ok = true;
+            auto take = [&]() {                                    // the next slot of the ring, filled
+                const int at = slot;
+                ok = ok && mbar_wait(&full[at], par, abort_flag, p.status);
+                if (++slot == a.slots) { slot = 0; par ^= 1; }
+                return at;
+            };
+            auto scores = [&](int x, int buf, int at) {            // of query tile x, into the columns of buffer buf
+                const uint64_t q0 = q_d + x * (kTile >> 4), k0 = k_d + at * (kTile >> 4);
+                tc_fence_after();
+#pragma unroll
+                for (int s = 0; s < 4 * NCH; ++s)
+                    if (s < ksteps) umma_f16(tmem + 128 * buf, q0 + ((s >> 2) * kPtChunk + (s & 3) * 32) / 16, k0 + ((s >> 2) * kPtChunk + (s & 3) * 32) / 16, idesc_s, s > 0);
                 umma_commit(&s_full[buf]);
-            }
-            __syncwarp();
-        };
-        PromptItem w;
-        for (int it = 0; ok && next_item(it, w); ++it) {
-            const int nblk[2] = {blocks_of(w, 0), blocks_of(w, 1)}, nmax = max(nblk[0], nblk[1]);
-            ok = __all_sync(0xffffffffu, mbar_wait(q_full, it & 1, abort_flag, p.status));
-            uint32_t k_addr = 0, v_addr = 0;
-            int k_slot = 0, v_slot = 0;
-            if (ok) take(k_addr, k_slot);
-            if (ok) {
-                scores(0, kTiles == 2 ? 0 : done[0] & 1, k_addr);
-                if (nblk[1]) scores(1, 1, k_addr);
-                if (elect_one()) {
-                    umma_commit(&empty[k_slot]);
-                    if (nmax == 1) umma_commit(q_empty);
-                }
-                __syncwarp();
-            }
-            if (kTiles == 1)
-                for (int j = 0; ok && j < nmax; ++j) {
-                    const int buf = done[0] & 1;
-                    if (j + 1 < nmax) {
-                        take(k_addr, k_slot);
-                        if (!ok) break;
-                        scores(0, buf ^ 1, k_addr);                // (behind the product that read this buffer's probabilities)
-                        if (elect_one()) {
-                            umma_commit(&empty[k_slot]);
+            };
+            auto values = [&](int x, int buf, int at, bool first) {    // probabilities of buffer buf times the values
+                const uint64_t v0 = v_d + at * (kTile >> 4);
+                tc_fence_after();
+#pragma unroll
+                for (int s = 0; s < kPtKeys / 16; ++s) umma_f16_ts(tmem + kPtO + 128 * x, tmem + 128 * buf + 8 * s, v0 + s * 128, idesc_o, !first || s > 0);
+            };
+            for (int it = 0; ok; ++it) {
+                ok = mbar_wait(&item_full[it & 1], (it >> 1) & 1, abort_flag, p.status);
+                if (!ok) break;
+                const PromptItem w = items[it & 1];
+                mbar_arrive(&item_empty[it & 1]);
+                if (w.rows < 0) break;
+                const int nblk[2] = {blocks_of(w, 0), blocks_of(w, 1)}, nmax = max(nblk[0], nblk[1]);
+                ok = mbar_wait(q_full, it & 1, abort_flag, p.status);
+                int k_at = take(), v_at;
+                if (!ok) break;
+                scores(0, kTiles == 2 ? 0 : done[0] & 1, k_at);
+                if (nblk[1]) scores(1, 1, k_at);
+                umma_commit(&empty[k_at]);
+                if (nmax == 1) umma_commit(q_empty);
+                if (kTiles == 1)
+                    for (int j = 0; j < nmax; ++j) {
+                        const int buf = done[0] & 1;
+                        if (j + 1 < nmax) {
+                            k_at = take();
+                            if (!ok) break;
+                            scores(0, buf ^ 1, k_at);              // (behind the product that read this buffer's probabilities)
+                            umma_commit(&empty[k_at]);
                             if (j + 2 == nmax) umma_commit(q_empty);
                         }
-                        __syncwarp();
-                    }
-                    take(v_addr, v_slot);
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait_poll(&p_full[buf], (done[0] >> 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
-                    if (!ok) break;
-                    ++done[0];
-                    tc_fence_after();
-                    if (elect_one()) {
-                        for (int s = 0; s < kPtKeys / 16; ++s)
-                            umma_f16_ts(tmem + kPtO, tmem + 128 * buf + 8 * s, desc_mn(v_addr + s * 2048), idesc_o, j > 0 || s > 0);
-                        umma_commit(&empty[v_slot]);
+                        v_at = take();
+                        ok = ok && mbar_wait_poll(&p_full[buf], (done[0] >> 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT);
+                        if (!ok) break;
+                        ++done[0];
+                        values(0, buf, v_at, j == 0);
+                        umma_commit(&empty[v_at]);
                         umma_commit(&o_done[0]);
                     }
-                    __syncwarp();
-                }
-            for (int j = 0; kTiles == 2 && ok && j < nmax; ++j) {
-                take(v_addr, v_slot);
-                const bool more = j + 1 < nmax;
-                if (ok && more) take(k_addr, k_slot);
-                for (int x = 0; ok && x < 2; ++x) {
-                    if (j >= nblk[x]) continue;
-                    ok = __all_sync(0xffffffffu, mbar_wait_poll(&p_full[x], done[x] & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
-                    if (!ok) break;
-                    ++done[x];
-                    tc_fence_after();
-                    if (elect_one()) {
-                        for (int s = 0; s < kPtKeys / 16; ++s)
-                            umma_f16_ts(tmem + kPtO + 128 * x, tmem + 128 * x + 8 * s, desc_mn(v_addr + s * 2048), idesc_o, j > 0 || s > 0);
+                for (int j = 0; kTiles == 2 && ok && j < nmax; ++j) {
+                    const bool more = j + 1 < nmax;
+                    v_at = take();
+                    if (more) k_at = take();
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (!ok || j >= nblk[x]) continue;
+                        ok = mbar_wait_poll(&p_full[x], done[x] & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT);
+                        if (!ok) break;
+                        ++done[x];
+                        values(x, x, v_at, j == 0);
                         if (j + 1 == nblk[x]) umma_commit(&o_done[x]);
+                        else scores(x, x, k_at);
                     }
-                    __syncwarp();
-                    if (j + 1 < nblk[x]) scores(x, x, k_addr);
-                }
-                if (ok && elect_one()) {
-                    umma_commit(&empty[v_slot]);
-                    if (more) umma_commit(&empty[k_slot]);
+                    if (!ok) break;
+                    umma_commit(&empty[v_at]);
+                    if (more) umma_commit(&empty[k_at]);
                     if (j + 2 == nmax) umma_commit(q_empty);       // (the last scores have been formed)
                 }
-                __syncwarp();
             }
         }
+        __syncwarp();
     } else {                                                       // ---- softmax ----
         const int x = warp >> 2, row = (warp & 3) * 32 + lane;
         const int t = row / group, g = row - t * group;
