@@ -378,13 +378,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     __shared__ __align__(16) uint4 answer;
-    __shared__ __align__(8) uint64_t bars[2 * kPtMaxSlots + 13];
+    __shared__ __align__(8) uint64_t bars[2 * kPtMaxSlots + 15];
     __shared__ PromptItem items[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
     uint64_t *full = bars, *empty = full + kPtMaxSlots, *q_full = empty + kPtMaxSlots, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2, *o_done = p_full + 2,
-             *item_full = o_done + 2, *item_empty = item_full + 2, *taken = item_empty + 2;
+             *item_full = o_done + 2, *item_empty = item_full + 2, *taken = item_empty + 2, *p_half = taken + 1;
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     const int hd = p.head_dim, hd16 = (hd + 15) & ~15, group = p.heads / p.kv_heads, tt = a.tokens;
     unsigned char *q_s = smem, *out_s = smem + kTiles * kTile, *ring = out_s + kTiles * 4 * kPtStage;
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         mbar_init(q_empty, 1);
         mbar_init(taken, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1);
+            mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1);
             mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 9);
         }
         fence_barrier_init();
@@ -522,11 +522,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                     if (s < ksteps) umma_f16(tmem + 128 * buf, q0 + ((s >> 2) * kPtChunk + (s & 3) * 32) / 16, k0 + ((s >> 2) * kPtChunk + (s & 3) * 32) / 16, idesc_s, s > 0);
                 umma_commit(&s_full[buf]);
             };
-            auto values = [&](int x, int buf, int at, bool first) {    // probabilities of buffer buf times the values
+            // Probabilities of buffer buf times the values, half of the keys at a time: the first half's product runs while the second half is weighed
+            auto values = [&](int x, int buf, int at, int half, bool first) {
                 const uint64_t v0 = v_d + at * (kTile >> 4);
                 tc_fence_after();
 #pragma unroll
-                for (int s = 0; s < kPtKeys / 16; ++s) umma_f16_ts(tmem + kPtO + 128 * x, tmem + 128 * buf + 8 * s, v0 + s * 128, idesc_o, !first || s > 0);
+                for (int i = 0; i < kPtKeys / 32; ++i) {
+                    const int s = half * (kPtKeys / 32) + i;
+                    umma_f16_ts(tmem + kPtO + 128 * x, tmem + 128 * buf + 8 * s, v0 + s * 128, idesc_o, !first || s > 0);
+                }
             };
             for (int it = 0; ok; ++it) {
                 ok = mbar_wait(&item_full[it & 1], (it >> 1) & 1, abort_flag, p.status);
@@ -553,10 +557,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                             if (j + 2 == nmax) umma_commit(q_empty);
                         }
                         v_at = take();
-                        ok = ok && mbar_wait_poll(&p_full[buf], (done[0] >> 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT);
+                        ok = ok && mbar_wait_poll(&p_half[buf], (done[0] >> 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT);
                         if (!ok) break;
+                        values(0, buf, v_at, 0, j == 0);
+                        ok = mbar_wait_poll(&p_full[buf], (done[0] >> 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT);
+                        if (!ok) break;
+                        values(0, buf, v_at, 1, false);
                         ++done[0];
-                        values(0, buf, v_at, j == 0);
                         umma_commit(&empty[v_at]);
                         umma_commit(&o_done[0]);
                     }
@@ -567,10 +574,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         if (!ok || j >= nblk[x]) continue;
+                        ok = mbar_wait_poll(&p_half[x], done[x] & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT);
+                        if (!ok) break;
+                        values(x, x, v_at, 0, j == 0);
                         ok = mbar_wait_poll(&p_full[x], done[x] & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT);
                         if (!ok) break;
+                        values(x, x, v_at, 1, false);
                         ++done[x];
-                        values(x, x, v_at, j == 0);
                         if (j + 1 == nblk[x]) umma_commit(&o_done[x]);
                         else scores(x, x, k_at);
                     }
@@ -665,14 +675,16 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                         e[i / 2] = pack2_t<BF16>(u, v);
                     }
                     tmem_st16(ts + 16 * c, e);
+                    if (c & 1) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(c == 1 ? &p_half[buf] : &p_full[buf]);
+                    }
                 }
-                tmem_st_wait();
                 float u, v;
                 unpack64(add2(sum[0], sum[1]), u, v);
                 l += u + v;
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[buf]);
             }
             if (!ok || n == 0) continue;
             ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], (kTiles == 2 ? tiles : done - 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
