@@ -276,7 +276,7 @@ struct RotateArgs {
     uint8_t* codes;                        // [page][KV head][keys | values][position][depth]
     float* scales;                         // [page][KV head][keys | values]
     unsigned* status;
-    int lanes_log2, row_tile, head_tile, row_heads, row_rows, row_magic, q_tiles, head_tiles;      // launcher-filled
+    int lanes_log2, lanes, lanes_magic, joint, row_tile, head_tile, row_heads, row_rows, row_magic, q_tiles, head_tiles;   // launcher-filled
     int page_heads, page_rows, page_magic, page_groups, page_units;
     float inv_hd;
 };

@@ -380,7 +380,7 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
     }
 }
 
-// A few rows of some query heads, or of key heads that go to no cache.
+// A few rows of some query heads, or of key heads that go to no cache; of all query heads and then all key heads (p.joint), which have the rows' cosines in common.
 template <int BF16, int LAY>
 __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, float* cs, int unit) {
     __shared__ long long s_pos[kRowTile];
@@ -388,20 +388,22 @@ __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, 
     const int tile = unit / p.head_tiles;
     int ht = unit - tile * p.head_tiles;
     const int r0 = tile * p.row_tile, n = min(p.row_tile, p.rows - r0);
-    const bool is_q = ht < p.q_tiles;
+    bool is_q = ht < p.q_tiles;
     if (!is_q) ht -= p.q_tiles;
-    const int all = is_q ? p.heads : p.kv_heads, h0 = ht * p.head_tile, nh = min(p.head_tile, all - h0);
+    const int h0 = ht * p.head_tile;
+    int nh = min(p.head_tile, (is_q ? p.heads : p.kv_heads) - h0);
     // (row, head) of this thread's group of lanes: `hpp` heads of `rpp` rows at a time, kAhead times as many rows on their way
     const int hpp = p.row_heads, rpp = p.row_rows;
-    const int c = tid & (L.group - 1), mine = tid >> L.log2_group, mr = mine * p.row_magic >> 16, mh = mine - mr * hpp;
+    const int mine = tid * p.lanes_magic >> 16, c = tid - mine * p.lanes, mr = mine * p.row_magic >> 16, mh = mine - mr * hpp;
     const bool mine_ok = 8 * c < L.hd && mr < rpp;
-    const size_t si = is_q ? p.q_stride : p.k_stride, so = is_q ? p.qo_stride : p.ko_stride;
+    size_t si = is_q ? p.q_stride : p.k_stride, so = is_q ? p.qo_stride : p.ko_stride;
     const uint16_t* src = (is_q ? p.q : p.k) + (size_t)(r0 + mr) * si + (h0 + mh) * L.hd;
     uint16_t* dst = (is_q ? p.q_out : p.k_out) + (size_t)(r0 + mr) * so + (h0 + mh) * L.hd;
     Raw next[kAhead];
+    int nh_load = nh;                                              // (of the heads that are being loaded)
     auto load = [&](int r, int h) {
         const uint16_t* x = src + (size_t)r * si + h * L.hd;
-        const bool ok = mine_ok && h + mh < nh;
+        const bool ok = mine_ok && h + mh < nh_load;
 #pragma unroll
         for (int e = 0; e < kAhead; ++e) {
             next[e].u = next[e].w = make_uint2(0, 0);
@@ -427,14 +429,15 @@ __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, 
         s_pos[tid] = pos;
     }
     const float* nw = is_q ? p.q_w : p.k_w;
-    const float eps = is_q ? p.q_eps : p.k_eps;
-    const Octet w = norm_weights<LAY>(nw, L, c, mine_ok);
+    float eps = is_q ? p.q_eps : p.k_eps;
+    Octet w = norm_weights<LAY>(nw, L, c, mine_ok);
     __syncthreads();
     if (p.turns) {
         fill_trig(p, L, cs, n, [&](int r) { return s_pos[r]; });
         __syncthreads();
     }
     const bool any_row = p.seqs.cu == nullptr;
+    bool more = p.joint;                                           // the key heads are still to come
     for (int h = 0, r = 0; h < nh;) {
         Raw cur[kAhead];
 #pragma unroll
@@ -442,7 +445,14 @@ __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, 
         const int h_now = h, r_now = r;
         r += kAhead * rpp;
         if (r >= n) { r = 0; h += hpp; }
-        if (h < nh) load(r, h);
+        const bool turn = more && h >= nh;
+        if (turn) {
+            src = p.k + (size_t)(r0 + mr) * p.k_stride + mh * L.hd;
+            si = p.k_stride;
+            nh_load = p.kv_heads;
+            h = 0;
+        }
+        if (turn || h < nh) load(r, h);
         uint16_t* y = dst + (size_t)r_now * so + h_now * L.hd;
         const bool head_ok = mine_ok && h_now + mh < nh;
 #pragma unroll
@@ -456,6 +466,15 @@ __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, 
                 rotate4(*reinterpret_cast<const float4*>(cs + row * L.hd + 4 * c), *reinterpret_cast<const float4*>(cs + row * L.hd + L.hd / 2 + 4 * c), o);
             if (live) store_pairs<BF16, LAY>(y, L, c, o);
             y += so * rpp;
+        }
+        if (turn) {
+            more = false;
+            dst = p.k_out + (size_t)(r0 + mr) * p.ko_stride + mh * L.hd;
+            so = p.ko_stride;
+            nh = nh_load;
+            nw = p.k_w;
+            eps = p.k_eps;
+            w = norm_weights<LAY>(nw, L, c, mine_ok);
         }
     }
 }
@@ -514,18 +533,23 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     a.lanes_log2 = 0;
     while (8 << a.lanes_log2 < a.head_dim) ++a.lanes_log2;
     const int per_pass = kRotThreads >> a.lanes_log2;
+    // Lanes of a head in row units: without norms they need not find one another, and heads of 96 or 80 depths leave none idle
+    a.lanes = paged || a.q_w || a.k_w ? 1 << a.lanes_log2 : a.head_dim / 8;
+    a.lanes_magic = (65536 + a.lanes - 1) / a.lanes;               // tid * magic >> 16 = tid / lanes
+    const int row_pass = kRotThreads / a.lanes;
     a.inv_hd = 1.0f / (float)a.head_dim;
     // row units: all heads of a few rows, so that they share the rows' cosines; of one row, as many heads as the block has at a time, while the
     // machine has room for more CTAs
     const int qh = a.q ? a.heads : 0, kh = a.k && !paged ? a.kv_heads : 0, most = qh > kh ? qh : kh;
     a.row_tile = (size_t)a.rows >= (size_t)sm_count * 8 ? kRowTile : 1;
-    a.head_tile = (size_t)a.rows >= (size_t)sm_count * 4 ? most : per_pass;
+    a.head_tile = (size_t)a.rows >= (size_t)sm_count * 4 ? most : row_pass;
     if (a.head_tile > most) a.head_tile = most;
     a.q_tiles = qh ? (qh + a.head_tile - 1) / a.head_tile : 0;
-    a.head_tiles = a.q_tiles + (kh ? (kh + a.head_tile - 1) / a.head_tile : 0);
-    a.row_heads = a.head_tile < per_pass ? a.head_tile : per_pass;
+    a.joint = qh && kh && a.head_tile == most;
+    a.head_tiles = a.joint ? 1 : a.q_tiles + (kh ? (kh + a.head_tile - 1) / a.head_tile : 0);
+    a.row_heads = a.head_tile < row_pass ? a.head_tile : row_pass;
     if (a.row_heads < 1) a.row_heads = 1;
-    a.row_rows = per_pass / a.row_heads;
+    a.row_rows = row_pass / a.row_heads;
     a.row_magic = (65536 + a.row_heads - 1) / a.row_heads;         // mine * magic >> 16 = mine / row_heads for mine below 256
     const long long row_units = (long long)((a.rows + a.row_tile - 1) / a.row_tile) * a.head_tiles;
     long long page_units = 0;
