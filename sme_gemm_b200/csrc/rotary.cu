@@ -21,7 +21,7 @@ namespace smeg {
 namespace {
 
 constexpr int kRotThreads = 128;
-constexpr int kRowTile = 4;                        // rows of a CTA of query heads, at most
+constexpr int kRowTile = 8;                        // rows of a CTA of query heads, at most
 constexpr int kHeld = 8;                           // runs of eight depths that a thread of a page's CTA keeps
 constexpr int kPageHeads = 32;                     // heads of a page's CTA, at most
 constexpr int kAhead = 4;                          // and that a thread of a row's CTA has on their way
@@ -538,10 +538,10 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     a.lanes_magic = (65536 + a.lanes - 1) / a.lanes;               // tid * magic >> 16 = tid / lanes
     const int row_pass = kRotThreads / a.lanes;
     a.inv_hd = 1.0f / (float)a.head_dim;
-    // row units: all heads of a few rows, so that they share the rows' cosines; of one row, as many heads as the block has at a time, while the
-    // machine has room for more CTAs
+    // row units: all heads of a few rows, so that they share the rows' cosines -- as many rows as the block's threads have on their way; of one row, as many
+    // heads as the block has at a time, while the machine has room for more CTAs.  (us with four and with eight rows: 5000 rows of 6 heads of 64, which
+    // are eight at a time, 6.8 and 5.4; 8192 rows of 28 / 4 heads of 96, four at a time, 22.8 and 24.2)
     const int qh = a.q ? a.heads : 0, kh = a.k && !paged ? a.kv_heads : 0, most = qh > kh ? qh : kh;
-    a.row_tile = (size_t)a.rows >= (size_t)sm_count * 8 ? kRowTile : 1;
     a.head_tile = (size_t)a.rows >= (size_t)sm_count * 4 ? most : row_pass;
     if (a.head_tile > most) a.head_tile = most;
     a.q_tiles = qh ? (qh + a.head_tile - 1) / a.head_tile : 0;
@@ -550,6 +550,7 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     a.row_heads = a.head_tile < row_pass ? a.head_tile : row_pass;
     if (a.row_heads < 1) a.row_heads = 1;
     a.row_rows = row_pass / a.row_heads;
+    a.row_tile = (size_t)a.rows < (size_t)sm_count * 8 ? 1 : (kAhead * a.row_rows < kRowTile ? kAhead * a.row_rows : kRowTile);
     a.row_magic = (65536 + a.row_heads - 1) / a.row_heads;         // mine * magic >> 16 = mine / row_heads for mine below 256
     const long long row_units = (long long)((a.rows + a.row_tile - 1) / a.row_tile) * a.head_tiles;
     long long page_units = 0;
