@@ -490,36 +490,47 @@ __global__ void __launch_bounds__(kRotThreads, 5) rotate_append_kernel(const __g
     else row_unit<BF16, LAY>(p, L, trig_s, blockIdx.x - p.page_units);
 }
 
-// The values of whole pages: 16 codes a thread.
+// The values of whole pages: a CTA takes kReadCodes of a page's codes, a thread eight at a time, so that a warp's loads and stores are whole lines.
+constexpr int kReadThreads = 256, kReadCodes = 2 * 8 * kReadThreads;
 template <int BF16>
-__global__ void __launch_bounds__(256) paged_read_kernel(uint16_t* __restrict__ out, const uint8_t* __restrict__ codes, const float* __restrict__ scales,
-                                                         const int* __restrict__ ids, size_t n, size_t per_page, size_t block, int pages, int out_vec, unsigned* status) {
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(uint16_t* __restrict__ out, const uint8_t* __restrict__ codes, const float* __restrict__ scales,
+                                                                  const int* __restrict__ ids, unsigned parts, unsigned per_page, unsigned block, int pages, int out_vec,
+                                                                  unsigned* status) {
     pdl_launch_dependents();
     pdl_wait();
-    const size_t idx = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 16;
-    if (idx >= n * per_page) return;
-    const size_t i = idx / per_page, off = idx - i * per_page;
+    const unsigned i = blockIdx.x / parts, off0 = (blockIdx.x - i * parts) * kReadCodes + 8 * threadIdx.x;
     const int id = ids[i];
-    uint4 w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-    float s = 0.0f;
-    if (id >= 0 && id < pages) {
-        w = *reinterpret_cast<const uint4*>(codes + (size_t)id * per_page + off);
-        s = scales[(size_t)id * (per_page / block) + off / block];
-    } else if (off == 0) {
-        atomicOr(status, STATUS_PAGE);
-    }
-    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
-    uint32_t o[8];
+    const bool there = id >= 0 && id < pages;
+    if (!there && off0 == 0) atomicOr(status, STATUS_PAGE);
+    const uint8_t* x = codes + (size_t)(there ? id : 0) * per_page;
+    const float* sc = scales + (size_t)(there ? id : 0) * (per_page / block);
+    uint16_t* y = out + (size_t)i * per_page;
+    uint2 w[2];
+    float s[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        o[e] = pack2_t<BF16>(byte_value(r[e / 2], 2 * (e & 1)) * s, byte_value(r[e / 2], 2 * (e & 1) + 1) * s);
+    for (int h = 0; h < 2; ++h) {
+        const unsigned off = off0 + h * (kReadCodes / 2);
+        w[h] = make_uint2(0x80808080u, 0x80808080u);
+        s[h] = 0.0f;
+        if (there && off < per_page) {
+            w[h] = *reinterpret_cast<const uint2*>(x + off);
+            s[h] = sc[off / block];
+        }
     }
-    if (out_vec) {
-        *reinterpret_cast<uint4*>(out + idx) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(out + idx + 8) = make_uint4(o[4], o[5], o[6], o[7]);
-    } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) out[idx + e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
+    for (int h = 0; h < 2; ++h) {
+        const unsigned off = off0 + h * (kReadCodes / 2);
+        if (off >= per_page) break;
+        const uint32_t r[2] = {w[h].x, w[h].y};
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = pack2_t<BF16>(byte_value(r[e / 2], 2 * (e & 1)) * s[h], byte_value(r[e / 2], 2 * (e & 1) + 1) * s[h]);
+        if (out_vec) {
+            *reinterpret_cast<uint4*>(y + off) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[off + e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
+        }
     }
 }
 
@@ -582,12 +593,14 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
 
 cudaError_t paged_read_launch(uint16_t* out, const uint8_t* codes, const float* scales, const int* ids, size_t n, int pages, int page, int kv_heads, int head_dim,
                               int bf16, unsigned* status, cudaStream_t stream) {
-    const size_t block = (size_t)page * head_dim, per_page = block * kv_heads * 2, threads = n * per_page / 16, grid = (threads + 255) / 256;
-    if (grid == 0) return cudaSuccess;
-    if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
+    const size_t block = (size_t)page * head_dim, per_page = block * kv_heads * 2, parts = (per_page + kReadCodes - 1) / kReadCodes;
+    if (n == 0) return cudaSuccess;
+    if (per_page > 0xffffffffu - kReadCodes || n > 0x7fffffffu / parts) return cudaErrorInvalidValue;
     const int vec = ((uintptr_t)out & 15) == 0;
-    if (bf16) return launch_pdl(paged_read_kernel<1>, dim3((unsigned)grid), dim3(256), 0, stream, out, codes, scales, ids, n, per_page, block, pages, vec, status);
-    return launch_pdl(paged_read_kernel<0>, dim3((unsigned)grid), dim3(256), 0, stream, out, codes, scales, ids, n, per_page, block, pages, vec, status);
+    const dim3 grid((unsigned)(n * parts));
+    if (bf16)
+        return launch_pdl(paged_read_kernel<1>, grid, dim3(kReadThreads), 0, stream, out, codes, scales, ids, (unsigned)parts, (unsigned)per_page, (unsigned)block, pages, vec, status);
+    return launch_pdl(paged_read_kernel<0>, grid, dim3(kReadThreads), 0, stream, out, codes, scales, ids, (unsigned)parts, (unsigned)per_page, (unsigned)block, pages, vec, status);
 }
 
 }  // namespace smeg
