@@ -286,6 +286,7 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
     const int block = page * L.hd;                                 // bytes of one head's keys or values in a page
     uint8_t* dst = p.codes + (((size_t)id * p.kv_heads + h0) * 2 + which) * block + at * L.hd;
     float* scale = p.scales + ((size_t)id * p.kv_heads + h0) * 2 + which;
+    const float old = tid < nh && at > 0 ? scale[2 * tid] : 0.0f;  // (asked for here, used behind the search)
     if (tid < kPageHeads) s_max[tid] = 0;
     const Octet w = norm_weights<LAY>(norm ? p.k_w : nullptr, L, c, mine_ok);
     // The first row's angles are formed here; row r is r steps of the frequencies further, by the sum formulas (steps: [256][cosines, sines], 32 bits)
@@ -303,7 +304,7 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
             float4 u = make_float4(1.f, 1.f, 1.f, 1.f), v = make_float4(0.f, 0.f, 0.f, 0.f);
             const float* t = p.steps + r * 2 * L.half + 4 * c;
             if (LAY != kAny || L.half % 4 == 0) {
-                if (4 * c < L.half) {
+                if (4 * c < L.half && r > 0) {                     // (no load stands before a single row's codes)
                     u = *reinterpret_cast<const float4*>(t);
                     v = *reinterpret_cast<const float4*>(t + L.half);
                 }
@@ -340,7 +341,7 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
     if (mine_ok && c == 0) atomicMax(&s_max[mh], mx);
     __syncthreads();
     if (tid < nh) {
-        const float old = at == 0 ? 0.0f : scale[2 * tid], top = __uint_as_float(s_max[tid]);
+        const float top = __uint_as_float(s_max[tid]);
         float now = top < __uint_as_float(0x7f800000u) ? __fdiv_rn(top, 127.0f) : __uint_as_float(0x7fc00000u);
         if (now < kLeastScale) now = 0.0f;
         if (old >= now || old != old) now = old;                   // (a block that holds a NaN or an infinity is NaN until its page starts over)
