@@ -217,12 +217,18 @@ struct PagedMaps {
     CUtensorMap codes;                               // [block][position][depth], swizzled boxes of 64 or 128 depths x 16 or 32 positions
 };
 
-// HC: depths in units of 64 (1, 2 or 4); NT: tiles of eight query rows.
+// CTAs of an SM and stages of a warp's ring.  HC: depths in units of 64 (1, 2 or 4); NT: tiles of eight query rows.
+// (Heads of 64 have little work behind a load, so more warps serve them better than deeper rings.  us with three CTAs of four stages and as it is: 128
+// sequences of 2000, 32 / 4 heads, 50.2 and 42.6; 512 rows behind 3500, 24 / 3 heads, 119.6 and 113.9; 64 x 5 rows of 3000 80.6 and 78.9.  Heads of 128 with three
+// CTAs of two stages: no faster than two of three.)
+__host__ __device__ constexpr int ctas_of(int hc, int nt) { return hc == 4 ? 1 : (hc == 2 ? 2 : (nt == 1 ? 5 : 4)); }
+__host__ __device__ constexpr int stages_of(int hc) { return hc == 1 ? 2 : 3; }
+
 template <int BF16, int HC, int NT>
-__global__ void __launch_bounds__(kPaThreads, HC == 4 ? 1 : (HC == 2 ? 2 : 3)) paged_attend_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedAttendArgs p) {
+__global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedAttendArgs p) {
     constexpr int MT = 4 * HC;                       // tiles of 16 depths
     constexpr int NR = 8 * NT;
-    constexpr int kStages = HC == 1 ? 4 : 3;
+    constexpr int kStages = stages_of(HC);
     constexpr int kPitch = HC == 1 ? 64 : 128, kPanel = 32 * kPitch, kPanels = HC == 4 ? 2 : 1;   // bytes of a key, of 32 keys; panels of 128 depths
     constexpr int kHalf = kPanels * kPanel, kStage = 2 * kHalf;                                   // keys, then values
     extern __shared__ unsigned char smem_dyn[];
@@ -752,7 +758,12 @@ __global__ void __launch_bounds__(kPjThreads) paged_join_items_kernel(const __gr
     }
 }
 
-int tile_rows_of(int group, int max_rows) { return (long long)group * max_rows > 8 ? 16 : 8; }
+// Query rows of a tile: 16 share the unpacking of the codes, and 8 leave fewer rows empty.  A tile of 8 costs three fifths of one of 16 (512 rows behind 3500, heads of 64, us:
+// 16 119, 8 139; of 128: 73 and 90), so 8 win for up to 8, 17 to 24 and 33 to 40 rows of a sequence and KV head (12 x 5 rows x 8 heads of 64: 20.6 and 19.4).
+int tile_rows_of(int group, int max_rows) {
+    const long long n = (long long)group * max_rows, by8 = (n + 7) / 8, by16 = (n + 15) / 16;
+    return 3 * by8 <= 5 * by16 ? 8 : 16;
+}
 
 long long items_bound(const PagedAttendArgs& a, int tile_rows) {
     return ((long long)a.seqs.rows * (a.heads / a.kv_heads) / tile_rows + a.seqs.seqs) * a.kv_heads;
@@ -761,7 +772,7 @@ long long items_bound(const PagedAttendArgs& a, int tile_rows) {
 // CTAs: as many as the GPU holds at a time (the occupancy of the variant), no more than there can be units.
 int workers_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
-    const int per_sm = hc == 4 ? 1 : (hc == 2 ? 2 : 3);
+    const int per_sm = ctas_of(hc, tile_rows / 8);
     const long long room = ((long long)a.seqs.cols << a.seqs.page_log2), tiles = (room + kUnitKeys - 1) / kUnitKeys;
     const long long items = items_bound(a, tile_rows);
     const long long most = (long long)sm_count * per_sm, units = items * (tiles > 0 ? tiles : 1);
@@ -782,7 +793,7 @@ cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t st
     if (enc(&m.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, (void*)a.codes, dim, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
             HC == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    const size_t smem = 1024 + (size_t)kPaWarps * (HC == 1 ? 4 : 3) * 4096 * HC;
+    const size_t smem = 1024 + (size_t)kPaWarps * stages_of(HC) * 4096 * HC;
     static std::atomic<int> attr_dev{-1};          // the opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);
