@@ -345,6 +345,32 @@ def run_profile_case(args):
         q = torch.randn(rows, 4096, device="cuda", dtype=torch.float16)
         out = torch.zeros(rows, 4096, device="cuda")
         fn, nsets = (lambda i: caches[i].attend_causal(q, rows, out)), 6
+    elif name in ("paged_append", "paged_decode", "packed_prompts"):
+        # 32 heads of 128 on 8 KV heads: 4096 rows of five prompts normalised, rotated and appended; 64 sequences of 500 to 5000 positions, a token each;
+        # causal attention over eleven prompts of 83 to 1040 rows
+        heads, kv, hd, page = 32, 8, 128, 64
+        lens = {"paged_append": [1475, 1147, 819, 491, 164], "paged_decode": [500 + 4500 * i // 63 for i in range(64)],
+                "packed_prompts": [1040, 966, 893, 820, 747, 673, 600, 526, 453, 200, 83]}[name]
+        decode = name == "paged_decode"
+        rows, seqs, cols = len(lens) if decode else sum(lens), len(lens), -(-max(lens) // page)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+        cu = ints([0] + (list(range(1, seqs + 1)) if decode else np.cumsum(lens).tolist()))
+        x = torch.randn(rows, (heads + 2 * kv) * hd, device="cuda").to(torch.bfloat16)
+        q, k, v = x.split([heads * hd, kv * hd, kv * hd], 1)
+        out = torch.empty(rows, heads * hd, device="cuda", dtype=torch.bfloat16)
+        if name == "packed_prompts":
+            fn, nsets = (lambda i: sg.attend_packed(q, k, v, cu, out, heads, kv)), 1
+        else:
+            cache = sg.PagedKvCache(heads, kv, hd, seqs * cols, page)
+            batch = sg.PagedBatch(cu, ints([n - 1 for n in lens] if decode else [0] * seqs), torch.arange(seqs * cols, dtype=torch.int32, device="cuda").view(seqs, cols))
+            if decode:
+                cache.codes.random_(0, 256)
+                cache.scales.fill_(0.01)
+                fn, nsets = (lambda i: cache.attend(q, batch, out)), 1
+            else:
+                rotary, norm = sg.Rotary(hd), sg.Norm.rms(np.ones(hd, np.float32), 1e-6)
+                k_out = torch.empty(rows, kv * hd, device="cuda", dtype=torch.bfloat16)
+                fn, nsets = (lambda i: cache.append(k, v, batch, rotary, k_norm=norm, k_out=k_out, q=q, q_out=out, q_norm=norm)), 1
     else:
         fn, nsets, _ = kernel_cases(torch, sg, orc)[name]()
     for i in range(6):
@@ -756,7 +782,7 @@ def main():
                     help="N > 1: fused sum + finish over peer memory (this library's kernel) or NCCL all-reduce + finishing pass")
     ap.add_argument("--profile-case", default=None,
                     choices=["q4_gemv", "q2_gemv", "q1_gemv", "q4_prefill", "q1_prefill", "mlp_gate_up", "mlp_down", "q4_rows8_bf16",
-                             "attn_prefill", "attn_decode"],
+                             "attn_prefill", "attn_decode", "paged_append", "paged_decode", "packed_prompts"],
                     help="run six plain launches of one kernel and exit (for profiler captures)")
     args = ap.parse_args()
     if args.profile_case:

@@ -24,7 +24,7 @@ constexpr int kRotThreads = 128;
 constexpr int kRowTile = 8;                        // rows of a CTA of query heads, at most
 constexpr int kHeld = 8;                           // runs of eight depths that a thread of a page's CTA keeps
 constexpr int kPageHeads = 32;                     // heads of a page's CTA, at most
-constexpr int kAhead = 4;                          // and that a thread of a row's CTA has on their way
+constexpr int kAhead = 2;                          // and that a thread of a row's CTA has on their way
 constexpr float kLeastScale = 7.703719777548943e-34f;   // 2^-110: a smaller scale has no reciprocal to speak of and counts as zero
 constexpr float kRound = 12582912.0f;              // 1.5 * 2^23: what is added to it is rounded to an integer, in the low bits of the sum
 
@@ -240,15 +240,24 @@ __device__ __forceinline__ int count_upto(int n, long long x, Key key) {
     return got;
 }
 
-// A (page, KV heads) of the batch, keys or values.  A thread keeps what it loaded -- kHeld runs of eight, as they lie -- from the search for the largest
-// magnitude to the codes, and norms and turns them a second time; a longer page is read twice.
-template <int BF16, int LAY>
+// The largest of x, |a|, |b|; NaN where one of them is.
+__device__ __forceinline__ float max_abs3(float x, float a, float b) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(a), "f"(b));
+    return r;
+}
+
+// A (page, KV heads) of the batch, keys or values.  A thread keeps what it has -- kHeld runs of eight -- from the search for the largest magnitude to the codes: values
+// as they were loaded, keys as they come out of norm and rotation, in 32 bits in shared memory (a place of each thread's own).  A longer page is read, and its keys
+// are formed, twice.
+template <int BF16, int LAY, int KEYS>
 __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L, float* cs, int unit) {
     __shared__ unsigned s_max[kPageHeads];
     __shared__ float s_inv[kPageHeads], s_ratio[kPageHeads];
     const PackedSeqs& B = p.seqs;
     const int tid = threadIdx.x, page = 1 << B.page_log2;
-    const int which = unit & 1, slot = (unit >> 1) / p.page_groups, hg = (unit >> 1) - slot * p.page_groups;
+    constexpr int which = KEYS ? 0 : 1;
+    const int slot = (unit >> 1) / p.page_groups, hg = (unit >> 1) - slot * p.page_groups;
     const int h0 = hg * p.page_heads, nh = min(p.page_heads, p.kv_heads - h0);
     const int s = count_upto(B.seqs, slot, [&](int i) { int f; seq_rows(B, i, &f); return first_slot(f, i, B.page_log2, 2); }) - 1;
     if (s < 0) return;
@@ -263,9 +272,9 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
     // (row, head) of this thread's group of lanes, pairs 4 c ... of it
     const int c = tid & (L.group - 1), mine = tid >> L.log2_group, rpp = p.page_rows, mr = mine * p.page_magic >> 16, mh = mine - mr * p.page_heads;
     const bool mine_ok = 8 * c < L.hd && mr < rpp && mh < nh;
-    const bool keys = which == 0, norm = keys && p.k_w != nullptr, rotate = keys && p.turns != nullptr;
-    const size_t stride = keys ? p.k_stride : p.v_stride, step = stride * rpp;
-    const uint16_t* src = (keys ? p.k : p.v) + (size_t)(first + r0 + mr) * stride + (h0 + mh) * L.hd;
+    const bool norm = KEYS && p.k_w != nullptr, rotate = KEYS && p.turns != nullptr;
+    const size_t stride = KEYS ? p.k_stride : p.v_stride, step = stride * rpp;
+    const uint16_t* src = (KEYS ? p.k : p.v) + (size_t)(first + r0 + mr) * stride + (h0 + mh) * L.hd;
     const int left = mine_ok ? n - mr : 0;                         // rows from this thread's first one on
     Raw held[kHeld];
     auto load = [&](int c0) {                                      // rows c0 + mr, c0 + mr + rpp, ...
@@ -325,17 +334,36 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
         }
         return o;
     };
-    unsigned mx = 0;                                               // (of the bits: an infinity or NaN is larger than every number)
+    float4* kept = reinterpret_cast<float4*>(cs + L.hd) + tid;     // [run][first, second members][thread]
+    float top_f = 0.0f;
+    unsigned top_16 = 0;                                           // (of the bits of two values: an infinity or NaN is larger than every number)
     const int chunk = kHeld * rpp;
+    const bool keep = n <= chunk;
     for (int c0 = 0; c0 < n; c0 += chunk) {
         if (c0) load(c0);
 #pragma unroll
         for (int e = 0; e < kHeld; ++e) {
             if (c0 + e * rpp >= n) break;                          // (the same for the whole block)
-            const Octet o = treat(e, c0 + e * rpp + mr);
+            if (KEYS) {
+                const Octet o = treat(e, c0 + e * rpp + mr);
+                if (c0 + e * rpp >= left) continue;                // (no row: zeros, and under a norm with an eps of zero not even those)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mx = max(mx, max(__float_as_uint(fabsf(o.a[j])), __float_as_uint(fabsf(o.b[j]))));
+                for (int j = 0; j < 4; ++j) top_f = max_abs3(top_f, o.a[j], o.b[j]);
+                if (keep) {
+                    kept[(2 * e) * kRotThreads] = make_float4(o.a[0], o.a[1], o.a[2], o.a[3]);
+                    kept[(2 * e + 1) * kRotThreads] = make_float4(o.b[0], o.b[1], o.b[2], o.b[3]);
+                }
+            } else {
+                const unsigned r[4] = {held[e].u.x, held[e].u.y, held[e].w.x, held[e].w.y};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top_16 = __vmaxu2(top_16, r[j] & 0x7fff7fffu);
+            }
         }
+    }
+    unsigned mx = __float_as_uint(top_f);
+    if (!KEYS) {
+        const float2 f = both<BF16>(top_16);
+        mx = max(__float_as_uint(f.x), __float_as_uint(f.y));
     }
     mx = head_max(mx, L.group);
     if (mine_ok && c == 0) atomicMax(&s_max[mh], mx);
@@ -366,14 +394,21 @@ __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L,
         }
     const float inv = mine_ok ? s_inv[mh] : 0.0f;
     uint8_t* to = dst + mh * 2 * block + mr * L.hd;
-    uint16_t* ko = keys && p.k_out ? p.k_out + (size_t)(first + r0 + mr) * p.ko_stride + (h0 + mh) * L.hd : nullptr;
+    uint16_t* ko = KEYS && p.k_out ? p.k_out + (size_t)(first + r0 + mr) * p.ko_stride + (h0 + mh) * L.hd : nullptr;
     for (int c0 = 0; c0 < n; c0 += chunk) {
-        if (n > chunk) load(c0);
+        if (!keep) load(c0);
 #pragma unroll
         for (int e = 0; e < kHeld; ++e) {
             const int r = c0 + e * rpp;
             if (r >= n) break;
-            const Octet o = treat(e, r + mr);
+            Octet o;
+            if (KEYS && keep) {
+                const float4 u = kept[(2 * e) * kRotThreads], v = kept[(2 * e + 1) * kRotThreads];
+                o.a[0] = u.x; o.a[1] = u.y; o.a[2] = u.z; o.a[3] = u.w;
+                o.b[0] = v.x; o.b[1] = v.y; o.b[2] = v.z; o.b[3] = v.w;
+            } else {
+                o = treat(e, r + mr);
+            }
             if (r >= left) continue;
             store_codes<LAY>(to + r * L.hd, L, c, o, inv);
             if (ko) store_pairs<BF16, LAY>(ko + (size_t)r * p.ko_stride, L, c, o);
@@ -480,15 +515,28 @@ __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, 
     }
 }
 
+__device__ __forceinline__ HeadLay head_lay(const RotateArgs& p) {
+    HeadLay L;
+    L.hd = p.head_dim; L.half = p.rot / 2; L.inter = p.interleaved; L.log2_group = p.lanes_log2; L.group = 1 << p.lanes_log2; L.inv_hd = p.inv_hd;
+    return L;
+}
+// Rows alone, and pages with rows: in one kernel the pages' registers cost the rows 3 to 14 %.  The next grid starts when these CTAs have gone, and not where they begin: its
+// CTAs would take the places that are free by then, and gather on a few SMs (rows at the start and so, us: 2001 of 28 / 4 heads of 96 8.2 and 7.7, 300 of 32 / 8 of 128 5.7 and
+// 4.4; append and read of 48 rows 7.5 and 6.6).  Rows with two runs a thread on their way and eight CTAs an SM: 800 rows 7.5 -> 5.4, 8192 37.2 -> 36.0 us.
+template <int BF16, int LAY>
+__global__ void __launch_bounds__(kRotThreads, 8) rotate_rows_kernel(const __grid_constant__ RotateArgs p) {
+    extern __shared__ __align__(16) float trig_s[];
+    pdl_wait();
+    row_unit<BF16, LAY>(p, head_lay(p), trig_s, blockIdx.x);
+}
 template <int BF16, int LAY>
 __global__ void __launch_bounds__(kRotThreads, 5) rotate_append_kernel(const __grid_constant__ RotateArgs p) {
     extern __shared__ __align__(16) float trig_s[];
-    HeadLay L;
-    L.hd = p.head_dim; L.half = p.rot / 2; L.inter = p.interleaved; L.log2_group = p.lanes_log2; L.group = 1 << p.lanes_log2; L.inv_hd = p.inv_hd;
-    pdl_launch_dependents();
+    const HeadLay L = head_lay(p);
     pdl_wait();
-    if ((int)blockIdx.x < p.page_units) page_unit<BF16, LAY>(p, L, trig_s, blockIdx.x);
-    else row_unit<BF16, LAY>(p, L, trig_s, blockIdx.x - p.page_units);
+    if ((int)blockIdx.x >= p.page_units) row_unit<BF16, LAY>(p, L, trig_s, blockIdx.x - p.page_units);
+    else if (blockIdx.x & 1) page_unit<BF16, LAY == kAny ? kAny : kNeighbours, 0>(p, L, trig_s, blockIdx.x);
+    else page_unit<BF16, LAY, 1>(p, L, trig_s, blockIdx.x);
 }
 
 // The values of whole pages: a CTA takes kReadCodes of a page's codes, a thread eight at a time, so that a warp's loads and stores are whole lines.
@@ -497,7 +545,6 @@ template <int BF16>
 __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(uint16_t* __restrict__ out, const uint8_t* __restrict__ codes, const float* __restrict__ scales,
                                                                   const int* __restrict__ ids, unsigned parts, unsigned per_page, unsigned block, int pages, int out_vec,
                                                                   unsigned* status) {
-    pdl_launch_dependents();
     pdl_wait();
     const unsigned i = blockIdx.x / parts, off0 = (blockIdx.x - i * parts) * kReadCodes + 8 * threadIdx.x;
     const int id = ids[i];
@@ -550,7 +597,7 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     a.lanes_magic = (65536 + a.lanes - 1) / a.lanes;               // tid * magic >> 16 = tid / lanes
     const int row_pass = kRotThreads / a.lanes;
     a.inv_hd = 1.0f / (float)a.head_dim;
-    // row units: all heads of a few rows, so that they share the rows' cosines -- as many rows as the block's threads have on their way; of one row, as many
+    // row units: all heads of a few rows, so that they share the rows' cosines -- four rows for each that the block's threads have at a time; of one row, as many
     // heads as the block has at a time, while the machine has room for more CTAs.  (us with four and with eight rows: 5000 rows of 6 heads of 64, which
     // are eight at a time, 6.8 and 5.4; 8192 rows of 28 / 4 heads of 96, four at a time, 22.8 and 24.2)
     const int qh = a.q ? a.heads : 0, kh = a.k && !paged ? a.kv_heads : 0, most = qh > kh ? qh : kh;
@@ -562,7 +609,7 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     a.row_heads = a.head_tile < row_pass ? a.head_tile : row_pass;
     if (a.row_heads < 1) a.row_heads = 1;
     a.row_rows = row_pass / a.row_heads;
-    a.row_tile = (size_t)a.rows < (size_t)sm_count * 8 ? 1 : (kAhead * a.row_rows < kRowTile ? kAhead * a.row_rows : kRowTile);
+    a.row_tile = (size_t)a.rows < (size_t)sm_count * 8 ? 1 : (4 * a.row_rows < kRowTile ? 4 * a.row_rows : kRowTile);
     a.row_magic = (65536 + a.row_heads - 1) / a.row_heads;         // mine * magic >> 16 = mine / row_heads for mine below 256
     const long long row_units = (long long)((a.rows + a.row_tile - 1) / a.row_tile) * a.head_tiles;
     long long page_units = 0;
@@ -584,11 +631,14 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     if (row_units + page_units > 0x7fffffffll) return cudaErrorInvalidValue;
     if (row_units + page_units == 0) return cudaSuccess;
     a.page_units = (int)page_units;
-    const size_t smem = a.turns ? (size_t)a.row_tile * a.head_dim * sizeof(float) : 0;
+    const size_t rows_smem = a.turns ? (size_t)a.row_tile * a.head_dim * sizeof(float) : 0;
+    const size_t page_smem = paged ? a.head_dim * sizeof(float) + (size_t)kHeld * 8 * kRotThreads * sizeof(float) : 0;
+    const size_t smem = rows_smem > page_smem ? rows_smem : page_smem;
     typedef void (*Kern)(RotateArgs);
-    static const Kern kerns[2][4] = {{rotate_append_kernel<0, 0>, rotate_append_kernel<0, 1>, rotate_append_kernel<0, 2>, rotate_append_kernel<0, 3>},
-                                     {rotate_append_kernel<1, 0>, rotate_append_kernel<1, 1>, rotate_append_kernel<1, 2>, rotate_append_kernel<1, 3>}};
-    const Kern kern = kerns[bf16 ? 1 : 0][lay];
+#define SMEG_ROT(K) {{K<0, 0>, K<0, 1>, K<0, 2>, K<0, 3>}, {K<1, 0>, K<1, 1>, K<1, 2>, K<1, 3>}}
+    static const Kern kerns[2][2][4] = {SMEG_ROT(rotate_rows_kernel), SMEG_ROT(rotate_append_kernel)};
+#undef SMEG_ROT
+    const Kern kern = kerns[paged ? 1 : 0][bf16 ? 1 : 0][lay];
     return launch_pdl(kern, dim3((unsigned)(row_units + page_units)), dim3(kRotThreads), smem, stream, a);
 }
 

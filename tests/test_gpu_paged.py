@@ -820,3 +820,13 @@ def test_refusals_of_overlaps_and_of_tables_without_pages():
     with pytest.raises(AssertionError, match="a page for each"):
         sg.PagedBatch(_int([0, 4]), _int([0]), torch.zeros(1, 0, dtype=torch.int32, device="cuda"))
     assert sg.PagedBatch(_int([0]), torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, 3, dtype=torch.int32, device="cuda")).seqs() == 0
+
+
+@pytest.mark.parametrize("kv,rows", [(3, [3, 1, 9]), (1, [5, 2, 70])])
+def test_a_norm_without_an_eps(kv, rows):
+    """Lanes without a row have nothing to normalise: no NaN of theirs reaches a scale."""
+    pool = Pool(2 * kv, kv, 64, 16, 3, 8, seed=kv)
+    norm = sg.Norm.rms(np.ones(64, np.float32), 0.0)
+    pool.append(rows, (), sg.Rotary(64), norm)
+    pool.append([1, 1, 1], (), sg.Rotary(64), norm)
+    pool.check(times=2)
