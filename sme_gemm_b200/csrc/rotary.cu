@@ -254,15 +254,17 @@ template <int BF16, int LAY, int KEYS>
 __device__ __forceinline__ void page_unit(const RotateArgs& p, const HeadLay& L, float* cs, int unit) {
     __shared__ unsigned s_max[kPageHeads];
     __shared__ float s_inv[kPageHeads], s_ratio[kPageHeads];
+    __shared__ int s_start[kRotThreads];
     const PackedSeqs& B = p.seqs;
     const int tid = threadIdx.x, page = 1 << B.page_log2;
+    if (tid < B.seqs) s_start[tid] = B.starts[tid];                // (asked for together with the row offsets, not behind them)
     constexpr int which = KEYS ? 0 : 1;
     const int slot = (unit >> 1) / p.page_groups, hg = (unit >> 1) - slot * p.page_groups;
     const int h0 = hg * p.page_heads, nh = min(p.page_heads, p.kv_heads - h0);
     const int s = count_upto(B.seqs, slot, [&](int i) { int f; seq_rows(B, i, &f); return first_slot(f, i, B.page_log2, 2); }) - 1;
     if (s < 0) return;
     int first;
-    const int rows = seq_rows(B, s, &first), start = B.starts[s];
+    const int rows = seq_rows(B, s, &first), start = s < kRotThreads ? s_start[s] : B.starts[s];
     if (start < 0) return;
     const long long piece = slot - first_slot(first, s, B.page_log2, 2);
     const int d = start & (page - 1);                              // slot of the sequence's first row in its page
@@ -449,7 +451,9 @@ __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, 
     };
     load(0, 0);                                                    // (on their way while the rows' angles are formed)
     // positions, -1 for a row that is nobody's
+    __shared__ int s_start[kRotThreads];
     int s = 0;
+    if (p.seqs.cu && tid < p.seqs.seqs) s_start[tid] = p.seqs.starts[tid];
     if (p.seqs.cu) s = count_upto(p.seqs.seqs, r0, [&](int i) { int f; seq_rows(p.seqs, i, &f); return (long long)f; }) - 1;
     if (tid < n) {
         long long pos = p.start + r0 + tid;
@@ -459,7 +463,7 @@ __device__ __forceinline__ void row_unit(const RotateArgs& p, const HeadLay& L, 
             if (s < 0) s = 0;
             while (s + 1 < p.seqs.seqs && p.seqs.cu[s + 1] <= r0 + tid) ++s;
             m = seq_rows(p.seqs, s, &f);
-            const int st = p.seqs.starts[s];
+            const int st = s < kRotThreads ? s_start[s] : p.seqs.starts[s];
             pos = st >= 0 && r0 + tid >= f && r0 + tid < f + m ? (long long)st + (r0 + tid - f) : -1;
         }
         s_pos[tid] = pos;
