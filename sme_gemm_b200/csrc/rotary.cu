@@ -13,6 +13,11 @@
 // batch are CTAs of one launch.  A row's cosines and sines are formed once in shared memory and serve all of its query heads.  A page's CTA has few
 // heads, so there they are formed for its first row alone, and row r takes the sum formulas with the cosines and sines of r frequencies, which the
 // caller's table holds.
+//
+// Bytes bound it from some thousand rows on (each 16-bit value is read and written once, a cached one is read once and leaves as a byte), the instructions next to them:
+// 8192 rows of 32 + 8 normalised heads of 128 take 36 us (4.7 TB/s of 6.5 measured), without norms, 28 + 4 heads of 96, 22.4 (4.5); 4096 rows of five
+// prompts with their pages 32 us, 16 of them the queries', where the issue slots are 58 % busy.  Short calls are a chain of dependent loads -- row offsets, page number,
+// rows, scale -- and a launch: one row 2.0 us, 48 single rows into their pages 4.5.
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
