@@ -297,7 +297,7 @@ struct PagedAttendArgs {
     float scale_log2e;
     float* ws;                             // paged_attend_ws_floats()
     unsigned* status;
-    int q_vec, out_vec;                    // launcher-filled
+    int q_vec, out_vec, cluster_log2;      // launcher-filled; CTAs of an item's cluster, 0: shares and join
     FastDiv by_group, by_quads, by_par;    // / heads of a group, / (head_dim / 4), / rows that the join has at a time
 };
 size_t paged_attend_ws_floats(const PagedAttendArgs& a, int sm_count);

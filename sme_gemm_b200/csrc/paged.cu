@@ -5,7 +5,8 @@
 //
 // What bounds it is the cache: 2 bytes per position, KV head and depth, each read once for all query rows of a tile (a tile: 8 or 16 rows x heads
 // of a group).  The keys of all (sequence, row tile, KV head) are one line of units of 128 keys, cut into equal shares for as many CTAs as the GPU
-// holds, whatever the lengths; an item that a cut goes through is joined by a second kernel from the shares' unnormalised sums.  Within a unit a
+// holds, whatever the lengths; an item that a cut goes through is joined by a second kernel from the shares' unnormalised sums (few short items: by a cluster each, in
+// distributed shared memory).  Within a unit a
 // warp has 32 keys and needs no other warp until its share of an item is done.
 //
 // Both products are mma.m16n8k16 with the cache as the 16-row operand, so that up to eight query rows cost one column tile:
@@ -228,7 +229,19 @@ struct PagedMaps {
 __host__ __device__ constexpr int ctas_of(int hc, int nt) { return hc == 4 ? 1 : (hc == 2 ? 2 : (nt == 1 ? 5 : 4)); }
 __host__ __device__ constexpr int stages_of(int hc) { return hc == 1 ? 2 : 3; }
 
-template <int BF16, int HC, int NT>
+__device__ __forceinline__ float ld_dsmem(uint32_t cluster_addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_dsmem4(uint32_t cluster_addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+// CL: the CTAs of a cluster (2^cluster_log2 of them) share one item's units and meet in distributed shared memory, without a second kernel: for few items of few units.
+template <int BF16, int HC, int NT, int CL>
 __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedAttendArgs p) {
     constexpr int MT = 4 * HC;                       // tiles of 16 depths
     constexpr int NR = 8 * NT;
@@ -253,18 +266,32 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
     pdl_wait();
     pdl_launch_dependents();                         // (behind the wait: what ran before this kernel is there for the next one's index work, too)
     long long total;
-    Place at;
-    if (!find_unit<kPaThreads>(p, NR, [&](long long n) { return share_begin(n, gridDim.x, blockIdx.x); }, &total, &at)) return;   // (with barriers: the mbarriers are set up)
     Walk now;
-    now.s = at.s;
-    now.left = share_begin(total, gridDim.x, blockIdx.x + 1) - share_begin(total, gridDim.x, blockIdx.x);
-    walk_to(p, now, NR);
-    {
+    if (CL) {
+        const int item = blockIdx.x >> p.cluster_log2, rank = blockIdx.x & ((1 << p.cluster_log2) - 1);
+        long long first_item, first_unit;
+        if (!find_item<kPaThreads>(p, NR, item, &total, &now.s, &first_item, &first_unit)) return;   // (the whole cluster)
+        walk_to(p, now, NR);
+        const long long mine = item - first_item;
+        now.row_tile = (int)quotient(mine, p.kv_heads);
+        now.kvh = (int)(mine - (long long)now.row_tile * p.kv_heads);
+        now.tile = (int)((long long)now.U.tiles * rank >> p.cluster_log2);
+        now.left = ((long long)now.U.tiles * (rank + 1) >> p.cluster_log2) - now.tile;
+    } else {
+        Place at;
+        if (!find_unit<kPaThreads>(p, NR, [&](long long n) { return share_begin(n, gridDim.x, blockIdx.x); }, &total, &at)) return;   // (with barriers: the mbarriers are set up)
+        now.s = at.s;
+        now.left = share_begin(total, gridDim.x, blockIdx.x + 1) - share_begin(total, gridDim.x, blockIdx.x);
+        walk_to(p, now, NR);
         const long long item = quotient(at.off, now.U.tiles);
         now.tile = (int)(at.off - item * now.U.tiles);
         now.row_tile = (int)quotient(item, p.kv_heads);
         now.kvh = (int)(item - (long long)now.row_tile * p.kv_heads);
     }
+    const Walk whose = now;
+    __shared__ float part_m[NR], part_l[NR];         // CL: this CTA's share of the item (part_l below zero: it had none), its sums behind the ring
+    float* part_o = reinterpret_cast<float*>(smem + kPaWarps * kStages * kStage);
+    if (CL && now.left == 0 && tid < NR) { part_m[tid] = -INFINITY; part_l[tid] = -1.0f; }
     // ---- this warp's ring ----
     Walk ahead = now;
     const uint32_t ring = smem_u32(smem) + warp * kStages * kStage;
@@ -604,7 +631,10 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
                 l = fmaf(f, s_l[w][n], l);
                 v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
             }
-            if (all_of_it) {
+            if (CL) {
+                if (d == 0) { part_m[n] = mx; part_l[n] = l; }
+                *reinterpret_cast<float4*>(part_o + n * 64 * HC + d) = v;
+            } else if (all_of_it) {
                 const float r = l == 0.0f ? 0.0f : __fdiv_rn(16777216.0f / kPScale, l);   // (a row that attends to nothing is zero)
                 const int i = div_by(n0 + n, p.by_group), head = kvh * group + (n0 + n) - i * group;
                 store_row4<BF16>(p, U.first + i, head, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
@@ -619,6 +649,39 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
             __syncthreads();
             if (last >= 0) issue();
         }
+    }
+    if (CL) {
+        cluster_sync_all();
+        const int ranks = 1 << p.cluster_log2, rank = blockIdx.x & (ranks - 1), n0 = whose.row_tile * NR;
+        const int nrow = (int)min((long long)NR, (long long)whose.U.rows * group - n0);
+        const uint32_t m_a = smem_u32(part_m), l_a = smem_u32(part_l), o_a = smem_u32(part_o);
+        for (int it = rank * kPaThreads + tid; it < nrow * (hd / 4); it += ranks * kPaThreads) {
+            const int n = div_by(it, p.by_quads), d = (it - n * (hd / 4)) * 4;
+            float m[8], s[8], mx = -INFINITY, l = 0.0f;
+            float4 x[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int from = min(e, ranks - 1);
+                m[e] = ld_dsmem(mapa_shared(m_a + n * 4, from));
+                s[e] = ld_dsmem(mapa_shared(l_a + n * 4, from));
+                x[e] = ld_dsmem4(mapa_shared(o_a + (n * 64 * HC + d) * 4, from));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < ranks) mx = fmaxf(mx, m[e]);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (e >= ranks || s[e] < 0.0f) continue;           // (a NaN of a share is no number below zero)
+                const float f = ex2(m[e] - ref);
+                l = fmaf(f, s[e], l);
+                v.x = fmaf(f, x[e].x, v.x); v.y = fmaf(f, x[e].y, v.y); v.z = fmaf(f, x[e].z, v.z); v.w = fmaf(f, x[e].w, v.w);
+            }
+            const float r = l == 0.0f ? 0.0f : __fdiv_rn(16777216.0f / kPScale, l);
+            const int i = div_by(n0 + n, p.by_group), head = whose.kvh * group + (n0 + n) - i * group;
+            store_row4<BF16>(p, whose.U.first + i, head, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+        }
+        cluster_sync_all();                                        // (nobody leaves while its shared memory is read)
     }
 }
 
@@ -783,9 +846,21 @@ int workers_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
     return (int)(units < most ? (units > 0 ? units : 1) : most);
 }
 
-template <int BF16, int HC, int NT>
+// CTAs of an item (log2) where a cluster each takes the place of shares and join; 0: it does not.  It does where all clusters are on the machine at a time and no CTA has
+// more than one unit above its equal share.  (us by shares and by clusters, heads of 128: 901 positions of 8 KV heads 7.6 and 6.9, four sequences of 900 10.8 and 9.1, 2500
+// positions of 32 KV heads 12.6 and 10.0; two units above: 3000 positions of 8 KV heads 8.7 and 9.3.)
+int cluster_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
+    const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
+    const long long room = ((long long)a.seqs.cols << a.seqs.page_log2), tiles = (room + kUnitKeys - 1) / kUnitKeys, items = items_bound(a, tile_rows);
+    const long long most = (long long)sm_count * ctas_of(hc, tile_rows / 8);
+    for (int c = 3; c > 0; --c)
+        if (items << c <= most && tiles > 1) return (tiles + (1 << c) - 1) >> c <= (items * tiles + most - 1) / most + 1 ? c : 0;
+    return 0;
+}
+
+template <int BF16, int HC, int NT, int CL>
 cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t stream) {
-    auto kern = paged_attend_kernel<BF16, HC, NT>;
+    auto kern = paged_attend_kernel<BF16, HC, NT, CL>;
     TensorMapEncodeFn enc = tensor_map_encoder();
     if (!enc) return cudaErrorNotSupported;
     const int page = 1 << a.seqs.page_log2;
@@ -797,7 +872,7 @@ cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t st
     if (enc(&m.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, (void*)a.codes, dim, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
             HC == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    const size_t smem = 1024 + (size_t)kPaWarps * stages_of(HC) * 4096 * HC;
+    const size_t smem = 1024 + (size_t)kPaWarps * stages_of(HC) * 4096 * HC + (CL ? 8 * NT * 64 * HC * 4 : 0);
     static std::atomic<int> attr_dev{-1};          // the opt-in is per device
     int dev = 0;
     cudaGetDevice(&dev);
@@ -806,7 +881,22 @@ cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t st
         if (e != cudaSuccess) return e;
         attr_dev.store(dev);
     }
-    return launch_pdl(kern, dim3((unsigned)workers), dim3(kPaThreads), smem, stream, m, a);
+    if (!CL) return launch_pdl(kern, dim3((unsigned)workers), dim3(kPaThreads), smem, stream, m, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)workers);
+    cfg.blockDim = dim3(kPaThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1u << a.cluster_log2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, m, a);
 }
 
 }  // namespace
@@ -814,7 +904,7 @@ cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t st
 // Floats of workspace for any batch of these sizes: two partial sums a worker.
 size_t paged_attend_ws_floats(const PagedAttendArgs& a, int sm_count) {
     const int tr = tile_rows_of(a.heads / a.kv_heads, a.max_rows), w = workers_of(a, tr, sm_count);
-    return w > 1 ? 2 * (size_t)w * part_floats(tr, a.head_dim) : 0;
+    return w > 1 && !cluster_of(a, tr, sm_count) ? 2 * (size_t)w * part_floats(tr, a.head_dim) : 0;
 }
 
 cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaStream_t stream) {
@@ -823,10 +913,12 @@ cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaS
     a.by_group = fast_div((uint32_t)(a.heads / a.kv_heads));
     a.by_quads = fast_div((uint32_t)(a.head_dim / 4));
     a.out_vec = a.out_stride % 4 == 0 && ((uintptr_t)a.out & 7) == 0;
-    const int tr = tile_rows_of(a.heads / a.kv_heads, a.max_rows), workers = workers_of(a, tr, sm_count);
+    const int tr = tile_rows_of(a.heads / a.kv_heads, a.max_rows);
+    a.cluster_log2 = cluster_of(a, tr, sm_count);
+    const int workers = a.cluster_log2 ? (int)(items_bound(a, tr) << a.cluster_log2) : workers_of(a, tr, sm_count);
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
     cudaError_t e;
-#define SMEG_PA(B, H, N) attend_launch<B, H, N>(a, workers, stream)
+#define SMEG_PA(B, H, N) (a.cluster_log2 ? attend_launch<B, H, N, 1>(a, workers, stream) : attend_launch<B, H, N, 0>(a, workers, stream))
     if (bf16) {
         if (tr == 8) e = hc == 1 ? SMEG_PA(1, 1, 1) : (hc == 2 ? SMEG_PA(1, 2, 1) : SMEG_PA(1, 4, 1));
         else e = hc == 1 ? SMEG_PA(1, 1, 2) : (hc == 2 ? SMEG_PA(1, 2, 2) : SMEG_PA(1, 4, 2));
@@ -835,7 +927,7 @@ cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaS
         else e = hc == 1 ? SMEG_PA(0, 1, 2) : (hc == 2 ? SMEG_PA(0, 2, 2) : SMEG_PA(0, 4, 2));
     }
 #undef SMEG_PA
-    if (e != cudaSuccess || workers == 1) return e;
+    if (e != cudaSuccess || workers == 1 || a.cluster_log2) return e;
     const long long items = items_bound(a, tr);
     if (items >= workers)
         return bf16 ? launch_pdl(paged_join_cuts_kernel<1>, dim3((unsigned)workers - 1), dim3(kPaThreads), 0, stream, a, workers, tr)

@@ -830,3 +830,18 @@ def test_a_norm_without_an_eps(kv, rows):
     pool.append(rows, (), sg.Rotary(64), norm)
     pool.append([1, 1, 1], (), sg.Rotary(64), norm)
     pool.check(times=2)
+
+
+@pytest.mark.parametrize("heads,kv,hd,page,lens,rows,dtype", [
+    (32, 8, 128, 64, [9000], [1], F16), (32, 8, 128, 64, [200 + 29 * i for i in range(50)], [1] * 50, BF16), (24, 3, 64, 16, [3000, 2500, 10], [5, 5, 5], F16),
+    (6, 6, 64, 32, [7000, 1], [1, 1], F16), (16, 2, 256, 64, [6000, 4000], [2, 1], BF16), (4, 4, 80, 128, [40 * i + 1 for i in range(60)], [1] * 60, F16)])
+def test_long_contexts_and_many_sequences(heads, kv, hd, page, lens, rows, dtype):
+    """Keys shared out evenly over the machine, the cut items joined afterwards: item by item and cut by cut."""
+    pool = Pool(heads, kv, hd, page, len(lens), -(-max(lens) // page) + 1, seed=len(lens) + hd, dtype=dtype)
+    pool.append(lens)
+    starts = [n - r for n, r in zip(lens, rows)]
+    q = _randn(pool.gen, sum(rows), heads * hd, dtype=dtype)
+    out = torch.full_like(q, 5.0)
+    pool.cache.attend(q, pool.batch(rows, starts=starts), out)
+    want, tol = _attended(pool, q, rows, starts)
+    _near(out, want, tol, dtype)
