@@ -835,6 +835,12 @@ int tile_rows_of(int group, int max_rows) {
 long long items_bound(const PagedAttendArgs& a, int tile_rows) {
     return ((long long)a.seqs.rows * (a.heads / a.kv_heads) / tile_rows + a.seqs.seqs) * a.kv_heads;
 }
+// The same, tight for sequences of a row each: r rows have ceil(r * group / tile_rows) tiles and never more than r * ceil(group / tile_rows).  (Which join is taken was measured
+// over the looser one.)
+long long items_most(const PagedAttendArgs& a, int tile_rows) {
+    const long long by_row = (long long)(a.heads / a.kv_heads + tile_rows - 1) / tile_rows * a.seqs.rows * a.kv_heads, bound = items_bound(a, tile_rows);
+    return by_row < bound ? by_row : bound;
+}
 
 // CTAs: as many as the GPU holds at a time (the occupancy of the variant), no more than there can be units.
 int workers_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
@@ -847,14 +853,19 @@ int workers_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
 }
 
 // CTAs of an item (log2) where a cluster each takes the place of shares and join; 0: it does not.  It does where all clusters are on the machine at a time and no CTA has
-// more than one unit above its equal share.  (us by shares and by clusters, heads of 128: 901 positions of 8 KV heads 7.6 and 6.9, four sequences of 900 10.8 and 9.1, 2500
-// positions of 32 KV heads 12.6 and 10.0; two units above: 3000 positions of 8 KV heads 8.7 and 9.3.)
+// more than three units, which is little beside the join whatever the lengths are, nor more than one above its equal share.  (us by shares and by clusters, heads of 128: 901
+// positions of 8 KV heads 7.6 and 6.9, four sequences of 1800 12.1 and 9.3, sixteen of 500 12.3 and 9.7, 2500 positions of 32 KV heads 12.6 and 10.0; two above: 3000 positions
+// of 8 KV heads 8.7 and 9.3; seven units: 12 x 5 rows of 800 to 3200 positions, heads of 64, 18.7 and 22.4.)
 int cluster_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
-    const long long room = ((long long)a.seqs.cols << a.seqs.page_log2), tiles = (room + kUnitKeys - 1) / kUnitKeys, items = items_bound(a, tile_rows);
+    const long long room = ((long long)a.seqs.cols << a.seqs.page_log2), tiles = (room + kUnitKeys - 1) / kUnitKeys, items = items_most(a, tile_rows);
     const long long most = (long long)sm_count * ctas_of(hc, tile_rows / 8);
+    if (tiles <= 1) return 0;
     for (int c = 3; c > 0; --c)
-        if (items << c <= most && tiles > 1) return (tiles + (1 << c) - 1) >> c <= (items * tiles + most - 1) / most + 1 ? c : 0;
+        if (items << c <= most) {
+            const long long units = (tiles + (1 << c) - 1) >> c;
+            return units <= 3 && units <= (items * tiles + most - 1) / most + 1 ? c : 0;
+        }
     return 0;
 }
 
@@ -915,7 +926,7 @@ cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaS
     a.out_vec = a.out_stride % 4 == 0 && ((uintptr_t)a.out & 7) == 0;
     const int tr = tile_rows_of(a.heads / a.kv_heads, a.max_rows);
     a.cluster_log2 = cluster_of(a, tr, sm_count);
-    const int workers = a.cluster_log2 ? (int)(items_bound(a, tr) << a.cluster_log2) : workers_of(a, tr, sm_count);
+    const int workers = a.cluster_log2 ? (int)(items_most(a, tr) << a.cluster_log2) : workers_of(a, tr, sm_count);
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
     cudaError_t e;
 #define SMEG_PA(B, H, N) (a.cluster_log2 ? attend_launch<B, H, N, 1>(a, workers, stream) : attend_launch<B, H, N, 0>(a, workers, stream))
