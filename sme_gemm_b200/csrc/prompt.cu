@@ -319,6 +319,14 @@ __device__ __forceinline__ void tma_4d(void* dst, const CUtensorMap* map, int x,
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
 }
+// From shared memory; the thread that issues it commits and waits.
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, int x, int y, int z, int w, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];\n\tcp.async.bulk.commit_group;"
+                 ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(src) : "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -347,7 +355,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 
 struct PromptTc {
-    CUtensorMap q, k, v;
+    CUtensorMap q, k, v, out;
     PromptArgs p;
     int tokens;                                    // of a query tile: 128 / heads of a group
     int slots;                                     // K / V ring
@@ -376,7 +384,8 @@ __device__ __forceinline__ int taken_cta(uint32_t answer) {        // its index,
     return ok ? (int)x : -1;
 }
 
-template <int BF16, int NCH>
+// BULK: a softmax warp's 32 rows are whole tokens, out lies on 16-byte boundaries, and full warps' results leave by bulk stores from the warp's stage.
+template <int BF16, int NCH, int BULK>
 __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptTc a) {
     constexpr int kTile = NCH * kPtChunk, kTiles = NCH <= 2 ? 2 : 1;
     const PromptArgs& p = a.p;
@@ -703,7 +712,36 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             const unsigned rows_in = __ballot_sync(0xffffffffu, in);
             const uint32_t mine = smem_u32(out_s) + warp * kPtStage;
             uint64_t zero = 0;                                     // 0 * every result: not a number where one of them is not finite
-            for (int c0 = 0; c0 < hd; c0 += 64) {
+            const bool bulk = BULK && rows_in == 0xffffffffu;
+            if (bulk) {
+                const int tok_w = w.first + low + (warp & 3) * 32 / group;
+                for (int c0 = 0; c0 < hd; c0 += 64) {
+                    uint32_t o[2][32], e[32];
+                    tmem_ld32(to + c0, o[0]);
+                    tmem_ld32(to + c0 + 32, o[1]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const uint64_t y = mul2(pack64(__uint_as_float(o[i / 16][2 * (i % 16)]), __uint_as_float(o[i / 16][2 * (i % 16) + 1])), inv2);
+                        if (c0 + 2 * i < hd) zero = fma2(y, 0, zero);
+                        float u, v;
+                        unpack64(y, u, v);
+                        e[i] = pack2_t<BF16>(u, v);
+                    }
+                    if (lane == 0) bulk_wait_read<0>();            // (the last store has read the stage)
+                    __syncwarp();
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(mine + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(e[4 * c]), "r"(e[4 * c + 1]), "r"(e[4 * c + 2]), "r"(e[4 * c + 3]) : "memory");
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) tma_store_4d(&a.out, c0, 0, w.kvh, tok_w, mine);
+                }
+            } else if (BULK && lane == 0) {
+                bulk_wait_read<0>();
+            }
+            if (BULK) __syncwarp();
+            for (int c0 = bulk ? hd : 0; c0 < hd; c0 += 64) {
                 uint32_t o[2][32];
                 tmem_ld32(to + c0, o[0]);                          // (what lies behind the head's depths is not used)
                 tmem_ld32(to + c0 + 32, o[1]);
@@ -746,11 +784,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             const bool bad = !(z0 + z1 == 0.0f);
             unsigned mask = __ballot_sync(0xffffffffu, in && bad && l > 0.0f);
             if (mask && spoilt_by_later(p, w.kvh, w.first, w.first + low, min(w.first + n * kPtKeys, p.rows)))
-                for (; mask; mask &= mask - 1) {
+                for (BULK ? bulk_wait_all() : void(); mask; mask &= mask - 1) {    // (behind what has been stored there)
                     const int r = __ffs(mask) - 1, tk = __shfl_sync(0xffffffffu, tok, r), h = __shfl_sync(0xffffffffu, head, r);
                     __syncwarp();
                     exact_row<BF16>(p, w.first, w.first + tk, h);
                 }
+        }
+        if (BULK) {
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
         }
         tc_fence_before();
     }
@@ -761,7 +803,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     }
 }
 
-template <int BF16, int NCH>
+template <int BF16, int NCH, int BULK>
 cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
     constexpr int kTiles = NCH <= 2 ? 2 : 1;
     *taken = false;
@@ -789,7 +831,15 @@ cudaError_t tc_launch(const PromptArgs& p, cudaStream_t stream, bool* taken) {
         enc(&a.v, type, 3, (void*)p.v, kd, vs, kb, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaSuccess;
-    auto kern = prompt_tc_kernel<BF16, NCH>;
+    // (us without and with bulk stores, heads of 128: eleven prompts of 7001 rows 83 and 78, four of 1024 47 and 44; nine of 300 rows of 256 31 and 26.  Heads of 64, one chunk
+    // a row: 60 prompts of 100 rows 18.9 and 20.5.)
+    if (BULK) {
+        const cuuint64_t os[3] = {hd * 2, hd * 2 * group, (cuuint64_t)p.out_stride * 2};
+        const cuuint32_t ob[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)(32 / group)};
+        if (enc(&a.out, type, 4, (void*)p.out, qd, os, ob, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return cudaSuccess;
+    }
+    auto kern = prompt_tc_kernel<BF16, NCH, BULK>;
     const size_t smem = 1024 + (size_t)(kTiles + a.slots) * NCH * kPtChunk + kTiles * 4 * kPtStage;
     static std::atomic<int> attr_dev{-1};          // the opt-in is per device
     int dev = 0;
@@ -832,8 +882,12 @@ cudaError_t prompt_launch(PromptArgs a, int sm_count, cudaStream_t stream) {
     if (aligned && a.scale_log2e > 0.0f && a.scale_log2e < 1e30f) {
         bool taken = false;
         typedef cudaError_t (*Launch)(const PromptArgs&, cudaStream_t, bool*);
-        static const Launch launches[2][4] = {{tc_launch<0, 1>, tc_launch<0, 2>, tc_launch<0, 3>, tc_launch<0, 4>}, {tc_launch<1, 1>, tc_launch<1, 2>, tc_launch<1, 3>, tc_launch<1, 4>}};
-        const cudaError_t e = launches[a.bf16 ? 1 : 0][(a.head_dim + 63) / 64 - 1](a, stream, &taken);
+        static const Launch launches[2][2][4] = {{{tc_launch<0, 1, 0>, tc_launch<0, 2, 0>, tc_launch<0, 3, 0>, tc_launch<0, 4, 0>},
+                                                  {tc_launch<1, 1, 0>, tc_launch<1, 2, 0>, tc_launch<1, 3, 0>, tc_launch<1, 4, 0>}},
+                                                 {{tc_launch<0, 1, 0>, tc_launch<0, 2, 1>, tc_launch<0, 3, 1>, tc_launch<0, 4, 1>},
+                                                  {tc_launch<1, 1, 0>, tc_launch<1, 2, 1>, tc_launch<1, 3, 1>, tc_launch<1, 4, 1>}}};
+        const bool bulk = 32 % (a.heads / a.kv_heads) == 0 && (((uintptr_t)a.out | (a.out_stride * 2)) & 15) == 0 && a.out_stride >> 38 == 0;
+        const cudaError_t e = launches[bulk][a.bf16 ? 1 : 0][(a.head_dim + 63) / 64 - 1](a, stream, &taken);
         if (taken || e != cudaSuccess) return e;
     }
     if (a.bf16) return a.head_dim <= 64 ? mma_launch<1, 64>(a, stream) : (a.head_dim <= 128 ? mma_launch<1, 128>(a, stream) : mma_launch<1, 256>(a, stream));
