@@ -606,9 +606,10 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     a.lanes_magic = (65536 + a.lanes - 1) / a.lanes;               // tid * magic >> 16 = tid / lanes
     const int row_pass = kRotThreads / a.lanes;
     a.inv_hd = 1.0f / (float)a.head_dim;
-    // row units: all heads of a few rows, so that they share the rows' cosines -- four rows for each that the block's threads have at a time; of one row, as many
-    // heads as the block has at a time, while the machine has room for more CTAs.  (us with four and with eight rows: 5000 rows of 6 heads of 64, which
-    // are eight at a time, 6.8 and 5.4; 8192 rows of 28 / 4 heads of 96, four at a time, 22.8 and 24.2)
+    // row units: all heads of a few rows, so that they share the rows' cosines: two, or four where there are CTAs enough, for each row that the block's threads have at a time;
+    // of one row, as many heads as the block has at a time, while the machine has room for more CTAs.  (us with tiles of two, four and eight rows: 2001 rows of 28 / 4 heads of 96
+    // 7.2, 8.5, 11.9, of 32 / 8 heads of 128 10.9, 12.9, 19.6; 8192 rows 36.9, 36.3, 37.5; 2001 rows of 6 heads of 64, of which there are two rows at a time, 3.8, 3.5, 4.4, 5000 rows
+    // 7.7, 6.3, 5.8)
     const int qh = a.q ? a.heads : 0, kh = a.k && !paged ? a.kv_heads : 0, most = qh > kh ? qh : kh;
     a.head_tile = (size_t)a.rows >= (size_t)sm_count * 4 ? most : row_pass;
     if (a.head_tile > most) a.head_tile = most;
@@ -618,7 +619,8 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     a.row_heads = a.head_tile < row_pass ? a.head_tile : row_pass;
     if (a.row_heads < 1) a.row_heads = 1;
     a.row_rows = row_pass / a.row_heads;
-    a.row_tile = (size_t)a.rows < (size_t)sm_count * 8 ? 1 : (4 * a.row_rows < kRowTile ? 4 * a.row_rows : kRowTile);
+    const int tile = ((size_t)a.rows < (size_t)sm_count * 32 ? 2 : 4) * a.row_rows;
+    a.row_tile = (size_t)a.rows < (size_t)sm_count * 8 ? 1 : (tile < kRowTile ? tile : kRowTile);
     a.row_magic = (65536 + a.row_heads - 1) / a.row_heads;         // mine * magic >> 16 = mine / row_heads for mine below 256
     const long long row_units = (long long)((a.rows + a.row_tile - 1) / a.row_tile) * a.head_tiles;
     long long page_units = 0;
