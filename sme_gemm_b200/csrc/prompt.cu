@@ -5,10 +5,10 @@
 // product.  The query rows of one KV head -- every row times every head of the group -- are the rows of a tile, so that grouped heads share one
 // read of the keys and values.
 //
-// Bound by the tensor cores where prompts are long: 8192 rows, 32 / 8 heads of 128, 455 us in single runs (1210 TFLOP/s of causal work), 485 and more when they run back to
-// back (the power cap; a long cuBLAS product holds 1409), 4096 rows of 16 / 2 heads of 256 111 us (1240).  Short prompts are bound by what an item of 64 rows has at its ends:
-// the first scores, the last product, and results on their way out (about 2.5 us) with no products beside them.  Eleven prompts of 7001 rows in all: 75 us.
-// Heads of 64 do a product in half the time and the same exponentials, so there these bound it: 347 us.
+// Bound by the tensor cores where prompts are long: 8192 rows, 32 / 8 heads of 128, 480 to 500 us back to back, under the power cap (1100 to 1150 TFLOP/s of causal work; a
+// long cuBLAS product holds 1409), 4096 rows of 16 / 2 heads of 256 116 us (1180).  Heads of 64 do a product in half the time and the same exponentials, which bound them
+// there: 350 us.  Short prompts are bound by an item's ends -- first scores, last product, results on their way out -- and the masked halves of last blocks: eleven
+// prompts of 7001 rows, 32 / 8 heads of 128, 73 to 77 us, 15 of which the results' way out took before it was a bulk store.
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
@@ -367,7 +367,8 @@ struct PromptItem {
 };
 
 // The grid has a CTA for every work slot, and a CTA that has finished its own takes over the next one that has not been launched: the barriers and the
-// tensor memory are set up once, and the next item's queries and keys are on their way while this one's last blocks are weighed and its results stored.
+// tensor memory are set up once, and the next item's queries and keys are on their way while this one's last blocks are weighed and its results stored.  (A CTA for every
+// item alone: 8192 rows 508 us against 459, eleven prompts of 7001 98 against 84.)
 __device__ __forceinline__ void take_next_cta(uint32_t answer, uint64_t* bar) {
     asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(smem_u32(bar)) : "memory");
 }
@@ -791,7 +792,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 }
         }
         if (BULK) {
-            if (lane == 0) bulk_wait_read<0>();
+            if (lane == 0) bulk_wait_all();                        // (stored, not only read: the grid that waits for this one finds the results)
             __syncwarp();
         }
         tc_fence_before();

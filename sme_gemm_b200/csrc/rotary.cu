@@ -14,10 +14,10 @@
 // heads, so there they are formed for its first row alone, and row r takes the sum formulas with the cosines and sines of r frequencies, which the
 // caller's table holds.
 //
-// Bytes bound it from some thousand rows on (each 16-bit value is read and written once, a cached one is read once and leaves as a byte), the instructions next to them:
-// 8192 rows of 32 + 8 normalised heads of 128 take 36 us (4.7 TB/s of 6.5 measured), without norms, 28 + 4 heads of 96, 22.4 (4.5); 4096 rows of five
-// prompts with their pages 32 us, 16 of them the queries', where the issue slots are 58 % busy.  Short calls are a chain of dependent loads -- row offsets, page number,
-// rows, scale -- and a launch: one row 2.0 us, 48 single rows into their pages 4.5.
+// Bytes bound it from some thousand rows on (each 16-bit value is read and written once, a cached one is read once and leaves as a byte), the instructions next to
+// them: 8192 rows of 32 + 8 normalised heads of 128 take 36 us (4.6 TB/s of 6.5 measured), without norms, 28 + 4 heads of 96, 23 (4.4), 2001 of those 7.2 (3.4);
+// 4096 rows of five prompts with their pages 31 us, 15 of them the pages', with issue slots 54 % busy at the 20 warps an SM that 96 registers allow.  Short calls are a
+// chain of dependent loads -- row offsets, page number, rows, scale -- and a launch: one row 2.1 us, append and read of 48 single rows 6.5.
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
@@ -538,8 +538,10 @@ __global__ void __launch_bounds__(kRotThreads, 8) rotate_rows_kernel(const __gri
     pdl_wait();
     row_unit<BF16, LAY>(p, head_lay(p), trig_s, blockIdx.x);
 }
-template <int BF16, int LAY>
-__global__ void __launch_bounds__(kRotThreads, 5) rotate_append_kernel(const __grid_constant__ RotateArgs p) {
+// CTAS: of an SM.  Five where there are that many (4096 rows of prompts, us with four, five, six and seven: 41.1, 38.2, 38.4, 39.2), four, which spill nothing, for the grids of a
+// step (48 single rows with four and five: 6.45 and 6.66; 37 rows: 5.63 and 5.84).
+template <int BF16, int LAY, int CTAS>
+__global__ void __launch_bounds__(kRotThreads, CTAS) rotate_append_kernel(const __grid_constant__ RotateArgs p) {
     extern __shared__ __align__(16) float trig_s[];
     const HeadLay L = head_lay(p);
     pdl_wait();
@@ -589,6 +591,16 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(uint16_t* __re
             for (int e = 0; e < 8; ++e) y[off + e] = (uint16_t)(o[e / 2] >> (16 * (e & 1)));
         }
     }
+}
+
+typedef void (*RotKernel)(RotateArgs);
+template <int BF16, int LAY>
+RotKernel rot_kernel_of(int kind) {                                // 0: rows alone; else the CTAs of an SM with pages
+    return kind == 0 ? rotate_rows_kernel<BF16, LAY> : (kind == 4 ? rotate_append_kernel<BF16, LAY, 4> : rotate_append_kernel<BF16, LAY, 5>);
+}
+template <int BF16>
+RotKernel rot_kernel(int lay, int kind) {
+    return lay == kHalves ? rot_kernel_of<BF16, kHalves>(kind) : (lay == kNeighbours ? rot_kernel_of<BF16, kNeighbours>(kind) : (lay == kMixed ? rot_kernel_of<BF16, kMixed>(kind) : rot_kernel_of<BF16, kAny>(kind)));
 }
 
 }  // namespace
@@ -645,11 +657,8 @@ cudaError_t rotate_append_launch(RotateArgs a, int bf16, int sm_count, cudaStrea
     const size_t rows_smem = a.turns ? (size_t)a.row_tile * a.head_dim * sizeof(float) : 0;
     const size_t page_smem = paged ? a.head_dim * sizeof(float) + (size_t)kHeld * 8 * kRotThreads * sizeof(float) : 0;
     const size_t smem = rows_smem > page_smem ? rows_smem : page_smem;
-    typedef void (*Kern)(RotateArgs);
-#define SMEG_ROT(K) {{K<0, 0>, K<0, 1>, K<0, 2>, K<0, 3>}, {K<1, 0>, K<1, 1>, K<1, 2>, K<1, 3>}}
-    static const Kern kerns[2][2][4] = {SMEG_ROT(rotate_rows_kernel), SMEG_ROT(rotate_append_kernel)};
-#undef SMEG_ROT
-    const Kern kern = kerns[paged ? 1 : 0][bf16 ? 1 : 0][lay];
+    const int kind = !paged ? 0 : (row_units + page_units <= 4ll * sm_count ? 4 : 5);
+    const RotKernel kern = bf16 ? rot_kernel<1>(lay, kind) : rot_kernel<0>(lay, kind);
     return launch_pdl(kern, dim3((unsigned)(row_units + page_units)), dim3(kRotThreads), smem, stream, a);
 }
 
