@@ -20,9 +20,9 @@
 // probabilities are f16 at 2^7, a group's scaled by its page's scale over the larger of the warp's two; the reference of a row's exponentials follows
 // its maximum when that is 2^8 above it; each 32 keys' sums are folded into 32-bit registers, since the tensor core cuts its sums off.
 //
-// Measured: a long context streams at 6.8 TB/s beside 12 to 15 us that do not depend on its length (two launches, the first bytes, the warps' meeting, the join): one token
-// over 131071 positions of 8 KV heads of 128 51.4 us (5.2 TB/s), 64 sequences of 500 to 5000 positions 78 us (4.9 TB/s).  With several rows of eight query heads each it is
-// bound by the unpacking and the exponentials (64 x 5 rows of 3000 positions, 24 / 3 heads of 64: 79 us).
+// Measured: a long context streams at 6.8 TB/s beside 12 to 15 us that do not depend on its length (launches, the first bytes, the warps' meeting, the join): one token over
+// 131071 positions of 8 KV heads of 128 51.4 us (5.2 TB/s), 64 sequences of 500 to 5000 positions 78 us (4.9 TB/s); 901 positions by clusters 6.9 us.  With several rows of
+// eight query heads each it is bound by the unpacking and the exponentials (64 x 5 rows of 3000 positions, 24 / 3 heads of 64: 79 us).
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
