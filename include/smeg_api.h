@@ -351,7 +351,8 @@ size_t smeg_paged_attend_workspace(size_t rows, size_t seqs, size_t table_cols, 
 int smeg_paged_attend_dev(const smeg_paged_attend_args *a, void *stream);
 
 /* Causal attention over whole packed prompts, 16-bit keys and values: row i of a sequence attends to the sequence's rows 0..=i.  head_dim a
- * multiple of 8 in 8..=256; any strides and starts, the tensor-core form for rows that start on 16-byte boundaries. */
+ * multiple of 8 in 8..=256; any strides and starts, the tcgen05 form for rows that start on 16-byte boundaries.  out shares no memory with the
+ * inputs (here and in smeg_paged_attend_dev). */
 typedef struct smeg_attn_packed_args {
     const uint16_t *q, *k, *v;
     uint16_t *out;
