@@ -693,6 +693,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                     if (c & 1) {
                         tmem_st_wait();
                         tc_fence_before();
+                        // One tile: every phase of o_done in its turn, the last one while the next cannot be over without this warp.  (These scores were formed before the product
+                        // before: without the wait a warp that is ahead of the others could take the parity of an earlier phase for that of its last one, and a result
+                        // leave before its products are done.)
+                        if (kTiles == 1 && c == 3 && done > 0) ok = __all_sync(0xffffffffu, mbar_wait_poll(&o_done[0], (done - 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));
                         __syncwarp();
                         if (lane == 0) mbar_arrive(c == 1 ? &p_half[buf] : &p_full[buf]);
                     }
@@ -700,6 +704,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 float u, v;
                 unpack64(add2(sum[0], sum[1]), u, v);
                 l += u + v;
+                if (kTiles == 1 && !ok) break;
             }
             if (!ok || n == 0) continue;
             ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], (kTiles == 2 ? tiles : done - 1) & 1, abort_flag, p.status, STATUS_TMEM_TIMEOUT));

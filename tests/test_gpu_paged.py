@@ -845,3 +845,26 @@ def test_long_contexts_and_many_sequences(heads, kv, hd, page, lens, rows, dtype
     pool.cache.attend(q, pool.batch(rows, starts=starts), out)
     want, tol = _attended(pool, q, rows, starts)
     _near(out, want, tol, dtype)
+
+
+@pytest.mark.parametrize("heads,kv,hd,dtype", [(16, 2, 256, F16), (12, 4, 192, BF16), (16, 2, 128, F16), (8, 8, 64, BF16)])
+def test_prompts_whose_warps_run_apart(heads, kv, hd, dtype):
+    """Sequences that end inside tiles and scores whose maxima move: a warp may be a block ahead of the others, and its results wait for all products all the same.  Every
+    run gives the same bits."""
+    gen = _gen(hd)
+    rows = [289, 245, 272, 261, 250, 277, 266, 255, 283, 244, 271, 260, 303]
+    total = sum(rows)
+    cu = _int([0] + np.cumsum(rows).tolist())
+    first = None
+    for run in range(12):
+        if run % 4 == 0:
+            q, k, v = _randn(gen, total, heads * hd, dtype=dtype, scale=1.5), _randn(gen, total, kv * hd, dtype=dtype), _randn(gen, total, kv * hd, dtype=dtype)
+            k += torch.linspace(0, 1, total, device="cuda").to(dtype)[:, None] * k          # later keys are larger: maxima move along
+            want, tol = _prompt(q, k, v, rows, heads, kv)
+            first = None
+        out = torch.full_like(q, 7.0)
+        sg.attend_packed(q, k, v, cu, out, heads, kv)
+        if first is None:
+            first = out
+            _near(out, want, tol, dtype)
+        assert torch.equal(out, first)
