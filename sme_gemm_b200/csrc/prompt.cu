@@ -31,88 +31,8 @@ __device__ __forceinline__ float ex2(float x) {
 
 // ---- rows formed again ----
 // A key block's second product multiplies every value of the block by every row's probability, also by the zeros of rows that do not attend to it: an
-// infinity or NaN there makes NaNs (0 * inf).  So a row whose result is not finite although its probabilities are is formed again, key by key over
-// what it attends to, where the blocks that it shares with later rows hold such a value.
-
-// Whether rows that attend to keys [first, low] and not to all of (low, to) may have to be: a value of (low, to) is an infinity or NaN at a depth that is not
-// lost to them anyway.  (A depth at which they attend to a NaN, or to infinities of both signs, is; the 64 keys up to low tell where values are lost altogether, and
-// rows of thousands of keys need not be formed again one by one.)  A warp; a lane has eight depths.
-__device__ __noinline__ bool spoilt_by_later(const PromptArgs& p, int kvh, int first, int low, int to) {
-    const unsigned expo = p.bf16 ? 0x7f80u : 0x7c00u;
-    const int d0 = (threadIdx.x & 31) * 8;
-    unsigned later = 0, nan = 0, up = 0, down = 0;                 // a bit a depth
-    if (d0 < p.head_dim) {
-        const uint16_t* v = p.v + (size_t)kvh * p.head_dim + d0;
-        for (int j = low + 1; j < to; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) later |= (unsigned)((v[(size_t)j * p.v_stride + e] & expo) == expo) << e;
-        if (later)
-            for (int j = low; j >= max(first, low - 63); --j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const unsigned x = v[(size_t)j * p.v_stride + e];
-                    nan |= (unsigned)((x & 0x7fffu) > expo) << e;
-                    up |= (unsigned)(x == expo) << e;
-                    down |= (unsigned)(x == (expo | 0x8000u)) << e;
-                }
-    }
-    return __any_sync(0xffffffffu, (later & ~(nan | (up & down))) != 0);
-}
-// Row `row` (of the packed batch) of query head `head` over keys [first, row].  A warp; a lane has eight depths, and four keys are on their way at a time.
-template <int BF16>
-__device__ __noinline__ void exact_row(const PromptArgs& p, int first, int row, int head) {
-    constexpr int kAhead = 4;
-    const int lane = threadIdx.x & 31, d = lane * 8, hd = p.head_dim, kvh = head / (p.heads / p.kv_heads);
-    const bool in = d < hd;
-    float q[8], acc[8], m = -kInf, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        q[e] = in ? t_to_f32<BF16>(p.q[(size_t)row * p.q_stride + (size_t)head * hd + d + e]) : 0.0f;
-        acc[e] = 0.0f;
-    }
-    for (int j0 = first; j0 <= row; j0 += kAhead) {
-        float s[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const uint16_t* k = p.k + (size_t)min(j0 + i, row) * p.k_stride + (size_t)kvh * hd + d;
-            s[i] = 0.0f;
-            if (in)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[i] = fmaf(q[e], t_to_f32<BF16>(k[e]), s[i]);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1)
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
-        float now = m;
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            s[i] *= p.scale_log2e;
-            now = fmaxf(now, s[i]);                                // (the last key again, where there are no four)
-        }
-        const float ref = now == -kInf ? 0.0f : now, a = ex2(m - ref);
-        m = now;
-        l *= a;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] *= a;
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (j0 + i > row) break;
-            const float w = ex2(s[i] - ref);
-            l += w;
-            const uint16_t* v = p.v + (size_t)(j0 + i) * p.v_stride + (size_t)kvh * hd + d;
-            if (in)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, t_to_f32<BF16>(v[e]), acc[e]);
-        }
-    }
-    if (in)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p.out[(size_t)row * p.out_stride + (size_t)head * hd + d + e] = f32_to_t<BF16>(__fdiv_rn(acc[e], l));
-}
-
-// ---- any strides, heads of up to 256 depths: warp-level MMAs ----
-constexpr int kPwThreads = 128, kPwRows = 64, kPwKeys = 64;
+// infinity or NaN there makes NaNs (0 * inf).  So rows whose results are not finite although their probabilities are get them from what they attend to alone, where the
+// blocks that they share with later rows hold such a value.
 
 template <int BF16>
 __device__ __forceinline__ void mma_t(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -125,12 +45,6 @@ __device__ __forceinline__ void mma_t(float (&c)[4], const uint32_t (&a)[4], uin
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
 // Eight 16-bit values of a row, from any address, zeros where there are none.
 __device__ __forceinline__ uint4 load8(const uint16_t* x, bool in, bool vec) {
     if (!in) return make_uint4(0, 0, 0, 0);
@@ -141,6 +55,235 @@ __device__ __forceinline__ uint4 load8(const uint16_t* x, bool in, bool vec) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Rows n0 .. n0 + nrow (at most 16 of a sequence's rows x heads of the group) of KV head kvh: those whose bit is set in `which` are formed and written.  A warp.  Keys that
+// all rows attend to go through the tensor cores, 32 at a time and PANEL depths a pass; the last few, which only some do, are added value by value, so that nothing is
+// multiplied by a zero that stands for "not attended".  (Whole keys are loaded as runs of eight depths: as the depths of a product may come in any order, lane t's
+// run of a 32-depth piece is its share of two products, and lane g's run of 64 depths a column of eight.)
+// (PANEL: 64 or 128 depths a pass.  VEC: rows on 16-byte boundaries.)  One infinity in the last rows of 8192, 32 / 8 heads of 128: 2.9 ms for 0.42, twice 256 steps of 32 keys;
+// infinities at one in a hundred of the values' rows 4.4 ms; a key at a time for each row 16 ms at 1024 rows, where these are 0.31.
+template <int BF16, int VEC, int PANEL>
+__device__ __forceinline__ void form_again(const PromptArgs& p, int first, int kvh, long long n0, int nrow, unsigned which, int vec) {
+    const bool vec_q = VEC || (vec & 1), vec_kv = VEC || (vec >> 1);
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, hd = p.head_dim, group = p.heads / p.kv_heads;
+    const int low = (int)(n0 / group), keys = (int)((n0 + nrow - 1) / group) + 1;                 // keys that every row attends to: low + 1
+    const uint16_t *q[2], *k0 = p.k + (size_t)first * p.k_stride + (size_t)kvh * hd, *v0 = p.v + (size_t)first * p.v_stride + (size_t)kvh * hd;
+    int tok[2];
+    size_t out_at[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const long long n = n0 + min(g + 8 * e, nrow - 1);
+        tok[e] = (int)(n / group);
+        const size_t head = (size_t)kvh * group + (size_t)(n - (long long)tok[e] * group);
+        q[e] = p.q + (size_t)(first + tok[e]) * p.q_stride + head * hd;
+        out_at[e] = (size_t)(first + tok[e]) * p.out_stride + head * hd;
+    }
+    for (int d0 = 0; d0 < hd; d0 += PANEL) {
+        float o[PANEL / 8][4], m[2] = {-kInf, -kInf}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int n = 0; n < PANEL / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
+        for (int key0 = 0; key0 < keys; key0 += 32) {
+            float s[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+            for (int c = 0; c < hd; c += 32) {
+                const int d = c + 8 * t;
+                const uint4 x = load8(q[0] + d, d < hd, vec_q), y = load8(q[1] + d, d < hd, vec_q);
+                const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint4 b = load8(k0 + (size_t)min(key0 + 8 * n + g, keys - 1) * p.k_stride + d, d < hd, vec_kv);
+                    mma_t<BF16>(s[n], a0, b.x, b.y);
+                    mma_t<BF16>(s[n], a1, b.z, b.w);
+                }
+            }
+            float mx[2] = {m[0], m[1]};
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] = key0 + 8 * n + 2 * t + (e & 1) <= tok[e >> 1] ? s[n][e] * p.scale_log2e : -kInf;
+                    mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+                const float ref = mx[e] == -kInf ? 0.0f : mx[e], alpha = ex2(m[e] - ref);
+                m[e] = mx[e];
+                mx[e] = ref;
+                l[e] *= alpha;
+#pragma unroll
+                for (int n = 0; n < PANEL / 8; ++n) {
+                    o[n][2 * e] *= alpha;
+                    o[n][2 * e + 1] *= alpha;
+                }
+            }
+            bool lost = false;                                         // a weight that f16 has no number for
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] = ex2(s[n][e] - mx[e >> 1]);
+                    l[e >> 1] += s[n][e];
+                    lost = lost || (s[n][e] > 0.0f && s[n][e] <= 0x1p-25f);
+                }
+            bool one_by_one = key0 + 31 > low;
+            if (!BF16 && !one_by_one && __any_sync(0xffffffffu, lost)) {   // (a lost weight of an infinity is none of zero)
+                bool found = false;
+                for (int d = d0 + 8 * t; d < min(hd, d0 + PANEL); d += 32)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const uint4 b = load8(v0 + (size_t)(key0 + 8 * n + g) * p.v_stride + d, true, vec_kv);
+                        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) found = found || (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+                    }
+                one_by_one = __any_sync(0xffffffffu, found);
+            }
+            if (!one_by_one) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t pa[4] = {pack2_t<BF16>(s[2 * h][0], s[2 * h][1]), pack2_t<BF16>(s[2 * h][2], s[2 * h][3]), pack2_t<BF16>(s[2 * h + 1][0], s[2 * h + 1][1]),
+                                            pack2_t<BF16>(s[2 * h + 1][2], s[2 * h + 1][3])};
+                    const uint16_t* v = v0 + (size_t)(key0 + 16 * h + 2 * t) * p.v_stride;
+#pragma unroll
+                    for (int c = 0; c < PANEL / 64; ++c) {
+                        const int d = d0 + 64 * c + 8 * g;
+                        if (c > 0 && d0 + 64 * c >= hd) break;
+                        const uint4 w0 = load8(v + d, d < hd, vec_kv), w1 = load8(v + p.v_stride + d, d < hd, vec_kv), w2 = load8(v + 8 * p.v_stride + d, d < hd, vec_kv),
+                                    w3 = load8(v + 9 * p.v_stride + d, d < hd, vec_kv);
+                        const uint32_t r0[4] = {w0.x, w0.y, w0.z, w0.w}, r1[4] = {w1.x, w1.y, w1.z, w1.w}, r2[4] = {w2.x, w2.y, w2.z, w2.w}, r3[4] = {w3.x, w3.y, w3.z, w3.w};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const unsigned pick = i & 1 ? 0x7632 : 0x5410;
+                            mma_t<BF16>(o[8 * c + i], pa, __byte_perm(r0[i / 2], r1[i / 2], pick), __byte_perm(r2[i / 2], r3[i / 2], pick));
+                        }
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int k = 0; k < 32 && key0 + k < keys; ++k) {
+                    float w[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float a = k & 1 ? (k & 8 ? (k & 16 ? s[3][2 * e + 1] : s[1][2 * e + 1]) : (k & 16 ? s[2][2 * e + 1] : s[0][2 * e + 1]))
+                                              : (k & 8 ? (k & 16 ? s[3][2 * e] : s[1][2 * e]) : (k & 16 ? s[2][2 * e] : s[0][2 * e]));
+                        w[e] = __shfl_sync(0xffffffffu, a, (lane & ~3) | ((k & 7) >> 1));
+                    }
+                    const bool on[2] = {key0 + k <= tok[0], key0 + k <= tok[1]};
+                    const uint16_t* v = v0 + (size_t)(key0 + k) * p.v_stride;
+#pragma unroll
+                    for (int c = 0; c < PANEL / 32; ++c) {
+                        const int d = d0 + 64 * (c >> 1) + 16 * t + 8 * (c & 1);
+                        const uint4 x = load8(v + d, d < hd, vec_kv);
+                        const uint32_t r[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float f = t_to_f32<BF16>((uint16_t)(r[i / 2] >> (16 * (i & 1))));
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if (on[e]) o[8 * (c >> 1) + i][2 * e + (c & 1)] = fmaf(w[e], f, o[8 * (c >> 1) + i][2 * e + (c & 1)]);
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+            if (!(which >> (g + 8 * e) & 1)) continue;
+#pragma unroll
+            for (int c = 0; c < PANEL / 32; ++c) {
+                const int d = d0 + 64 * (c >> 1) + 16 * t + 8 * (c & 1);
+                if (d >= hd) continue;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p.out[out_at[e] + d + i] = f32_to_t<BF16>(__fdiv_rn(o[8 * (c >> 1) + i][2 * e + (c & 1)], l[e]));
+            }
+        }
+    }
+}
+
+// Which of a run of eight values are NaN, infinite, infinite below zero: a bit a value.
+struct Odd {
+    unsigned nan, up, down;
+    __device__ __forceinline__ unsigned any() const { return nan | up | down; }
+    __device__ __forceinline__ unsigned lost() const { return nan | (up & down); }                // a sum of these is a NaN
+};
+template <int BF16>
+__device__ __forceinline__ void note(Odd& o, const uint4 x) {
+    constexpr unsigned kExp = BF16 ? 0x7f80u : 0x7c00u;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const unsigned u = w[e / 2] >> (16 * (e & 1)) & 0xffffu;
+        o.nan |= (unsigned)((u & 0x7fffu) > kExp) << e;
+        o.up |= (unsigned)(u == kExp) << e;
+        o.down |= (unsigned)(u == (kExp | 0x8000u)) << e;
+    }
+}
+// Rows r0 .. of a tile of `rows` that starts at n0 and whose key blocks end before row `to` of the batch: those of `mask` have results that are not finite.  A warp, once what
+// it has stored is there.  A depth counts where a key that not all of the warp's rows attend to has a value that is not finite.  Where one that they all attend to has one
+// as well, the sum is what these leave -- an infinity, or a NaN -- and is written; else the rows are formed again.  (A depth that is
+// infinite at every position is the former: 8192 rows 0.88 ms for 0.42.)
+template <int BF16, int VEC, int PANEL>
+__device__ __forceinline__ void mend(const PromptArgs& p, int first, int kvh, long long n0, int to, int r0, int rows, unsigned mask, int vec) {
+    __syncwarp();
+    const int lane = threadIdx.x & 31, hd = p.head_dim, group = p.heads / p.kv_heads, low = first + (int)((n0 + r0) / group);
+    const uint16_t* v = p.v + (size_t)kvh * hd;
+    const bool in = 8 * lane < hd, vec_kv = VEC || (vec >> 1);
+    Odd later = {0, 0, 0}, had = {0, 0, 0};                            // of this lane's depths 8 lane ..
+#pragma unroll 4
+    for (int j = low + 1; j < to; ++j) note<BF16>(later, load8(v + (size_t)j * p.v_stride + 8 * lane, in, vec_kv));
+    const unsigned depths = later.any();
+    for (unsigned left = __ballot_sync(0xffffffffu, depths != 0); left; left &= left - 1) {
+        const int c = __ffs(left) - 1;                                 // eight depths, a key a lane, from the last one back
+        const unsigned want = __shfl_sync(0xffffffffu, depths, c);
+        Odd o = {0, 0, 0};
+        for (int j0 = low; j0 >= first; j0 -= 128) {
+            uint4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = j0 - 32 * i - lane;
+                x[i] = load8(v + (size_t)max(j, first) * p.v_stride + 8 * c, j >= first, vec_kv);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) note<BF16>(o, x[i]);
+            const unsigned u = __reduce_or_sync(0xffffffffu, o.nan | o.up << 8 | o.down << 16);
+            o = {u & 0xffu, u >> 8 & 0xffu, u >> 16};
+            if ((want & ~o.lost()) == 0) break;                        // (nothing changes a NaN)
+        }
+        if (lane == c) had = o;
+    }
+    if (__any_sync(0xffffffffu, (depths & ~had.any()) != 0)) {
+        for (int h = 0; h < 32; h += 16)
+            if (mask >> h & 0xffffu) form_again<BF16, VEC, PANEL>(p, first, kvh, n0 + r0 + h, min(16, rows - r0 - h), mask >> h & 0xffffu, vec);
+        return;
+    }
+    int at = low;                                                      // keys up to here are in `had`
+    for (; mask; mask &= mask - 1) {
+        const long long n = n0 + r0 + __ffs(mask) - 1;
+        const int tok = (int)(n / group), head = kvh * group + (int)(n - (long long)tok * group);
+        for (; at < first + tok; ++at) note<BF16>(had, load8(v + (size_t)(at + 1) * p.v_stride + 8 * lane, in, vec_kv));
+        uint16_t* y = p.out + (size_t)(first + tok) * p.out_stride + (size_t)head * hd + 8 * lane;
+        for (int e = 0; e < 8; ++e)
+            if (depths >> e & 1) y[e] = f32_to_t<BF16>(had.lost() >> e & 1 ? __uint_as_float(0x7fc00000u) : (had.up >> e & 1 ? kInf : -kInf));
+    }
+}
+
+// ---- any strides, heads of up to 256 depths: warp-level MMAs ----
+constexpr int kPwThreads = 128, kPwRows = 64, kPwKeys = 64;
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
 // Sequence and piece of a work slot: `slot` counts pieces of 2^log2_len packed (row, head of the group) pairs.  The block's threads together.
 __device__ __forceinline__ bool find_piece(const PromptArgs& p, int group, long long slot, int log2_len, int threads, int* first, int* rows, long long* piece) {
     int n = 0;
@@ -157,7 +300,7 @@ __device__ __forceinline__ bool find_piece(const PromptArgs& p, int group, long 
 }
 
 template <int BF16, int HD>
-__global__ void __launch_bounds__(kPwThreads) prompt_mma_kernel(const __grid_constant__ PromptArgs p, int vec_q, int vec_kv) {
+__global__ void __launch_bounds__(kPwThreads, HD == 64 ? 4 : (HD == 128 ? 3 : 2)) prompt_mma_kernel(const __grid_constant__ PromptArgs p, int vec_q, int vec_kv) {
     constexpr int LD = HD + 8;
     extern __shared__ __align__(16) uint16_t tile[];
     uint16_t *q_s = tile, *k_s = q_s + kPwRows * LD, *v_s = k_s + kPwKeys * LD;
@@ -170,7 +313,7 @@ __global__ void __launch_bounds__(kPwThreads) prompt_mma_kernel(const __grid_con
     if (!find_piece(p, group, (long long)(gridDim.x - 1 - blockIdx.x), 6, kPwThreads, &first, &rows, &piece)) return;
     const long long n0 = piece * kPwRows;
     const int nrow = (int)min((long long)kPwRows, (long long)rows * group - n0);
-    const int i_first = (int)(n0 / group), keys = (int)((n0 + nrow - 1) / group) + 1;      // rows of the sequence; keys of the tile's last row
+    const int keys = (int)((n0 + nrow - 1) / group) + 1;                                   // of the tile's last row
     for (int it = tid; it < kPwRows * (HD / 8); it += kPwThreads) {
         const int r = it / (HD / 8), d = (it - r * (HD / 8)) * 8;
         const int i = (int)((n0 + r) / group), head = kvh * group + (int)(n0 + r - (long long)i * group);
@@ -277,18 +420,14 @@ __global__ void __launch_bounds__(kPwThreads) prompt_mma_kernel(const __grid_con
                 }
             }
     }
+    unsigned which = 0;                                                // a bit a row
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-        unsigned mask = __ballot_sync(0xffffffffu, bad[e]);
-        mask = (mask | mask >> 1 | mask >> 2 | mask >> 3) & 0x11111111u;      // one bit a row
-        if (!mask || !spoilt_by_later(p, kvh, first, first + i_first, first + keys)) continue;
-        for (; mask; mask &= mask - 1) {
-            const long long n = n0 + 16 * warp + (__ffs(mask) - 1) / 4 + 8 * e;
-            const int i = (int)(n / group);
-            __syncwarp();
-            exact_row<BF16>(p, first, first + i, kvh * group + (int)(n - (long long)i * group));
-        }
+        const unsigned mask = __ballot_sync(0xffffffffu, bad[e]);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) which |= (unsigned)((mask >> (4 * r) & 0xfu) != 0) << (r + 8 * e);
     }
+    if (which) mend<BF16, 0, HD == 64 ? 64 : 128>(p, first, kvh, n0, first + keys, 16 * warp, nrow, which, vec_q | vec_kv << 1);
 }
 
 // ---- rows on 16-byte boundaries: tcgen05 ----
@@ -354,6 +493,10 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return r;
 }
 
+// The last items of a CTA: it takes no more once a softmax warp has met rows to mend.  When one warp has done item f, the slowest is at f - 2 (a place of two is free again when
+// all have read it) and the loads at f + 3 at most (that CTA may have been asked for).
+constexpr int kPtKept = 8;
+
 struct PromptTc {
     CUtensorMap q, k, v, out;
     PromptArgs p;
@@ -385,6 +528,21 @@ __device__ __forceinline__ int taken_cta(uint32_t answer) {        // its index,
     return ok ? (int)x : -1;
 }
 
+// The rows of this warp that are left, by item: mend() for each.
+template <int BF16, int NCH>
+__device__ __forceinline__ void mend_items(const PromptTc& a, const PromptItem* items, const unsigned (*odd)[kPtKept]) {
+    const int warp = threadIdx.x >> 5, tt = a.tokens, group = a.p.heads / a.p.kv_heads;
+#pragma unroll 1
+    for (int k = 0; k < kPtKept; ++k) {
+        const unsigned mask = odd[warp][k];
+        if (!mask) continue;
+        const PromptItem w = items[k];
+        const int low = w.tok0 + (warp >> 2) * tt, ntok = min(tt, w.rows - low), n = (low + ntok - 1) / kPtKeys + 1;
+        mend<BF16, 1, NCH == 1 ? 64 : 128>(a.p, w.first, w.kvh, (long long)low * group, min(w.first + n * kPtKeys, a.p.rows), (warp & 3) * 32, ntok * group, mask, 3);
+    }
+}
+template <int BF16>
+__device__ __noinline__ void mend_items_1(const PromptTc& a, const PromptItem* items, const unsigned (*odd)[kPtKept]) { mend_items<BF16, 1>(a, items, odd); }
 // BULK: a softmax warp's 32 rows are whole tokens, out lies on 16-byte boundaries, and full warps' results leave by bulk stores from the warp's stage.
 template <int BF16, int NCH, int BULK>
 __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptTc a) {
@@ -394,7 +552,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     __shared__ __align__(16) uint4 answer;
     __shared__ __align__(8) uint64_t bars[2 * kPtMaxSlots + 15];
-    __shared__ PromptItem items[2];
+    __shared__ PromptItem items[2], kept[kPtKept];
+    __shared__ unsigned odd[8][kPtKept];                           // of a softmax warp's rows of an item, those with results that are not finite
+    __shared__ int odd_any;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
@@ -404,8 +564,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     const int hd = p.head_dim, hd16 = (hd + 15) & ~15, group = p.heads / p.kv_heads, tt = a.tokens;
     unsigned char *q_s = smem, *out_s = smem + kTiles * kTile, *ring = out_s + kTiles * 4 * kPtStage;
 
+    if (tid < 8 * kPtKept) odd[tid / kPtKept][tid % kPtKept] = 0;
     if (tid == 0) {
         abort_word = 0;
+        odd_any = 0;
         for (int i = 0; i < a.slots; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
@@ -483,6 +645,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                 if (!ok) break;
                 if (lane == 0) {
                     items[k] = w;
+                    kept[it % kPtKept] = w;
                     mbar_arrive(&item_full[k]);
                 }
                 __syncwarp();
@@ -504,6 +667,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
                     for (int j = 0; ok && j < n; ++j) ok = (j + 1 == n || load(&a.k, w, j + 1)) && load(&a.v, w, j);
                 }
                 if (!ok) break;
+            }
+            if (__any_sync(0xffffffffu, *const_cast<volatile int*>(&odd_any))) {
+                cta = -1;                                          // (rows to mend: the slots that are left get CTAs of their own)
+                continue;
             }
             if (elect_one()) {
                 fence_proxy_async();                               // (the last answer has been read)
@@ -612,7 +779,6 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
         const int t = row / group, g = row - t * group;
         const uint32_t ts0 = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * x, to = ts0 + kPtO;
         const float sc = p.scale_log2e;
-        const bool vec = (((uintptr_t)p.out | (p.out_stride * 2)) & 15) == 0;
         int done = 0, tiles = 0;                                   // blocks and tiles so far
         bool ok = true;
         PromptItem w;
@@ -788,13 +954,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
             float z0, z1;
             unpack64(zero, z0, z1);
             const bool bad = !(z0 + z1 == 0.0f);
-            unsigned mask = __ballot_sync(0xffffffffu, in && bad && l > 0.0f);
-            if (mask && spoilt_by_later(p, w.kvh, w.first, w.first + low, min(w.first + n * kPtKeys, p.rows)))
-                for (BULK ? bulk_wait_all() : void(); mask; mask &= mask - 1) {    // (behind what has been stored there)
-                    const int r = __ffs(mask) - 1, tk = __shfl_sync(0xffffffffu, tok, r), h = __shfl_sync(0xffffffffu, head, r);
-                    __syncwarp();
-                    exact_row<BF16>(p, w.first, w.first + tk, h);
-                }
+            const unsigned mask = __ballot_sync(0xffffffffu, bad && l > 0.0f) & rows_in;
+            if (mask) {
+                odd[warp][it % kPtKept] = mask;
+                *const_cast<volatile int*>(&odd_any) = 1;
+            }
         }
         if (BULK) {
             if (lane == 0) bulk_wait_all();                        // (stored, not only read: the grid that waits for this one finds the results)
@@ -806,6 +970,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prompt_tc_kernel(const __grid_c
     if (warp == 9) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+    // Rows to mend, once nobody waits for this CTA.  (A call within the softmax loop costs its registers there, whatever is behind it: 7001 rows 65.7 us and 71.5, 8192 rows 494 and 521.  Here,
+    // inline, 64.1 and 489; heads of 64 are better off with a call, 200 rows 8.5 and 8.7.)
+    if (odd_any && warp_index() < 8) {
+        if (NCH == 1) mend_items_1<BF16>(a, kept, odd);
+        else mend_items<BF16, NCH>(a, kept, odd);
     }
 }
 

@@ -868,3 +868,71 @@ def test_prompts_whose_warps_run_apart(heads, kv, hd, dtype):
             first = out
             _near(out, want, tol, dtype)
         assert torch.equal(out, first)
+
+
+def _lost(v, rows, heads, kv):
+    """What the infinities and NaNs among v leave of each result whose weights are all above zero: 0 nothing, +-inf, NaN ([rows, heads * head_dim], 64 bits)."""
+    out = []
+    r0 = 0
+    for r in rows:
+        x = v[r0:r0 + r].double().reshape(r, kv, -1)
+        nan, up, down = (torch.cummax(y.to(torch.int8), 0).values.bool() for y in (torch.isnan(x), x == math.inf, x == -math.inf))
+        y = torch.zeros_like(x)
+        y[up], y[down], y[nan | (up & down)] = math.inf, -math.inf, math.nan
+        out.append(y.repeat_interleave(heads // kv, 1).reshape(r, -1))
+        r0 += r
+    return torch.cat(out)
+
+
+@pytest.mark.parametrize("heads,kv,hd,dtype,shift", [(8, 2, 64, F16, 0), (8, 2, 128, BF16, 0), (4, 2, 256, F16, 0), (6, 1, 80, BF16, 0), (3, 3, 96, F16, 0), (4, 2, 192, BF16, 0),
+                                                     (8, 2, 64, BF16, 1), (8, 2, 128, F16, 1), (2, 2, 256, F16, 1), (5, 5, 40, F16, 1),
+                                                     (32, 8, 64, F16, 0), (32, 8, 128, BF16, 0)])
+@pytest.mark.parametrize("kind", ["channel", "down", "scattered", "late"])
+def test_infinities_all_over_the_values_of_packed_prompts(heads, kv, hd, dtype, shift, kind):
+    """A depth that is infinite at every position, infinities and NaNs at every hundredth, one at the end of each sequence: each result is the sum over what its row attends to.
+    (With 32 heads there are more items of work than SMs.)"""
+    gen = _gen(hd + len(kind))
+    rows = [1400, 33, 1300] if heads == 32 else [700, 33, 300]
+    total = sum(rows)
+    width = (heads + 2 * kv) * hd + 8
+    x = _randn(gen, total * width + shift, dtype=dtype)[shift:].view(total, width)
+    q, k, v = x[:, :heads * hd], x[:, heads * hd:(heads + kv) * hd], x[:, (heads + kv) * hd:(heads + 2 * kv) * hd]
+    if kind in ("channel", "down"):
+        v[:, 5] = math.inf if kind == "channel" else -math.inf
+    elif kind == "late":
+        v[[rows[0] - 10, rows[0] + 32, total - 1], hd - 3] = torch.tensor([math.inf, math.nan, -math.inf], device="cuda", dtype=dtype)
+    else:
+        at = torch.rand(v.shape, generator=gen, device="cuda") < 0.01 / hd
+        v[at] = torch.tensor([math.inf, -math.inf, math.nan], device="cuda", dtype=dtype)[torch.randint(0, 3, v.shape, generator=gen, device="cuda")][at]
+    out = torch.empty(total, heads * hd, dtype=dtype, device="cuda")
+    sg.attend_packed(q, k, v, _int([0] + np.cumsum(rows).tolist()), out, heads, kv)
+    lost = _lost(v, rows, heads, kv)
+    clean = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    want, tol = _prompt(q, k, clean, rows, heads, kv)
+    whole = lost == 0
+    assert whole.any() and not whole.all()
+    _near(out[whole], want[whole], tol[whole], dtype)
+    assert torch.equal(out[~whole].double().nan_to_num(7.0, posinf=8.0, neginf=9.0), lost[~whole].nan_to_num(7.0, posinf=8.0, neginf=9.0))
+
+
+def test_an_infinite_channel_costs_no_pass_of_single_values():
+    """Every row of such a prompt is formed again.  Warp-level products take some ten times as long as the others, their operands come from the L2 cache piece by piece, which
+    doubles that, and a pass comes before: 25 times at most, where a key at a time for each row took hundreds."""
+    gen = _gen(77)
+    heads, kv, hd, n = 32, 8, 128, 4096
+    q, k, v = _randn(gen, n, heads * hd), _randn(gen, n, kv * hd), _randn(gen, n, kv * hd)
+    bad = v.clone()
+    bad.view(n, kv, hd)[:, :, 9] = math.inf
+    out, cu, took = torch.empty_like(q), _int([0, n]), []
+    for x in (v, bad):
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            sg.attend_packed(q, k, x, cu, out, heads, kv)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        took.append(min(times[1:]))
+    assert torch.all(out.view(n, heads, hd)[:, :, 9] == math.inf) and torch.isfinite(out.view(n, heads, hd)[:, :, :9]).all()
+    assert took[1] < 25 * took[0], took
