@@ -17,7 +17,7 @@
 // keeps the operand loads off each other's banks); a lane then takes 16 consecutive depths of a key as four steps of the first product, and 16
 // depths of its four keys as eight row tiles of the second.  The ring runs ahead over the ends of items, so that the next item's keys are on their way
 // while the warps' shares of this one meet.  A query row is scaled by a power of two into f16's range (so bf16 queries are exact too); the
-// probabilities are f16 at 2^7, a group's scaled by its page's scale over the larger of the warp's two; the reference of a row's exponentials follows
+// probabilities are f16 at 2^7, and a page's product is multiplied by its scale in 32 bits; the reference of a row's exponentials follows
 // its maximum when that is 2^8 above it; each 32 keys' sums are folded into 32-bit registers, since the tensor core cuts its sums off.
 //
 // Measured: a long context streams at 6.8 TB/s beside 12 to 15 us that do not depend on its length (launches, the first bytes, the warps' meeting, the join): one token over
@@ -240,8 +240,12 @@ __device__ __forceinline__ float4 ld_dsmem4(uint32_t cluster_addr) {
     return v;
 }
 
-// CL: the CTAs of a cluster (2^cluster_log2 of them) share one item's units and meet in distributed shared memory, without a second kernel: for few items of few units.
-template <int BF16, int HC, int NT, int CL>
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+// P16: pages of 16 positions, two of which make a piece; else a piece lies in one.  CL: the CTAs of a cluster (2^cluster_log2 of them) share one item's units and meet in distributed shared memory, without a second kernel: for few items of few units.
+template <int BF16, int HC, int NT, int CL, int P16>
 __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kernel(const __grid_constant__ PagedMaps maps, const __grid_constant__ PagedAttendArgs p) {
     constexpr int MT = 4 * HC;                       // tiles of 16 depths
     constexpr int NR = 8 * NT;
@@ -256,7 +260,7 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int hd = p.head_dim, group = p.heads / p.kv_heads, page = 1 << p.seqs.page_log2;
+    const int hd = p.head_dim, group = p.heads / p.kv_heads, page = P16 ? 16 : 1 << p.seqs.page_log2;
     if (tid == 0) {
         abort_word = 0;
         for (int w = 0; w < kPaWarps; ++w)
@@ -306,7 +310,7 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
                 int id[2];
                 id[0] = (unsigned)row[0] < (unsigned)p.seqs.pages ? row[0] : -1;
                 id[1] = key0 + 16 >= ahead.U.keys ? -2 : id[0];
-                if (page < 32 && id[1] != -2) id[1] = (unsigned)row[1] < (unsigned)p.seqs.pages ? row[1] : -1;
+                if (P16 && id[1] != -2) id[1] = (unsigned)row[1] < (unsigned)p.seqs.pages ? row[1] : -1;
                 if (lane == 0) {
                     if ((id[0] == -1 || id[1] == -1) && p.status) atomicOr(p.status, STATUS_PAGE);
                     const int z0 = 2 * (id[0] * p.kv_heads + ahead.kvh), z1 = 2 * (id[1] * p.kv_heads + ahead.kvh);
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
                     const uint32_t dst = ring + put * kStage;
                     uint64_t* bar = &full[warp][put];
                     const int y = key0 & (page - 1);
-                    if (page >= 32) {
+                    if (!P16) {
                         mbar_expect_tx(bar, id[0] < 0 ? 0 : kStage);
                         if (id[0] >= 0)
 #pragma unroll
@@ -468,10 +472,12 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
                             mma_f16(sc[j][b], a0, a1, a2, a3, qf[j][4 * c + w][0], qf[j][4 * c + w][1], c + w == 0 ? start0[j] : sc[j][b]);
                     }
                 }
-            const float st = fmaxf(fmaxf(sv[0], sv[1]), 0.0f);         // (fmaxf drops a NaN: it stays with the rows that attend to it)
-            float ratio[2];
+            // Probabilities at 2^7, NaN under a scale that is NaN: it stays with the rows that attend to it.  Two pages of 16 have a product each, with their own scale.  (With a common factor for
+            // both, the smaller scale's probabilities have few bits or none left in f16 where the scales are far apart, whatever the weight of the larger one's keys is for a row: none, where
+            // the row does not attend to them.)
+            float one[2];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) ratio[b] = (sv[b] == st ? 1.0f : (st > 0.0f ? __fdividef(sv[b], st) : sv[b])) * kPScale;
+            for (int b = 0; b < 2; ++b) one[b] = fmaf(sv[P16 ? b : 0], 0.0f, kPScale);
             const bool whole = key0 + 32 <= low && here0 && here1;
             uint32_t pf[NT][2][2];
 #pragma unroll
@@ -529,52 +535,61 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
                     for (int e = 0; e < 4; ++e) {
                         const float x = ex2(sc[j][b][e] - ref[e & 1]);
                         l_run[j][e & 1] += x;
-                        w[e] = x * ratio[b];
+                        w[e] = x * one[b];
                         if (!whole && !(on >> (4 * b + e) & 1)) w[e] = 0.0f;          // (not 0 * the NaN of a page that the row does not attend to)
                     }
                     pf[j][b][0] = mov_trans(pack2_t<0>(w[0], w[1]));
                     pf[j][b][1] = mov_trans(pack2_t<0>(w[2], w[3]));
                 }
             }
-            // values
-            float off0[NT][4];
+            // values: += the products of groups FIRST .. FIRST + COUNT times their scale
+            auto add_values = [&](auto from, auto count, float scale) {
+                constexpr int FIRST = decltype(from)::value, LAST = FIRST + decltype(count)::value - 1;
+                float off0[NT][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                mma_f16(off0[j], kOffset, kOffset, kOffset, kOffset, pf[j][0][0], pf[j][0][1], zero4);
-                mma_f16(off0[j], kOffset, kOffset, kOffset, kOffset, pf[j][1][0], pf[j][1][1], off0[j]);
+                for (int j = 0; j < NT; ++j) {
+                    mma_f16(off0[j], kOffset, kOffset, kOffset, kOffset, pf[j][FIRST][0], pf[j][FIRST][1], zero4);
+                    if (LAST > FIRST) mma_f16(off0[j], kOffset, kOffset, kOffset, kOffset, pf[j][LAST][0], pf[j][LAST][1], off0[j]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) off0[j][e] = -off0[j][e];
-            }
+                    for (int e = 0; e < 4; ++e) off0[j][e] = -off0[j][e];
+                }
 #pragma unroll
-            for (int c = 0; c < (HC == 4 ? 2 : 1); ++c) {
-                uint32_t vw[2][4][4];                                  // group, key, word
+                for (int c = 0; c < (HC == 4 ? 2 : 1); ++c) {
+                    uint32_t vw[2][4][4];                              // group, key, word
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                    for (int b = FIRST; b <= LAST; ++b)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t a = stage + kHalf + c * kPanel + (16 * b + 8 * (r >> 1)) * kPitch + (r & 1 ? v_odd : v_even);
-                        const uint4 v = HC == 1 ? lds8(a) : lds16(a);
-                        vw[b][r][0] = v.x; vw[b][r][1] = v.y; vw[b][r][2] = v.z; vw[b][r][3] = v.w;
-                    }
-#pragma unroll
-                for (int w = 0; w < (HC == 1 ? 2 : 4); ++w)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {                      // depths 4 w + 2 h and the next: row tile m
-                        const int m = 8 * c + 2 * w + h;
-                        float acc[NT][4];
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            const uint32_t x = __byte_perm(vw[b][0][w], vw[b][1][w], h ? 0x7632 : 0x5410), y = __byte_perm(vw[b][2][w], vw[b][3][w], h ? 0x7632 : 0x5410);
-                            const uint32_t a0 = even_bytes(x), a1 = odd_bytes(x), a2 = even_bytes(y), a3 = odd_bytes(y);
-#pragma unroll
-                            for (int j = 0; j < NT; ++j) mma_f16(acc[j], a0, a1, a2, a3, pf[j][b][0], pf[j][b][1], b ? acc[j] : off0[j]);
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t a = stage + kHalf + c * kPanel + (16 * b + 8 * (r >> 1)) * kPitch + (r & 1 ? v_odd : v_even);
+                            const uint4 v = HC == 1 ? lds8(a) : lds16(a);
+                            vw[b][r][0] = v.x; vw[b][r][1] = v.y; vw[b][r][2] = v.z; vw[b][r][3] = v.w;
                         }
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            fma2(o[j][m][0], o[j][m][1], acc[j][0], acc[j][1], st);
-                            fma2(o[j][m][2], o[j][m][3], acc[j][2], acc[j][3], st);
+                    for (int w = 0; w < (HC == 1 ? 2 : 4); ++w)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {                  // depths 4 w + 2 h and the next: row tile m
+                            const int m = 8 * c + 2 * w + h;
+                            float acc[NT][4];
+#pragma unroll
+                            for (int b = FIRST; b <= LAST; ++b) {
+                                const uint32_t x = __byte_perm(vw[b][0][w], vw[b][1][w], h ? 0x7632 : 0x5410), y = __byte_perm(vw[b][2][w], vw[b][3][w], h ? 0x7632 : 0x5410);
+                                const uint32_t a0 = even_bytes(x), a1 = odd_bytes(x), a2 = even_bytes(y), a3 = odd_bytes(y);
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) mma_f16(acc[j], a0, a1, a2, a3, pf[j][b][0], pf[j][b][1], b > FIRST ? acc[j] : off0[j]);
+                            }
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                fma2(o[j][m][0], o[j][m][1], acc[j][0], acc[j][1], scale);
+                                fma2(o[j][m][2], o[j][m][3], acc[j][2], acc[j][3], scale);
+                            }
                         }
-                    }
+                }
+            };
+            if (P16) {
+                add_values(Int<0>(), Int<1>(), fmaxf(sv[0], 0.0f));    // (fmaxf drops a NaN)
+                add_values(Int<1>(), Int<1>(), fmaxf(sv[1], 0.0f));
+            } else {
+                add_values(Int<0>(), Int<2>(), fmaxf(sv[0], 0.0f));
             }
             last = get;
             if (++get == kStages) { get = 0; parity ^= 1; }
@@ -869,9 +884,9 @@ int cluster_of(const PagedAttendArgs& a, int tile_rows, int sm_count) {
     return 0;
 }
 
-template <int BF16, int HC, int NT, int CL>
+template <int BF16, int HC, int NT, int CL, int P16>
 cudaError_t attend_launch(const PagedAttendArgs& a, int workers, cudaStream_t stream) {
-    auto kern = paged_attend_kernel<BF16, HC, NT, CL>;
+    auto kern = paged_attend_kernel<BF16, HC, NT, CL, P16>;
     TensorMapEncodeFn enc = tensor_map_encoder();
     if (!enc) return cudaErrorNotSupported;
     const int page = 1 << a.seqs.page_log2;
@@ -929,7 +944,8 @@ cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaS
     const int workers = a.cluster_log2 ? (int)(items_most(a, tr) << a.cluster_log2) : workers_of(a, tr, sm_count);
     const int hc = a.head_dim <= 64 ? 1 : (a.head_dim <= 128 ? 2 : 4);
     cudaError_t e;
-#define SMEG_PA(B, H, N) (a.cluster_log2 ? attend_launch<B, H, N, 1>(a, workers, stream) : attend_launch<B, H, N, 0>(a, workers, stream))
+#define SMEG_PA2(B, H, N, C) (a.seqs.page_log2 == 4 ? attend_launch<B, H, N, C, 1>(a, workers, stream) : attend_launch<B, H, N, C, 0>(a, workers, stream))
+#define SMEG_PA(B, H, N) (a.cluster_log2 ? SMEG_PA2(B, H, N, 1) : SMEG_PA2(B, H, N, 0))
     if (bf16) {
         if (tr == 8) e = hc == 1 ? SMEG_PA(1, 1, 1) : (hc == 2 ? SMEG_PA(1, 2, 1) : SMEG_PA(1, 4, 1));
         else e = hc == 1 ? SMEG_PA(1, 1, 2) : (hc == 2 ? SMEG_PA(1, 2, 2) : SMEG_PA(1, 4, 2));
@@ -938,6 +954,7 @@ cudaError_t paged_attend_launch(PagedAttendArgs a, int bf16, int sm_count, cudaS
         else e = hc == 1 ? SMEG_PA(0, 1, 2) : (hc == 2 ? SMEG_PA(0, 2, 2) : SMEG_PA(0, 4, 2));
     }
 #undef SMEG_PA
+#undef SMEG_PA2
     if (e != cudaSuccess || workers == 1 || a.cluster_log2) return e;
     const long long items = items_bound(a, tr);
     if (items >= workers)

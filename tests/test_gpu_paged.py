@@ -936,3 +936,39 @@ def test_an_infinite_channel_costs_no_pass_of_single_values():
         took.append(min(times[1:]))
     assert torch.all(out.view(n, heads, hd)[:, :, 9] == math.inf) and torch.isfinite(out.view(n, heads, hd)[:, :, :9]).all()
     assert took[1] < 25 * took[0], took
+
+
+@pytest.mark.parametrize("heads,kv,hd,dtype,ratio", [(2, 1, 64, F16, 2.0 ** -14), (8, 1, 128, BF16, 2.0 ** -20), (4, 2, 256, BF16, 2.0 ** -40), (24, 1, 64, BF16, 2.0 ** -60), (2, 2, 128, F16, 2.0 ** -9)])
+@pytest.mark.parametrize("small_first", [True, False])
+def test_pages_of_small_values_beside_pages_of_large_ones(heads, kv, hd, dtype, ratio, small_first):
+    """Two pages of 16 of one piece of 32 keys, the values of one far below the other's: rows that attend to the first page alone, and rows whose weights lie on the small one.  The
+    bound counts a page's scale with its weight: an error of a product's steps is one of what the product adds."""
+    pool = Pool(heads, kv, hd, 16, 1, 6, seed=hd + heads, dtype=dtype)
+    group, n = heads // kv, 64
+    k, v = (_randn(pool.gen, n, kv * hd, dtype=dtype, scale=s) for s in (0.05, 1.0))
+    small = (torch.arange(n, device="cuda") // 16 % 2 == (0 if small_first else 1))
+    v[small] *= ratio
+    k.view(n, kv, hd)[:, :, 0] = torch.where(small, 8.0, -8.0)[:, None].to(dtype)       # a query's first depth says how much less the large page's keys weigh
+    pool.cache.append(k, v, pool.batch([n]))
+    pool.have = [n]
+    start, rows = 8, n - 8
+    q = _randn(pool.gen, rows, heads * hd, dtype=dtype)
+    q.view(rows, heads, hd)[:, :, 0] = (torch.arange(rows, device="cuda") % 3 * 1.5 * math.sqrt(hd))[:, None].to(dtype)   # e^0, e^-24, e^-48
+    out = torch.empty_like(q)
+    pool.cache.attend(q, pool.batch([rows], starts=[start]), out)
+    x, sc = pool.values(0)
+    kk, vv = x.repeat_interleave(group, 2)
+    sk, sv = sc.repeat_interleave(group, 2)[..., 0]
+    z = torch.einsum("rhd,nhd->hrn", q.double().reshape(rows, heads, hd), kk) * pool.cache.scale()
+    z = z.masked_fill(torch.arange(n, device="cuda")[None, :] > start + torch.arange(rows, device="cuda")[:, None], -math.inf)
+    p = torch.softmax(z, -1)
+    want, a, step = (torch.einsum("hrn,nhd->rhd", p, y) for y in (vv, vv.abs(), sv[..., None].expand(-1, -1, hd)))
+    # A score's chain: (hd / 16 + 4) * 2^-23 of sum |q| * 255 * scale_k and 2^-21 of itself, four times that of the result; a probability's rounding 2^-11 of what it adds, or half
+    # of f16's last place (2^-25, of probabilities that stand 2^7 higher, in sums that reach 1 at least) of its page's values, 32 keys a time
+    e = (hd / 16 + 4) * 2.0 ** -23 * pool.cache.scale() * q.double().abs().reshape(rows, heads, hd).sum(-1) * 255 * sk.amax() + 2.0 ** -21 * z.masked_fill(z == -math.inf, 0).abs().amax(-1).T
+    on = (z > -math.inf).to(torch.float64)
+    floor = torch.einsum("hrn,nhd->rhd", on, vv.abs()) * 2.0 ** -32
+    tol = a * (2.0 ** -11 + 2.0 ** -18 + 4 * e[..., None]) + 2.0 ** -20 * 255 * step + floor * 2.0
+    _near(out.view(rows, heads, hd), want, tol, dtype)
+    lone = out.view(rows, heads, hd)[:8]                          # rows of the first page alone
+    assert lone.abs().amax() > 0
