@@ -286,7 +286,7 @@ int smeg_attn_kv_causal_f16_dev(uint16_t *out, const void *q, int q_f32, size_t 
  * sequence s's; rows behind the last one are left as they are.  Rows are heads * head_dim 16-bit values (f16, or bf16 with bf16 = 1), stride
  * elements apart.  starts[s] is the position of the sequence's first row, below zero for a sequence that is idle in this call; table[s *
  * table_cols + i] is the pool's page that holds its positions i * page ... (int32, device).  Row offsets outside the batch are clamped;
- * a position whose table entry names no page of the pool is skipped and raises bit 3 of smeg_last_status.
+ * a position whose table entry names no page of the pool, or that lies behind the table's columns, is skipped and raises bit 3 of smeg_last_status.
  *
  * The cache: codes uint8 [pages][kv_heads][keys, values][page][head_dim], scales f32 [pages][kv_heads][keys, values]; a value is (code - 128) *
  * scale.  page: a power of two in 16..=256; head_dim a multiple of 16 in 16..=256.  Scale = largest magnitude / 127 over the positions that were

@@ -375,11 +375,13 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
         const int kvh = now.kvh, tile0 = now.tile, tile1 = (int)min((long long)U.tiles, tile0 + now.left);
         const int n0 = now.row_tile * NR, nrow = (int)min((long long)NR, (long long)U.rows * group - n0);   // packed rows x heads of the tile
 
+        if (tid == 0 && p.status && beyond_table(U)) atomicOr(p.status, STATUS_PAGE);
+
         // ---- queries: B fragments, a power of two to each row ----
         uint32_t qf[NT][4 * HC][2];
         float row_scale[NT][2], start0[NT][4];
         int limit[NT][2];                            // keys that rows 2 t and 2 t + 1 of a tile attend to
-        const int low = U.start >= 0 ? min(U.start + div_by(n0, p.by_group) + 1, U.keys) : 0;    // keys that every row of the tile attends to
+        const int low = keys_of_row(U, div_by(n0, p.by_group));                                   // keys that every row of the tile attends to
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int n = n0 + 8 * j + g, i = div_by(n, p.by_group), head = kvh * group + (n - i * group);
@@ -430,7 +432,7 @@ __global__ void __launch_bounds__(kPaThreads, ctas_of(HC, NT)) paged_attend_kern
             for (int e = 0; e < 2; ++e) {
                 row_scale[j][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e));
                 const int m = n0 + 8 * j + 2 * t + e;
-                limit[j][e] = 8 * j + 2 * t + e < nrow && U.start >= 0 ? min(U.start + div_by(m, p.by_group) + 1, U.keys) : 0;
+                limit[j][e] = 8 * j + 2 * t + e < nrow ? keys_of_row(U, div_by(m, p.by_group)) : 0;
             }
         }
 

@@ -78,6 +78,13 @@ SMEG_HD SeqUnits seq_units(const PackedSeqs& p, int s, int group, int kv_heads, 
     u.items = ((long long)u.rows * group + tile_rows - 1) / tile_rows * kv_heads;
     return u;
 }
+// Keys that the sequence's row i attends to: positions up to its own that the table has room for.
+SMEG_HD int keys_of_row(const SeqUnits& u, int i) {
+    const uint32_t own = (uint32_t)u.start + (uint32_t)i + 1;      // (below 2^32: a start and a row are below 2^31)
+    return u.start < 0 ? 0 : (own < (uint32_t)u.keys ? (int)own : u.keys);
+}
+// Whether some row's own position lies behind what the table has room for.
+SMEG_HD bool beyond_table(const SeqUnits& u) { return u.start >= 0 && (uint32_t)u.start + (uint32_t)u.rows > (uint32_t)u.keys; }
 // x / y for x not below zero, in 32 bits where that will do (a 64-bit quotient is a hundred instructions).
 SMEG_HD long long quotient(long long x, int y) { return x <= 0xffffffffll ? (long long)((uint32_t)x / (uint32_t)y) : x / y; }
 // Worker w of n takes the units from share_begin(w) to share_begin(w + 1); unit u is worker share_of(u)'s.

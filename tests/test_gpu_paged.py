@@ -972,3 +972,21 @@ def test_pages_of_small_values_beside_pages_of_large_ones(heads, kv, hd, dtype, 
     _near(out.view(rows, heads, hd), want, tol, dtype)
     lone = out.view(rows, heads, hd)[:8]                          # rows of the first page alone
     assert lone.abs().amax() > 0
+
+
+@pytest.mark.parametrize("cols,seqs", [(2, 3), (40, 3), (60, 70)])
+def test_rows_behind_the_table_attend_to_what_it_has_room_for(cols, seqs):
+    """By clusters, by shares item by item and cut by cut: such rows attend to all positions of the table, and bit 3 of the status tells."""
+    pool = Pool(8, 2, 64, 64, seqs, cols, seed=cols)
+    room = cols * 64
+    pool.append([room] * seqs)
+    q = _randn(pool.gen, 2 * seqs, 512)
+    for start in (room - 1, room, room + 100, 2 ** 31 - 2, 2 ** 31 - 1):
+        starts = [5] + [start] * (seqs - 1)
+        out = torch.full_like(q, 7.0)
+        pool.cache.attend(q, pool.batch([2] * seqs, starts=starts), out)
+        assert sg.last_status() == 8
+        want, tol = _attended(pool, q, [2] * seqs, starts)
+        _near(out, want, tol, F16)
+    pool.cache.attend(q, pool.batch([2] * seqs, starts=[room - 2] * seqs), out)
+    assert sg.last_status() == 0

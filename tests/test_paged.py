@@ -129,3 +129,10 @@ def test_null_argument_structures_are_refused():
     read = dict(out=4096, codes=4096, scales=4096, ids=4096, n=1, pages=5, page=64, kv_heads=2, head_dim=64, bf16=0, reserved=0)
     for kw, rc in ((dict(page=24), -4), (dict(n=0), 0), (dict(out=0), -4), (dict(codes=4104), -4), (dict(head_dim=40), -4), (dict(kv_heads=0), -4), (dict(n=1 << 31), -3)):
         assert L.smeg_paged_read_dev(READ_ARGS.pack(*{**read, **kw}.values()), None) == rc
+
+
+def test_keys_of_a_row_at_starts_of_every_size(tmp_path):
+    exe = tmp_path / "paged_rows_check"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-o", str(exe), os.path.join(HERE, "cpp", "paged_rows_check.cc")], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.startswith("ok "), r.stdout + r.stderr
