@@ -295,7 +295,7 @@ int smeg_attn_kv_causal_f16_dev(uint16_t *out, const void *q, int q_f32, size_t 
  * one sequence; pages may be shared by the tables of any number of sequences that only read them. */
 typedef struct smeg_rotate_args {
     const uint16_t *q, *k, *v;          /* q may be NULL; v NULL in smeg_rotate_heads_dev */
-    uint16_t *q_out, *k_out;            /* may be q and k themselves; k_out may be NULL in smeg_paged_append_dev */
+    uint16_t *q_out, *k_out;            /* q and k themselves, or memory that no other rows of the call share; k_out may be NULL in smeg_paged_append_dev */
     size_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
     const float *q_norm, *k_norm;       /* head_dim weights of the heads' RMS norms, or NULL */
     const double *turns;                /* turns per position (frequency / 2 pi) of the rot / 2 rotated pairs, or NULL: no rotation */

@@ -17,6 +17,7 @@
 
 #include "../../include/smeg_api.h"
 #include "kernels.h"
+#include "rows.h"
 #include "layout.h"
 #include "handles.h"
 #include "pack.h"
@@ -1341,6 +1342,13 @@ static int rotate_dev(const smeg_rotate_args* b, bool paged, cudaStream_t stream
         if (b->seqs == 0) return 0;
         if (too_long(b->rows, b->kv_heads, b->kv_heads, b->seqs, b->table_cols, b->page, b->pages)) return -3;
     }
+    // an output is its own input, or shares nothing with any
+    const size_t q_len = b->heads * hd, kv_len = b->kv_heads * hd;
+    const RowsAt q = {b->q, b->q_stride, q_len}, k = {b->k, b->k_stride, kv_len}, v = {paged ? b->v : nullptr, b->v_stride, kv_len}, qo = {b->q ? b->q_out : nullptr, b->q_out_stride, q_len},
+                 ko = {b->k ? b->k_out : nullptr, b->k_out_stride, kv_len};
+    if ((!same_rows(q, qo, b->rows) && rows_share(q, qo, b->rows)) || (!same_rows(k, ko, b->rows) && rows_share(k, ko, b->rows)) || rows_share(qo, k, b->rows) ||
+        rows_share(qo, ko, b->rows) || rows_share(ko, q, b->rows) || rows_share(qo, v, b->rows) || rows_share(ko, v, b->rows))
+        return -4;
     DeviceState* ds = dev_state();
     if (!ds) return -5;
     RotateArgs a;
@@ -1399,6 +1407,8 @@ int smeg_paged_attend_dev(const smeg_paged_attend_args* b, void* stream) {
     if (!b->q || !b->out || !b->codes || !b->scales || !b->cu_rows || !b->starts || !b->table || ((uintptr_t)b->codes & 15) != 0 || ((uintptr_t)b->scales & 7) != 0) return -4;
     if (b->q_stride < b->heads * b->head_dim || b->out_stride < b->heads * b->head_dim) return -4;
     if (too_long(b->rows, b->heads, b->kv_heads, b->seqs, b->table_cols, b->page, b->pages) || b->pages == 0) return -3;
+    const size_t q_len = b->heads * b->head_dim;
+    if (rows_share({b->out, b->out_stride, q_len}, {b->q, b->q_stride, q_len}, b->rows)) return -4;
     DeviceState* ds = dev_state();
     if (!ds) return -5;
     PagedAttendArgs a;
@@ -1419,6 +1429,8 @@ int smeg_attn_packed_dev(const smeg_attn_packed_args* b, void* stream) {
     if (!heads_ok(b->heads, b->kv_heads, b->head_dim, 8) || !b->q || !b->k || !b->v || !b->out || !b->cu_rows) return -4;
     if (b->q_stride < q_len || b->out_stride < q_len || b->k_stride < kv_len || b->v_stride < kv_len) return -4;
     if (too_long(b->rows, b->heads, b->kv_heads, b->seqs, 0, 16, 0)) return -3;
+    const RowsAt out = {b->out, b->out_stride, q_len};
+    if (rows_share(out, {b->q, b->q_stride, q_len}, b->rows) || rows_share(out, {b->k, b->k_stride, kv_len}, b->rows) || rows_share(out, {b->v, b->v_stride, kv_len}, b->rows)) return -4;
     DeviceState* ds = dev_state();
     if (!ds) return -5;
     PromptArgs a;

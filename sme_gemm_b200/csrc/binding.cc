@@ -16,6 +16,7 @@
 #include <cstring>
 
 #include "../../include/smeg_api.h"
+#include "rows.h"
 
 namespace {
 
@@ -72,6 +73,24 @@ uint16_t* rows_of(PyObject* x, const char* what, int64_t width, const Rows& like
     require(like.rows == 0 || ((one == 1 || width == 1) && (like.rows == 1 || s >= width)), what, " has its rows' values side by side");
     *stride = (size_t)(s >= width ? s : width);
     return static_cast<uint16_t*>(t.data_ptr());
+}
+// An output of rows may be the input that it comes from (own), and shares no memory with the others.
+void apart(const smeg::RowsAt& out, const smeg::RowsAt& in, const Rows& like, const char* what, const char* from, bool own) {
+    if ((own && smeg::same_rows(out, in, (size_t)like.rows)) || !smeg::rows_share(out, in, (size_t)like.rows)) return;
+    PyErr_Format(PyExc_AssertionError, own ? "%s is %s, or shares no memory with it" : "%s shares no memory with %s", what, from);
+    throw Refused();
+}
+// q_out and k_out of a rotation or an append.
+void turned_apart(const smeg_rotate_args& a, const Rows& like) {
+    const size_t q_len = a.heads * a.head_dim, kv_len = a.kv_heads * a.head_dim;
+    const smeg::RowsAt q = {a.q, a.q_stride, q_len}, k = {a.k, a.k_stride, kv_len}, v = {a.v, a.v_stride, kv_len}, qo = {a.q_out, a.q_out_stride, q_len}, ko = {a.k_out, a.k_out_stride, kv_len};
+    apart(qo, q, like, "q_out", "q", true);
+    apart(ko, k, like, "k_out", "k", true);
+    apart(qo, k, like, "q_out", "k", false);
+    apart(qo, v, like, "q_out", "v", false);
+    apart(ko, q, like, "k_out", "q", false);
+    apart(ko, v, like, "k_out", "v", false);
+    apart(qo, ko, like, "q_out", "k_out", false);
 }
 const int32_t* ints(PyObject* x, const char* what, int device, int64_t* n) {
     const at::Tensor& t = tensor(x, what, " is a contiguous int32 CUDA tensor");
@@ -215,6 +234,7 @@ PyObject* rotate(PyObject*, PyObject* const* v, Py_ssize_t n) {
         a.bf16 = like.bf16();
         a.rows = (size_t)like.rows;
         a.head_dim = (size_t)hd;
+        turned_apart(a, like);
         if (like.rows == 0) return 0;
         On on(like.device);
         return f_rotate(&a, on.raw());
@@ -258,6 +278,7 @@ PyObject* append(PyObject*, PyObject* const* v, Py_ssize_t n) {
         a.scales = ptr_at<float>(cache, 1);
         a.pages = at(cache, 2);
         a.page = at(cache, 3);
+        turned_apart(a, like);
         if (like.rows == 0 || a.seqs == 0) return 0;
         On on(like.device);
         return f_append(&a, on.raw());
@@ -279,6 +300,7 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
         const int64_t width = (int64_t)(a.heads * a.head_dim);
         a.q = rows_of(v[0], "q", width, like, &a.q_stride);
         a.out = rows_of(v[1], "out", width, like, &a.out_stride);
+        apart({a.out, a.out_stride, (size_t)width}, {a.q, a.q_stride, (size_t)width}, like, "out", "q", false);
         a.codes = ptr_at<const uint8_t>(cache, 0);
         a.scales = ptr_at<const float>(cache, 1);
         a.pages = at(cache, 2);
@@ -348,7 +370,9 @@ PyObject* packed(PyObject*, PyObject* const* v, Py_ssize_t n) {
         a.k = rows_of(v[1], "k", row, like, &a.k_stride);
         a.v = rows_of(v[2], "v", row, like, &a.v_stride);
         a.out = rows_of(v[4], "out", width, like, &a.out_stride);
-        require(like.rows == 0 || (a.out != a.q && a.out != a.k && a.out != a.v), "out", " is none of the inputs");
+        const smeg::RowsAt out = {a.out, a.out_stride, (size_t)width};
+        for (const smeg::RowsAt& in : {smeg::RowsAt{a.q, a.q_stride, (size_t)width}, smeg::RowsAt{a.k, a.k_stride, (size_t)row}, smeg::RowsAt{a.v, a.v_stride, (size_t)row}})
+            require(!smeg::rows_share(out, in, (size_t)like.rows), "out", " is none of the inputs, and shares no memory with them");
         int64_t count;
         a.cu_rows = ints(v[3], "cu_rows", like.device, &count);
         require(count >= 1, "", "cu_rows has one value more than there are sequences");

@@ -139,8 +139,8 @@ def _rotation(rotary, head_dim: int):
 
 def rotate_heads(q, k, positions, rotary, q_out, k_out, *, q_norm=None, k_norm=None, head_dim: int | None = None) -> None:
     """q_out, k_out = the heads of the rows q and k (either may be None), each normalised (q_norm, k_norm: RMS norms of head_dim weights) and rotated by
-    its row's position, in one pass with one rounding.  positions: an int32 tensor, one a row, or the first row's as a number.  The outputs may be
-    the inputs.  rotary None: the norms alone (head_dim is needed then)."""
+    its row's position, in one pass with one rounding.  positions: an int32 tensor, one a row, or the first row's as a number.  q_out may be
+    q, and k_out k; else the outputs share no memory with one another or the inputs.  rotary None: the norms alone (head_dim is needed then)."""
     assert rotary is not None or head_dim is not None, "without a rotation, head_dim says what a head is"
     hd = rotary._head_dim if rotary is not None else head_dim
     assert head_dim is None or head_dim == hd, "the rotation is one of heads of head_dim"
@@ -249,8 +249,8 @@ class PagedKvCache:
 
     def append(self, k, v, batch: PagedBatch, rotary: Rotary | None = None, *, k_norm=None, k_out=None, q=None, q_out=None, q_norm=None) -> None:
         """The rows k and v (kv_heads * head_dim values) to the pages of their sequences' positions; keys are normalised (k_norm) and rotated on the way.
-        k_out: the keys so treated as 16-bit rows as well.  q, q_out: the queries, normalised (q_norm) and rotated, in the same pass.  The outputs
-        may be the inputs.  Rows of idle sequences and rows behind the last sequence are left as they are."""
+        k_out: the keys so treated as 16-bit rows as well.  q, q_out: the queries, normalised (q_norm) and rotated, in the same pass.  q_out
+        may be q, and k_out k; else they share no memory with one another or the inputs.  Rows of idle sequences and rows behind the last sequence are left as they are."""
         assert isinstance(batch, PagedBatch), "batch is a PagedBatch"
         args = (k, v, k_out, q, q_out, *_head_norm(q_norm, "q_norm"), *_head_norm(k_norm, "k_norm"), _rotation(rotary, self._head_dim), batch._fields, self._fields)
         rc = (_CALLS or _calls()).append(*args)

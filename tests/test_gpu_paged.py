@@ -990,3 +990,26 @@ def test_rows_behind_the_table_attend_to_what_it_has_room_for(cols, seqs):
         _near(out, want, tol, F16)
     pool.cache.attend(q, pool.batch([2] * seqs, starts=[room - 2] * seqs), out)
     assert sg.last_status() == 0
+
+
+def test_outputs_that_share_memory_with_other_rows():
+    """Refused; slices of the same rows side by side, and an output in its own input's place, are not."""
+    cache = sg.PagedKvCache(4, 2, 32, 5, 16)
+    batch = sg.PagedBatch(_int([0, 4]), _int([0]), _int([[0, 1]]))
+    x = torch.zeros(9, 320, dtype=F16, device="cuda")             # [q | k | v | 64 more]
+    q, k, v = x[:4, :128], x[:4, 128:192], x[:4, 192:256]
+    turn, cu = sg.Rotary(32), _int([0, 4])
+    for bad in (lambda: sg.rotate_heads(q, k, 0, turn, x[1:5, :128], k), lambda: sg.rotate_heads(q, k, 0, turn, x[:4, 64:192], k), lambda: sg.rotate_heads(q, k, 0, turn, q, x[:4, 96:160]),
+                lambda: sg.rotate_heads(q, k, 0, turn, x[:8].view(4, 640)[:, :128], k), lambda: sg.rotate_heads(k, v, 0, turn, v, k),
+                lambda: cache.append(k, v, batch, turn, k_out=v), lambda: cache.append(k, v, batch, turn, k_out=k, q=q, q_out=x[:4, 192:320]),
+                lambda: cache.append(k, v, batch, turn, k_out=x[:4, 100:164]), lambda: cache.attend(q, batch, q), lambda: cache.attend(q, batch, x[3:7, :128]),
+                lambda: sg.attend_packed(q, k, v, cu, x[:4, 192:320], 4, 2), lambda: sg.attend_packed(q, k, v, cu, x[:4, 8:136], 4, 2)):
+        with pytest.raises(AssertionError, match="no memory with"):
+            bad()
+    sg.rotate_heads(q, k, 0, turn, q, k)
+    sg.rotate_heads(q, None, 0, turn, x[4:8, :128], None)
+    cache.append(k, v, batch, turn, k_out=k, q=q, q_out=q)
+    cache.append(k, v, batch, turn, k_out=x[:4, 256:])
+    cache.attend(q, batch, x[5:9, 192:])
+    cache.attend(q, batch, x[:4, 192:])                           # (beside q in the same rows)
+    sg.attend_packed(q, k, v, cu, x[4:8, 128:256], 4, 2)

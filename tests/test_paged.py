@@ -136,3 +136,45 @@ def test_keys_of_a_row_at_starts_of_every_size(tmp_path):
     subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-o", str(exe), os.path.join(HERE, "cpp", "paged_rows_check.cc")], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and r.stdout.startswith("ok "), r.stdout + r.stderr
+
+
+def test_rows_that_share_memory_are_told_from_rows_side_by_side(tmp_path):
+    exe = tmp_path / "rows_share_check"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-o", str(exe), os.path.join(HERE, "cpp", "rows_share_check.cc")], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.startswith("ok "), r.stdout + r.stderr
+    assert all(int(x) > 10000 for x in r.stdout.split()[1:])
+
+
+M = 1 << 20                                                   # rows that share nothing
+ROWS = dict(q=M, k=2 * M, v=3 * M, q_out=4 * M, k_out=5 * M, rows=4, q_stride=256, k_stride=128, v_stride=128, q_out_stride=256, k_out_stride=128)
+
+
+@pytest.mark.parametrize("kw", [dict(q_out=M + 2), dict(q_out=M, q_out_stride=264), dict(k_out=2 * M - 254), dict(q_out=2 * M + 256), dict(k_out=M + 512), dict(k_out=4 * M + 1024), dict(q_out=2 * M),
+                                dict(q=M, k=M + 512, q_stride=512, k_stride=512, q_out=M + 256, q_out_stride=512)])
+def test_outputs_that_share_memory_with_other_rows_are_refused(kw):
+    L = sg.lib()
+    assert L.smeg_rotate_heads_dev(_rotate(**{**ROWS, **kw}), None) == -4
+    assert L.smeg_paged_append_dev(_paged(**{**ROWS, **kw}), None) == -4
+
+
+def test_outputs_in_place_and_side_by_side_are_not_refused():
+    """Past the checks, which without a GPU ends at the device (-5)."""
+    if torch.cuda.is_available():
+        pytest.skip("would run on made-up addresses")
+    L = sg.lib()
+    wide = dict(q_stride=512, k_stride=512, v_stride=512, q_out_stride=512, k_out_stride=512)
+    for kw in (dict(), dict(q_out=M, k_out=2 * M), {**wide, **dict(q=M, k=M + 512, v=M + 768, q_out=M, k_out=M + 512)}, {**wide, **dict(q=M, k=M + 512, v=M + 768, q_out=2 * M, k_out=2 * M + 512)}):
+        assert L.smeg_rotate_heads_dev(_rotate(**{**ROWS, **kw}), None) == -5
+        assert L.smeg_paged_append_dev(_paged(**{**ROWS, **kw}), None) == -5
+    for kw in (dict(v=M + 512, **wide), dict(k_out=3 * M), dict(q_out=3 * M + 4)):
+        assert L.smeg_paged_append_dev(_paged(**{**ROWS, **{**dict(q=M, q_out=M), **kw}}), None) == (-5 if "q_stride" in kw else -4)
+    a = dict(q=M, out=M + 256, q_stride=256, out_stride=256, codes=4096, scales=4096, cu=4096, starts=4096, table=4096, seqs=2, cols=3, pages=5, page=64, rows=2,
+             heads=2, kv_heads=2, head_dim=64, scale=0.125, bf16=0, ws=0, bytes=0)
+    assert L.smeg_paged_attend_dev(PAGED_ATTEND_ARGS.pack(*a.values()), None) == -5
+    for at in (M, M + 2, M + 254, M - 2, M + 512):
+        assert L.smeg_paged_attend_dev(PAGED_ATTEND_ARGS.pack(*{**a, "out": at}.values()), None) == -4
+    a = dict(q=M, k=M + 512, v=M + 768, out=2 * M, q_stride=512, k_stride=512, v_stride=512, out_stride=256, cu=4096, seqs=1, rows=2, heads=4, kv_heads=2, head_dim=64, scale=0.125, bf16=0)
+    assert L.smeg_attn_packed_dev(ATTN_PACKED_ARGS.pack(*a.values()), None) == -5
+    for at in (M, M + 512, M + 1022, M + 1024 + 768 + 254):
+        assert L.smeg_attn_packed_dev(ATTN_PACKED_ARGS.pack(*{**a, "out": at}.values()), None) == -4
