@@ -67,6 +67,13 @@ class Rotary:
         self._turns = {}                                       # device -> turns per position, and where they are
         self._call = self._turns, self._rot, self._interleaved, self._factor
 
+    def __getstate__(self):                                    # a copy, or one of another process, has tables of its own
+        return self._head_dim, self._rot, self._base, self._interleaved, self._frequencies, self._factor
+
+    def __setstate__(self, state) -> None:
+        self._head_dim, self._rot, self._base, self._interleaved, frequencies, factor = state
+        self._set(frequencies, factor)
+
     def _scaled(self, frequencies, factor: float = 1.0) -> "Rotary":
         r = Rotary(self._head_dim, self._base, self._rot, self._interleaved)
         r._set(frequencies, self._factor * factor)
@@ -171,6 +178,12 @@ class PagedBatch:
         self._device = starts.get_device()
         self._fields = cu_rows.data_ptr(), starts.data_ptr(), table.data_ptr(), n, table.shape[1], self._device
 
+    def __getstate__(self):                                    # (the addresses are the tensors', which a copy has its own of)
+        return self._tensors
+
+    def __setstate__(self, tensors) -> None:
+        self.__init__(*tensors)
+
     @property
     def cu_rows(self):
         return self._tensors[0]
@@ -205,6 +218,14 @@ class PagedKvCache:
         self._scales = torch.zeros((pages, kv_heads, 2), dtype=torch.float32, device=device)
         self._device = self._codes.get_device()
         self._set_scale(1.0 / np.sqrt(np.float32(head_dim)))
+
+    def __getstate__(self):                                    # (as PagedBatch)
+        return {name: x for name, x in self.__dict__.items() if name not in ("_device", "_fields")}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        self._device = self._codes.get_device()
+        self._set_scale(self._scale)
 
     def _set_scale(self, scale: float) -> None:
         self._scale = float(np.float32(scale))

@@ -1013,3 +1013,29 @@ def test_outputs_that_share_memory_with_other_rows():
     cache.attend(q, batch, x[5:9, 192:])
     cache.attend(q, batch, x[:4, 192:])                           # (beside q in the same rows)
     sg.attend_packed(q, k, v, cu, x[4:8, 128:256], 4, 2)
+
+
+def test_copies_of_caches_batches_and_rotations_stand_by_themselves():
+    import copy
+    pool = Pool(4, 2, 64, 16, 2, 4, seed=61)
+    rotary = sg.Rotary(64)
+    pool.append([20, 5], rotary=rotary)
+    cache, other, turn = pool.cache.with_scale(0.2), copy.deepcopy(pool.cache), copy.deepcopy(rotary)
+    x = _randn(pool.gen, 2, 2 * 128)
+    k, v = x.split([128, 128], 1)
+    batch = pool.batch([1, 1])
+    twin = copy.deepcopy(batch)
+    before = cache.codes.clone()
+    other.append(k, v, twin, turn)
+    assert torch.equal(cache.codes, before) and not torch.equal(other.codes, before) and other.scale() == cache.scale()
+    cache.append(k, v, batch, rotary)
+    assert torch.equal(cache.codes, other.codes) and torch.equal(cache.scales, other.scales)
+    twin.starts.fill_(-1)                                        # the copy's own
+    q = _randn(pool.gen, 2, 256)
+    out, idle = torch.empty_like(q), torch.full_like(q, 3.0)
+    cache.attend(q, batch, out)
+    other.attend(q, twin, idle)
+    assert out.any(1).all() and not idle.any()
+    again = torch.empty_like(q)
+    other.attend(q, batch, again)
+    assert torch.equal(again, out)

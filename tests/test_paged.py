@@ -178,3 +178,15 @@ def test_outputs_in_place_and_side_by_side_are_not_refused():
     assert L.smeg_attn_packed_dev(ATTN_PACKED_ARGS.pack(*a.values()), None) == -5
     for at in (M, M + 512, M + 1022, M + 1024 + 768 + 254):
         assert L.smeg_attn_packed_dev(ATTN_PACKED_ARGS.pack(*{**a, "out": at}.values()), None) == -4
+
+
+def test_a_copied_rotation_has_no_addresses_of_the_first_one():
+    import copy
+    import pickle
+    r = sg.Rotary(64, base=500.0, rotary_dim=32, interleaved=True).yarn(8.0, 4096)
+    r._turns[0] = (4096, 8192, None, None)                    # as a call on device 0 leaves it
+    for c in (copy.copy(r), copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert c._turns == {} and c._call[0] is c._turns and c._call[1:] == r._call[1:]
+        assert np.array_equal(c.frequencies(), r.frequencies()) and c.factor() == r.factor()
+        assert (c.head_dim(), c.rotary_dim(), c.interleaved()) == (64, 32, True)
+        assert np.array_equal(c.linear(2.0).frequencies(), r.linear(2.0).frequencies())
