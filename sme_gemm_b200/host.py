@@ -1125,8 +1125,13 @@ class SelfAttention:
         assert qkv.n() == (heads + 2 * kv_heads) * head_dim, "qkv has (heads + 2 * kv_heads) * head_dim outputs"
         assert out.k() == heads * head_dim, "out takes heads * head_dim inputs"
         self.qkv, self.out, self._heads, self._kv_heads, self._head_dim = qkv, out, heads, kv_heads, head_dim
-        self.rotary = self.q_norm = self.k_norm = None
+        self._rotary = self._q_norm = self._k_norm = None
         self._turns = False                                  # rotated or normalised heads
+
+    # what with_rotary has set, and nothing else does: an assignment would leave the heads as they are
+    rotary = property(lambda self: self._rotary, doc="The heads' rotation, or None (with_rotary).")
+    q_norm = property(lambda self: self._q_norm, doc="The query heads' norm, or None (with_rotary).")
+    k_norm = property(lambda self: self._k_norm, doc="The key heads' norm, or None (with_rotary).")
 
     def with_rotary(self, rotary, q_norm=None, k_norm=None) -> "SelfAttention":
         """The queries and keys of the block normalised per head (q_norm, k_norm: RMS norms of head_dim weights, or None) and rotated by
@@ -1134,7 +1139,7 @@ class SelfAttention:
         assert rotary is None or (isinstance(rotary, _paged.Rotary) and rotary.head_dim() == self._head_dim), "the rotation is one of heads of head_dim"
         for norm in (q_norm, k_norm):
             assert norm is None or (norm.is_rms and norm.width() == self._head_dim), "the heads' norms are RMS norms of head_dim weights"
-        self.rotary, self.q_norm, self.k_norm = rotary, q_norm, k_norm
+        self._rotary, self._q_norm, self._k_norm = rotary, q_norm, k_norm
         self._turns = any(x is not None for x in (rotary, q_norm, k_norm))
         return self
 

@@ -190,3 +190,18 @@ def test_a_copied_rotation_has_no_addresses_of_the_first_one():
         assert np.array_equal(c.frequencies(), r.frequencies()) and c.factor() == r.factor()
         assert (c.head_dim(), c.rotary_dim(), c.interleaved()) == (64, 32, True)
         assert np.array_equal(c.linear(2.0).frequencies(), r.linear(2.0).frequencies())
+
+
+def test_a_blocks_rotation_is_set_by_with_rotary_alone():
+    class Part:                                               # as wide as a projection, without weights
+        def __init__(self, n, k):
+            self.n, self.k = (lambda: n), (lambda: k)
+
+    attn = sg.SelfAttention(Part(8 * 64, 256), Part(256, 4 * 64), 4, 2, 64)
+    assert attn.rotary is None and attn.q_norm is None and attn.k_norm is None and not attn._turns
+    for name in ("rotary", "q_norm", "k_norm"):
+        with pytest.raises(AttributeError):
+            setattr(attn, name, sg.Rotary(64))
+    r = sg.Rotary(64)
+    assert attn.with_rotary(r) is attn and attn.rotary is r and attn._turns
+    assert not attn.with_rotary(None)._turns and attn.rotary is None
