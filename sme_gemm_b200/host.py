@@ -1186,9 +1186,9 @@ class SelfAttention:
         return _paged.PagedKvCache(self._heads, self._kv_heads, self._head_dim, pages, page)
 
     def attend_batch(self, x, cache, batch, m: int, fresh: bool = False):
-        """attend() for the m packed rows of a PagedBatch against a PagedKvCache: their heads normalised and rotated at the sequences' positions, keys and
-        values appended to the pages.  fresh: every sequence starts at position 0, so that the rows attend to one another's 16-bit keys and
-        values and not to the codes.  Rows behind the last sequence come out as zeros."""
+        """attend() for the m packed f16 rows of a PagedBatch against a PagedKvCache: their heads normalised and rotated at the sequences' positions, keys and
+        values appended to the pages.  fresh: every sequence starts at position 0 and none is idle, so that the rows attend to one another's 16-bit
+        keys and values and not to the codes.  Rows behind the last sequence come out as zeros."""
         assert _is_torch(x) and x.dtype == torch.float16 and _numel(x) == m * self.width(), "x is m * width"
         assert cache.heads() == self._heads and cache.kv_heads() == self._kv_heads and cache.head_dim() == self._head_dim, \
             "the cache's heads match the block's"
@@ -1287,9 +1287,11 @@ class Block:
         self.mlp.accumulate(h, x, rows)
 
     def accumulate_batch(self, x, cache, batch, rows: int, fresh: bool = False) -> None:
-        """accumulate for the packed rows of a PagedBatch against a PagedKvCache (SelfAttention.accumulate_batch)."""
+        """accumulate for the packed rows of a PagedBatch against a PagedKvCache (SelfAttention.accumulate_batch; heads sharded over ranks have no
+        form of it)."""
         assert _is_torch(x) and x.dtype == torch.float32 and x.numel() == rows * self.width(), "x is rows * width"
         assert self.attn is not None, "this block was built without its attention half"
+        assert hasattr(self.attn, "accumulate_batch"), f"{type(self.attn).__name__} has no packed batches"
         h = torch.empty((rows, self.width()), dtype=torch.float16, device=x.device)
         self.norm1.forward(x, h)
         self.attn.accumulate_batch(h, cache, batch, x, rows, fresh)

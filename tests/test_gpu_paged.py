@@ -1039,3 +1039,16 @@ def test_copies_of_caches_batches_and_rotations_stand_by_themselves():
     again = torch.empty_like(q)
     other.attend(q, batch, again)
     assert torch.equal(again, out)
+
+
+def test_a_layer_over_sharded_heads_has_no_packed_batches():
+    from sme_gemm_b200.tp import TpSelfAttention
+    gen = _gen(71)
+    block = _layer(gen, 256, 4, 2, 64, sg.Rotary(64), True)
+    cache, batch = block.attn.paged_cache(8, 16), sg.PagedBatch(_int([0, 3]), _int([0]), _int([[0, 1]]))
+    sharded = sg.Block.new(block.norm1, TpSelfAttention(block.attn, 1), block.norm2, block.mlp)
+    x = torch.randn(3, 256, generator=gen, device="cuda")
+    y = x.clone()
+    with pytest.raises(AssertionError, match="TpSelfAttention has no packed batches"):
+        sharded.accumulate_batch(x, cache, batch, 3, True)
+    assert torch.equal(x, y)
