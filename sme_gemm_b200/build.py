@@ -63,27 +63,42 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
-def build_binding(force: bool = False, verbose: bool = False) -> str:
-    """The Python module behind paged.py (csrc/binding.cc): links against torch, takes the library's entry points by address."""
+def _binding_command(torch):
     import sysconfig
 
-    import torch                                               # (the one its headers belong to; it needs no GPU)
-    src = os.path.join(CSRC, "binding.cc")
-    api = os.path.join(os.path.dirname(HERE), "include", "smeg_api.h")
     out = os.path.join(HERE, "_binding" + sysconfig.get_config_var("EXT_SUFFIX"))
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(api)):
-        return out
     root = os.path.dirname(torch.__file__)
     inc = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
     libs = os.path.join(root, "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-           *[x for i in inc for x in ("-isystem", i)], src, "-o", out, f"-L{libs}", f"-Wl,-rpath,{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    return out, ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+                 *[x for i in inc for x in ("-isystem", i)], os.path.join(CSRC, "binding.cc"), "-o", out, f"-L{libs}", f"-Wl,-rpath,{libs}", "-ltorch_python", "-ltorch_cpu",
+                 "-lc10", "-lc10_cuda"]
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str | None:
+    """The Python module behind paged.py (csrc/binding.cc): links against torch, takes the library's entry points by address.  It belongs to one torch:
+    another version, place or ABI of it builds the module again.  None without torch, which the library does not need."""
+    try:
+        import torch                                           # (the one its headers belong to; it needs no GPU)
+    except ImportError:
+        sys.stderr.write("torch is not installed: the calls on packed batches (paged.py) are left out\n")
+        return None
+    out, cmd = _binding_command(torch)
+    key = "\n".join([str(torch.__version__), *cmd]) + "\n"
+    stamp = os.path.join(HERE, "_binding.stamp")
+    sources = [os.path.join(CSRC, "binding.cc"), os.path.join(CSRC, "rows.h"), os.path.join(os.path.dirname(HERE), "include", "smeg_api.h")]
+    if not force and os.path.exists(out) and os.path.exists(stamp) and os.path.getmtime(out) >= max(map(os.path.getmtime, sources)):
+        with open(stamp) as f:
+            if f.read() == key:
+                return out
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or r.returncode:
         sys.stderr.write(r.stdout)
     if r.returncode:
         raise RuntimeError("g++ failed on binding.cc")
+    with open(stamp, "w") as f:
+        f.write(key)
     return out
 
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import importlib
 import math
+import os
 
 import numpy as np
 
@@ -28,7 +29,9 @@ def _calls():
         try:
             m = importlib.import_module("._binding", __package__)
         except ImportError as e:
-            raise RuntimeError("sme_gemm_b200/_binding is missing: build it with `python -m sme_gemm_b200.build`") from e
+            there = any(f.startswith("_binding.") and f.endswith(".so") for f in os.listdir(os.path.dirname(os.path.abspath(__file__))))
+            what = f"does not load ({e})" if there else "is missing"
+            raise RuntimeError(f"sme_gemm_b200/_binding {what}: build it with `python -m sme_gemm_b200.build`") from e
         m.bind(*(ctypes.cast(getattr(L, "smeg_" + n), ctypes.c_void_p).value for n in (
             "rotate_heads_dev", "paged_append_dev", "paged_attend_dev", "paged_attend_workspace", "attn_packed_dev", "paged_read_dev")))
         _CALLS = m

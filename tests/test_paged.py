@@ -2,6 +2,7 @@
 import math
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -205,3 +206,52 @@ def test_a_blocks_rotation_is_set_by_with_rotary_alone():
     r = sg.Rotary(64)
     assert attn.with_rotary(r) is attn and attn.rotary is r and attn._turns
     assert not attn.with_rotary(None)._turns and attn.rotary is None
+
+
+def test_the_library_builds_without_torch():
+    code = ("import sys; sys.modules['torch'] = None\n"
+            "from sme_gemm_b200 import build\nprint(build.build(), build.build_binding())")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600, cwd=os.path.dirname(HERE))
+    assert r.returncode == 0 and r.stdout.strip().endswith("libsmeg_b200.so None") and "paged.py" in r.stderr, r.stdout + r.stderr
+
+
+def test_the_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    from sme_gemm_b200 import build
+    runs = []
+
+    def run(cmd, **kw):
+        runs.append(cmd)
+        out = cmd[cmd.index("-o") + 1]
+        open(out, "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build, "HERE", str(tmp_path / "pkg"))
+    monkeypatch.setattr(build.subprocess, "run", run)
+    os.makedirs(tmp_path / "pkg")
+    os.makedirs(tmp_path / "include")
+    open(tmp_path / "include" / "smeg_api.h", "w").close()
+    out = build.build_binding()
+    assert len(runs) == 1 and build.build_binding() == out and len(runs) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.other")
+    assert build.build_binding() == out and len(runs) == 2 and build.build_binding() == out and len(runs) == 2
+    monkeypatch.setattr(torch, "compiled_with_cxx11_abi", lambda: not runs)
+    build.build_binding()
+    assert len(runs) == 3
+    os.remove(out)
+    build.build_binding()
+    assert len(runs) == 4
+
+
+def test_a_binding_that_does_not_load_says_why(monkeypatch):
+    from sme_gemm_b200 import paged
+    monkeypatch.setattr(paged, "_CALLS", None)
+
+    def fails(*a):
+        raise ImportError("undefined symbol: of_another_torch")
+
+    monkeypatch.setattr(paged.importlib, "import_module", fails)
+    with pytest.raises(RuntimeError, match="does not load .undefined symbol: of_another_torch.*build it"):
+        paged._calls()
+    monkeypatch.setattr(paged.os, "listdir", lambda d: ["paged.py"])
+    with pytest.raises(RuntimeError, match="_binding is missing: build it"):
+        paged._calls()
