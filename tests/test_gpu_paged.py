@@ -1052,3 +1052,87 @@ def test_a_layer_over_sharded_heads_has_no_packed_batches():
     with pytest.raises(AssertionError, match="TpSelfAttention has no packed batches"):
         sharded.accumulate_batch(x, cache, batch, 3, True)
     assert torch.equal(x, y)
+
+
+# ------------------------------------------------------------------------------------------------ searches of several passes, threads
+
+@pytest.mark.parametrize("seqs,heads,kv,hd,cols,form", [(129, 4, 1, 64, 8, "clusters"), (200, 4, 1, 64, 8, "clusters"), (250, 8, 1, 16, 10, "clusters"), (300, 4, 1, 64, 30, "shares"),
+                                                        (270, 4, 1, 128, 40, "cuts")])
+def test_searches_through_more_sequences_than_threads(seqs, heads, kv, hd, cols, form):
+    """129 and more sequences are several passes of a CTA's search for its item (257 and more of the join's): lengths of every kind, sequences without rows, idle ones."""
+    rng = np.random.default_rng(seqs)
+    page = 64
+    lens = [int(x) for x in rng.integers(1, cols * page + 1, seqs)]
+    pool = Pool(heads, kv, hd, page, seqs, cols, seed=seqs)
+    pool.append(lens)
+    rows = [0 if i % 17 == 3 else 1 for i in range(seqs)]
+    rows[-1] = 1
+    idle = set(range(5, seqs, 23))
+    starts = [-1 if s in idle else n - 1 for s, n in enumerate(lens)]
+    q = _randn(pool.gen, sum(rows) + 1, heads * hd)
+    out = torch.full_like(q, 5.0)
+    pool.cache.attend(q, pool.batch(rows, starts=starts), out)
+    want, tol = _attended(pool, q[:-1], rows, starts)
+    _near(out[:-1], want, tol, F16)
+    assert torch.all(out[-1] == 5.0)
+
+
+def test_two_streams_whose_inputs_are_there():
+    """As above, with the streams waiting for the inputs and the outputs against 64 bits."""
+    gen = _gen(43)
+    rows = [300, 400]
+    x = _randn(gen, 700, 48 * 128)
+    q, k, v = x.split([32 * 128, 8 * 128, 8 * 128], 1)
+    cu = _int([0, 300, 700])
+    outs = [torch.full((700, 32 * 128), 7.0, dtype=F16, device="cuda") for _ in range(8)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for i, o in enumerate(outs):
+        with torch.cuda.stream(streams[i % 2]):
+            sg.attend_packed(q, k, v, cu, o, 32, 8)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    _near(outs[0], *_prompt(q, k, v, rows, 32, 8), F16)
+
+
+def test_two_host_threads_on_one_rotation_and_one_cache():
+    """Each thread on a stream, and in sequences, of its own; the rotation's first call on the device is one of theirs."""
+    import threading
+    pool = Pool(8, 2, 64, 16, 2, 12, seed=81)
+    rotary, steps = sg.Rotary(64), 60
+    x = [[_randn(pool.gen, 1, 12 * 64) for _ in range(steps)] for _ in range(2)]
+    want = [[torch.empty(1, 512, dtype=F16, device="cuda") for _ in range(steps)] for _ in range(2)]
+    got = [[torch.full_like(o, 7.0) for o in w] for w in want]
+
+    def serve(cache, turn, t, out, stream):
+        with torch.cuda.stream(stream):
+            for i in range(steps):
+                q, k, v = x[t][i].split([512, 128, 128], 1)
+                batch = batches[t][i]
+                turned = torch.empty_like(q)
+                cache.append(k, v, batch, turn, q=q, q_out=turned)
+                cache.attend(turned, batch, out[t][i])
+
+    batches = [[sg.PagedBatch(_int([0, 1]), _int([i]), pool.table[t:t + 1].contiguous()) for i in range(steps)] for t in range(2)]
+    for t in range(2):
+        serve(pool.cache, sg.Rotary(64), t, want, torch.cuda.current_stream())
+    codes = pool.cache.codes.clone()
+    torch.cuda.synchronize()
+    failed = []
+
+    def thread(t):
+        try:
+            serve(pool.cache, rotary, t, got, streams[t])
+        except BaseException as e:                                # noqa: BLE001
+            failed.append(e)
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    threads = [threading.Thread(target=thread, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    assert all(torch.equal(a, b) for t in range(2) for a, b in zip(got[t], want[t])) and torch.equal(codes, pool.cache.codes)
