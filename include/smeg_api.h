@@ -291,7 +291,7 @@ int smeg_attn_kv_causal_f16_dev(uint16_t *out, const void *q, int q_f32, size_t 
  * The cache: codes uint8 [pages][kv_heads][keys, values][page][head_dim], scales f32 [pages][kv_heads][keys, values]; a value is (code - 128) *
  * scale.  page: a power of two in 16..=256; head_dim a multiple of 16 in 16..=256.  Scale = largest magnitude / 127 over the positions that were
  * appended since the page's first one; it starts over with that one and otherwise only grows, and codes that are there are then rounded
- * again.  A block that received a NaN or an infinity has a NaN scale until its page starts over.  A page that is appended to belongs to
+ * again.  (A value within 2^-10 codes of the middle between two may take either: 32-bit products with the scale's reciprocal.)  A block that received a NaN or an infinity has a NaN scale until its page starts over.  A page that is appended to belongs to
  * one sequence; pages may be shared by the tables of any number of sequences that only read them. */
 typedef struct smeg_rotate_args {
     const uint16_t *q, *k, *v;          /* q may be NULL; v NULL in smeg_rotate_heads_dev */
@@ -331,7 +331,8 @@ typedef struct smeg_paged_read_args {
 int smeg_paged_read_dev(const smeg_paged_read_args *a, void *stream);
 
 /* Attention of a batch's rows against the cache, which already holds them: row i of sequence s attends to positions 0..=starts[s] + i; per
- * head softmax(scale * q . k) @ v in 32 bits, one rounding.  Rows of idle sequences become zeros.  Query head h uses KV head h / (heads / kv_heads).
+ * head softmax(scale * q . k) @ v with 32-bit scores and sums; the probabilities are rounded to f16 for the second product (2^-11 of what each adds),
+ * the result once.  Rows of idle sequences become zeros.  Query head h uses KV head h / (heads / kv_heads).
  * scales lies on
  * an 8-byte boundary.  workspace: smeg_paged_attend_workspace(...) bytes of device memory, 16-byte aligned, that nothing else uses until the call has run. */
 typedef struct smeg_paged_attend_args {
@@ -350,7 +351,8 @@ typedef struct smeg_paged_attend_args {
 size_t smeg_paged_attend_workspace(size_t rows, size_t seqs, size_t table_cols, size_t page, size_t heads, size_t kv_heads, size_t head_dim);
 int smeg_paged_attend_dev(const smeg_paged_attend_args *a, void *stream);
 
-/* Causal attention over whole packed prompts, 16-bit keys and values: row i of a sequence attends to the sequence's rows 0..=i.  head_dim a
+/* Causal attention over whole packed prompts, 16-bit keys and values: row i of a sequence attends to the sequence's rows 0..=i.  32-bit scores and sums;
+ * the probabilities are rounded to the rows' type for the second product (half a step of it of what each adds; smeg_attn_kv_causal_dev is closer, 2e-5).  head_dim a
  * multiple of 8 in 8..=256; any strides and starts, the tcgen05 form for rows that start on 16-byte boundaries.  out shares no memory with the
  * inputs (here and in smeg_paged_attend_dev). */
 typedef struct smeg_attn_packed_args {

@@ -21,8 +21,8 @@
 // its maximum when that is 2^8 above it; each 32 keys' sums are folded into 32-bit registers, since the tensor core cuts its sums off.
 //
 // Measured: a long context streams at 6.8 TB/s beside 12 to 15 us that do not depend on its length (launches, the first bytes, the warps' meeting, the join): one token over
-// 131071 positions of 8 KV heads of 128 51.4 us (5.2 TB/s), 64 sequences of 500 to 5000 positions 78 us (4.9 TB/s); 901 positions by clusters 6.9 us.  With several rows of
-// eight query heads each it is bound by the unpacking and the exponentials (64 x 5 rows of 3000 positions, 24 / 3 heads of 64: 79 us).
+// 131071 positions of 8 KV heads of 128 50.7 us (5.3 TB/s), 64 sequences of 500 to 5000 positions 76.5 us (5.0 TB/s); 901 positions by clusters 6.9 us.  With several rows of
+// eight query heads each it is bound by the unpacking and the exponentials (64 x 5 rows of 3000 positions, 24 / 3 heads of 64: 77 us).
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"

@@ -511,7 +511,7 @@ struct PromptItem {
 
 // The grid has a CTA for every work slot, and a CTA that has finished its own takes over the next one that has not been launched: the barriers and the
 // tensor memory are set up once, and the next item's queries and keys are on their way while this one's last blocks are weighed and its results stored.  (A CTA for every
-// item alone: 8192 rows 508 us against 459, eleven prompts of 7001 98 against 84.)
+// item alone, timed in turn with this: 8192 rows 532 us against 490, eleven prompts of 7001 88.7 against 63.9.)
 __device__ __forceinline__ void take_next_cta(uint32_t answer, uint64_t* bar) {
     asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(smem_u32(bar)) : "memory");
 }

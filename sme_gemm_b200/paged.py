@@ -287,7 +287,7 @@ class PagedKvCache:
     def attend(self, q, batch: PagedBatch, out) -> None:
         """out = the attention of the query rows (heads * head_dim values) against their sequences' cached positions, which already hold the rows' own
         (append, then attend, with the same batch): row i of a sequence attends to positions 0..=start + i.  Rows of idle sequences become
-        zeros, rows behind the last sequence stay as they are.  out shares no memory with q."""
+        zeros, rows behind the last sequence stay as they are.  Probabilities are f16 in the product with the values.  out shares no memory with q."""
         assert isinstance(batch, PagedBatch), "batch is a PagedBatch"
         rc = (_CALLS or _calls()).attend(q, out, batch._fields, self._fields)
         if rc:
@@ -303,7 +303,8 @@ class PagedKvCache:
 def attend_packed(q, k, v, cu_rows, out, heads: int, kv_heads: int, scale: float | None = None) -> None:
     """out = causal attention over whole packed prompts: rows cu_rows[s] .. cu_rows[s + 1] (int32 CUDA tensor) are a sequence's, row i of it attends to
     its rows 0..=i.  q, out: rows of heads * head_dim values, k, v of kv_heads * head_dim, f16 or bf16, at any row stride; scale 1 / sqrt(head_dim).
-    Rows behind the last sequence are left as they are.  out shares no memory with the inputs."""
+    Rows behind the last sequence are left as they are.  Probabilities have the rows' type in the product with the values (KvCache's attention is closer).
+    out shares no memory with the inputs."""
     assert kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "heads must be a positive multiple of kv_heads"
     rc = (_CALLS or _calls()).packed(q, k, v, cu_rows, out, heads, kv_heads, scale)
     if rc:
